@@ -641,6 +641,105 @@ int moearc_x_attn_decode_static(moearc_ctx *c, float *out, const float *q, const
                                 unsigned long kv_begin, unsigned long n_kv, unsigned long page_tokens,
                                 float scale, unsigned int kv_type);
 
+/* ---- one paged KV cache for many sequences (kvcache.cu, attn_batch.cu; no counterpart in the
+ * reference, whose engine keeps one sequence) -------------------------------------------------
+ * The caller owns every buffer; this struct (host memory, read during the call) names them. A
+ * sequence is a row: row s holds n_kv[s] tokens, token j in slot j % page_tokens of page
+ * tables[s][j / page_tokens], in every layer's K and V pool ([page][slot][kv_head][head_dim], as
+ * moearc_kv_append). refs[p] counts the rows that hold page p; a page is free when it is 0. Table
+ * entries at and past ceil(n_kv[s] / page_tokens) are MOEARC_X_NO_PAGE. An entry not below n_pages
+ * inside a row is a hole: its tokens do not exist. moearc_x_kv_reset makes the empty cache; the
+ * calls below keep these rules, and tables, n_kv and refs stay on the device throughout.
+ *
+ * Row lists (seqs, src, dst, add, keep) are HOST arrays of at most MOEARC_X_KV_LIST entries,
+ * copied into the launch by value (a captured graph keeps them). What depends on device state is
+ * checked there: a call that cannot be done has no effect at all and raises a bit of *status:
+ * MOEARC_X_KV_FULL (too few free pages), MOEARC_X_KV_LONG (a row past its table), MOEARC_X_KV_TAKEN
+ * (a fork onto a row that holds tokens). New pages are the free pages of lowest id, in list order.
+ * All calls are enqueued on the context's stream; the same cache must not be changed from two
+ * streams at once, and calls that may overlap need a work buffer each. */
+#define MOEARC_X_NO_PAGE 0xFFFFFFFFu
+#define MOEARC_X_KV_LIST 1024u
+#define MOEARC_X_KV_LAYERS 128u
+#define MOEARC_X_KV_FULL 1u
+#define MOEARC_X_KV_LONG 2u
+#define MOEARC_X_KV_TAKEN 4u
+typedef struct {
+    void *const *k_pages;      /* HOST arrays of n_layer device pointers; a pool's pages hold */
+    void *const *v_pages;      /* page_tokens x n_kv_heads x head_dim elements each */
+    unsigned int n_layer;      /* <= MOEARC_X_KV_LAYERS */
+    unsigned int n_pages;      /* <= 2^28 */
+    unsigned int page_tokens;  /* any size; max_pages * page_tokens < 2^31 */
+    unsigned int n_kv_heads, head_dim;  /* head_dim <= 1024 */
+    unsigned int kv_type;      /* F32 0, F16 1, BF16 30 */
+    unsigned int max_seq;      /* rows, <= 65536 */
+    unsigned int max_pages;    /* table entries of a row, <= 2^24 */
+    unsigned int *tables;      /* device [max_seq][max_pages] */
+    unsigned int *n_kv;        /* device [max_seq] */
+    unsigned int *refs;        /* device [n_pages] */
+    unsigned int *status;      /* device word */
+    void *work;                /* device, 16-byte aligned; holds nothing between calls */
+    unsigned long work_bytes;  /* >= moearc_x_kv_work_bytes */
+} moearc_x_kv_cache;
+/* Bytes of `work` that the page calls and attention with up to n_heads query heads (0: page calls
+ * only) need; 0 on an unsupported shape. */
+unsigned long moearc_x_kv_work_bytes(moearc_ctx *c, const moearc_x_kv_cache *kv, unsigned int n_heads);
+/* Every row empty, every page free, status 0. The pools are left as they are. */
+int moearc_x_kv_reset(moearc_ctx *c, const moearc_x_kv_cache *kv);
+/* Row seqs[i] gains add[i] tokens (distinct rows): pages for them, n_kv advanced; their K and V are
+ * the caller's to store (moearc_x_attn_decode_batch stores the last). A last page that is only
+ * partly filled and held by other rows too is copied first, so that the row writes on a page of its
+ * own. */
+int moearc_x_kv_grow(moearc_ctx *c, const moearc_x_kv_cache *kv, const unsigned int *seqs, const unsigned int *add,
+                     unsigned int n);
+/* Row dst[i] (empty) becomes row src[i]: full pages are shared, a partly filled last page is copied
+ * in every pool; with deep != 0 every page is copied (a hole's place in list order takes no page).
+ * dst rows are distinct and none of the src rows; a src may repeat. */
+int moearc_x_kv_fork(moearc_ctx *c, const moearc_x_kv_cache *kv, const unsigned int *src, const unsigned int *dst,
+                     unsigned int n, int deep);
+/* Row seqs[i] (distinct rows) is cut to its first keep[i] tokens (keep NULL: to none): the pages
+ * past them are given up, and free once no row holds them. A row no longer than keep[i] is left. */
+int moearc_x_kv_free(moearc_ctx *c, const moearc_x_kv_cache *kv, const unsigned int *seqs, const unsigned int *keep,
+                     unsigned int n);
+/* Moves the pages in use together: with n_live of them, the i-th live page at or past n_live moves, in
+ * every pool, to the i-th free page below it. tables_out, refs_out (each may be the cache's own
+ * array) get the tables and counts that go with the moved pages, *n_live (device word, may be
+ * NULL) their number. The pages moved from keep their contents, so the old tables stay readable
+ * until pages at or past n_live are handed out again. */
+int moearc_x_kv_compact(moearc_ctx *c, const moearc_x_kv_cache *kv, unsigned int *tables_out, unsigned int *refs_out,
+                        unsigned int *n_live);
+/* Waits for the stream, reads and clears *status; -1 on a device failure. */
+int moearc_x_kv_status(moearc_ctx *c, const moearc_x_kv_cache *kv);
+/* Decode attention of one new token for each of n_seq <= MOEARC_X_KV_LIST batch rows, in one layer:
+ * out[i][h] = sum over j of softmax_j(scale q[i][h] . k_j, sinks[h]) v_j over the tokens kv_begin[i]
+ * <= j < n_kv of cache row seqs[i] that exist (holes do not), zeros when none does. f32 out
+ * [n_seq][n_heads][head_dim]; q row i at q + i * q_stride (floats; heads then channels within it,
+ * so q may lie in a fused projection's row). With k_new and v_new (f32, row i at i * new_stride,
+ * [n_kv_heads][head_dim]) the row's last token n_kv - 1 is theirs: rounded to kv_type, stored in
+ * its slot (which no other row may hold: moearc_x_kv_grow sees to that) and attended as stored;
+ * a row without tokens in range stores nothing. seqs: HOST list of distinct rows, or NULL for rows
+ * 0 .. n_seq - 1; kv_begin: device [n_seq] or NULL (0); sinks: device [n_heads] or NULL. Queries,
+ * and keys and values in range, are finite; what lies in pages outside the range may be anything.
+ * Results do not depend on timing: the same call gives the same bits. Enqueues two kernels, no
+ * allocation; lengths and tables are read on the device, so a captured call follows them. */
+int moearc_x_attn_decode_batch(moearc_ctx *c, const moearc_x_kv_cache *kv, unsigned int layer, float *out, const float *q,
+                               unsigned long q_stride, const float *k_new, const float *v_new, unsigned long new_stride,
+                               const unsigned int *seqs, const unsigned int *kv_begin, const float *sinks, unsigned int n_seq,
+                               unsigned int n_heads, float scale);
+
+/* ---- log probabilities (logprobs.cu; no counterpart in the reference) ------------------------
+ * For each of n_rows rows of logits (type F32, F16 or BF16; row i at i * row_stride elements,
+ * n_vocab <= row_stride of them used), with x = scale * logit (scale > 0: one over the temperature):
+ * logprob[i] = log softmax(x)[tokens[i]] (a token id not below n_vocab, as padding, gives 0);
+ * entropy[i] = -sum softmax(x) log softmax(x); top_ids[i][0 .. k-1], top_logprobs[i][..] the k <= 32
+ * largest, largest first, equal values by lowest id. tokens and logprob go together and may be
+ * NULL, as may entropy; top_* only with k = 0. Logits of -inf are tokens with probability 0; a row
+ * of them only has entropy 0 and log probabilities of -inf. A row with a NaN or +inf gives NaN, and
+ * its alternatives rank a NaN with -inf. f32 arithmetic on any type; no allocation; one kernel. */
+int moearc_x_token_logprobs(moearc_ctx *c, const void *logits, unsigned int type, unsigned long row_stride,
+                            unsigned int n_rows, unsigned int n_vocab, float scale, const unsigned int *tokens,
+                            float *logprob, float *entropy, unsigned int k, unsigned int *top_ids, float *top_logprobs);
+
 #ifdef __cplusplus
 }
 #endif

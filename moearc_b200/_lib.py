@@ -167,6 +167,15 @@ SIGNATURES: dict[str, tuple] = {
     "moearc_x_gguf_slice_last": (I, [P, C.c_char_p, C.c_ulonglong, P]),
     "moearc_x_mma_peak": (I, [P, I, I, C.POINTER(C.c_double)]),
     "moearc_x_attn_decode_static": (I, [P, P, P, P, P, P, P, UL, UL, UL, UL, UL, UL, F, U]),
+    "moearc_x_kv_work_bytes": (UL, [P, P, U]),
+    "moearc_x_kv_reset": (I, [P, P]),
+    "moearc_x_kv_grow": (I, [P, P, P, P, U]),
+    "moearc_x_kv_fork": (I, [P, P, P, P, U, I]),
+    "moearc_x_kv_free": (I, [P, P, P, P, U]),
+    "moearc_x_kv_compact": (I, [P, P, P, P, P]),
+    "moearc_x_kv_status": (I, [P, P]),
+    "moearc_x_attn_decode_batch": (I, [P, P, U, P, P, UL, P, P, UL, P, P, P, U, U, F]),
+    "moearc_x_token_logprobs": (I, [P, P, U, UL, U, U, F, P, P, P, U, P, P]),
 }
 
 
@@ -191,6 +200,14 @@ class MoeDesc(C.Structure):
     """moearc_x_moe_desc (include/moearc.h)."""
     _fields_ = [("n_embd", U), ("n_ff", U), ("n_expert", U), ("k", U), ("gating", U), ("act", U),
                 ("alpha", F), ("limit", F), ("wtype", U), ("max_tokens", U)]
+
+
+class KvCacheDesc(C.Structure):
+    """moearc_x_kv_cache (include/moearc.h)."""
+    _fields_ = [("k_pages", C.POINTER(P)), ("v_pages", C.POINTER(P)), ("n_layer", U), ("n_pages", U), ("page_tokens", U),
+                ("n_kv_heads", U), ("head_dim", U), ("kv_type", U), ("max_seq", U), ("max_pages", U), ("tables", P),
+                ("n_kv", P), ("refs", P), ("status", P), ("work", P), ("work_bytes", UL)]
+
 
 _lib: C.CDLL | None = None
 

@@ -1,0 +1,975 @@
+// attn_batch.cu — decode attention of one new token for every row of a ragged batch over the
+// paged cache of kvcache.cu.
+//
+//   out[i, h] = sum_j softmax_j(scale q[i, h] . k_j  [, sink_h]) v_j,   begin_i <= j < n_kv_i,
+//
+// over the keys whose table entry is a page; zeros where there are none. GQA: the `group` query
+// heads of a kv head share its keys. The row's newest token may come with the call (k_new, v_new):
+// it is rounded to the cache's type, attended as such and stored in its slot.
+//
+// The operator reads each live key and value once, 2 n_kv_heads head_dim elements a token, and
+// does 4 group flops for each: it is bound by HBM. So:
+//
+// - Work is split evenly whatever the lengths are. The keys of all rows form one line of tiles; each
+//   CTA of a grid that just fills the GPU takes an equal run of it, found from a prefix sum over the
+//   lengths that every CTA computes. A run that ends inside a row leaves a partial (max, sum,
+//   accumulator) behind, at most two a CTA, and a second kernel joins them in tile order; so
+//   results do not depend on timing, and partials do not grow with the batch.
+// - A warp is one kv head (with up to 8 of its query heads) of the CTA's tile, so that the CTA's
+//   warps together read whole rows of a page; where a model has fewer heads than warps, several
+//   warps share a head, taking alternate tiles. A warp streams its K and V tiles through a ring of
+//   cp.async stages of its own, which runs on across rows: no barrier in the loop, and the next
+//   row's keys are on their way before this row is finished.
+// - 16-bit caches multiply on the tensor cores (mma.sync m16n8k16; the M = 128 of tcgen05 would be
+//   filled to a sixteenth by 8 heads, and the kernel is bound by memory either way). q and the
+//   softmax weights stay f32 in effect: a bf16 cache takes them as three bf16 terms (24 bits),
+//   an f16 cache as two f16 terms (22 bits) of values scaled by a power of two.
+//   A tile's P V is summed from zero and added to the f32 accumulator by an ordinary add: the
+//   tensor core's own accumulation truncates, which a long context would show.
+// - f32 caches, and head sizes without a tensor-core form, take a CUDA-core kernel on the same
+//   line of tiles.
+#include <algorithm>
+#include <cmath>
+#include <type_traits>
+
+#include "kvcache.cuh"
+
+using namespace moearc;
+
+namespace moearc {
+size_t kv_page_work_bytes(unsigned n_pages);
+}
+
+namespace {
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr int MAX_SMEM = 227 * 1024;
+
+struct seq_list {
+    unsigned row[KV_LIST];
+};
+
+struct attn_args {
+    float *out;
+    const float *q, *k_new, *v_new, *sinks;
+    uint8_t *k, *v;  // the layer's pools
+    const unsigned *tables, *n_kv, *begin;
+    size_t q_stride, new_stride, token_bytes, head_bytes;  // bytes: n_kv_heads x head_dim elements, head_dim elements
+    unsigned n_seq, max_pages, n_pages, pt, cap;
+    int listed;  // rows come from the list (else row i is batch row i)
+    int n_heads, group, D, subs;  // subs: virtual heads a kv head (its query heads by GP)
+    int hg, rsplit, nhg;          // virtual heads a CTA, warps a head, head groups
+    int min_tiles;
+    float scale2;  // scale x log2(e): scores are kept in powers of two
+    float *part;   // [CTA][2][hg][GP][D + 2]
+    int *pre;      // [n_seq + 1] tile prefix, [n_seq + 1] = CTAs that work
+};
+
+// The keys [lo, hi) of batch row i in cache row `row`, hi cut to the table.
+__device__ __forceinline__ void span_of(const attn_args &a, const seq_list &L, unsigned i, unsigned &row, unsigned &lo, unsigned &hi) {
+    row = a.listed ? L.row[i] : i;
+    hi = min(a.n_kv[row], a.cap);
+    lo = a.begin ? min(a.begin[i], hi) : 0;
+}
+
+// CTA c's run of the `total` tiles over `ctas` CTAs: the first total % ctas take one more.
+__device__ __forceinline__ long run_start(long total, int ctas, int c) { return total / ctas * c + min((long)c, total % ctas); }
+__device__ __forceinline__ int run_owner(long total, int ctas, long g) {
+    const long b = total / ctas, r = total % ctas;
+    return (int)(g < r * (b + 1) ? g / (b + 1) : r + (g - r * (b + 1)) / b);
+}
+
+__device__ __forceinline__ void cp_async(void *smem, const void *gmem, int bytes, bool valid) {
+    const unsigned s = (unsigned)__cvta_generic_to_shared(smem);
+    if (bytes == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(s), "l"(gmem), "r"(valid ? 16 : 0) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(s), "l"(gmem), "r"(valid ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory"); }
+
+// ---- the tensor-core tile (16-bit caches) -----------------------------------------------------
+
+template <bool BF>
+__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    if constexpr (BF)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], const void *p) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"((unsigned)__cvta_generic_to_shared(p)) : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], const void *p) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"((unsigned)__cvta_generic_to_shared(p)) : "memory");
+}
+
+template <bool BF>
+__device__ __forceinline__ uint16_t to16(float v) {
+    if constexpr (BF) return f32_to_bf16_bits(v);
+    else return __half_as_ushort(__float2half_rn(v));
+}
+template <bool BF>
+__device__ __forceinline__ float from16(uint16_t b) {
+    if constexpr (BF) return bf16_bits_to_f32(b);
+    else return f16_bits_to_f32(b);
+}
+// Two values as packed pairs of 16-bit terms: x = t0 + t1 (+ t2), each term the rounding of what
+// the ones before it leave.
+template <bool BF>
+__device__ __forceinline__ void terms(float x, float y, uint32_t &t0, uint32_t &t1, uint32_t &t2) {
+    const uint16_t x0 = to16<BF>(x), y0 = to16<BF>(y);
+    const float xr = x - from16<BF>(x0), yr = y - from16<BF>(y0);
+    const uint16_t x1 = to16<BF>(xr), y1 = to16<BF>(yr);
+    t0 = x0 | (uint32_t)y0 << 16;
+    t1 = x1 | (uint32_t)y1 << 16;
+    if constexpr (BF) t2 = to16<BF>(xr - from16<BF>(x1)) | (uint32_t)to16<BF>(yr - from16<BF>(y1)) << 16;
+}
+
+template <int D_, bool BF>
+struct mma_tile {
+    static constexpr int KEYS = 16, GP = 8, D = D_, WARPS = D_ > 128 ? 4 : 8, NS = 3;
+    // Rows of a stage: chunk c of row r lies at c ^ (r & 7) where a row is whole 128-byte lines,
+    // else rows are padded by one chunk to an odd number of them, so that the eight rows of an
+    // ldmatrix meet eight different bank groups.
+    static constexpr bool SWZ = D % 64 == 0;
+    static constexpr int CH = D / 8, ROW = SWZ ? D : D + 8;
+    static constexpr int STAGE = 2 * KEYS * ROW * 2;  // bytes: K rows, then V rows
+    static constexpr float PSCALE = BF ? 1.f : 4096.f;  // f16 weights scaled away from subnormals
+
+    uint32_t qa[D / 16][4], ql[BF ? D / 16 : 1][2];
+    float o[D / 8][2], m, l, sc;
+    static __host__ __device__ int stage_bytes(int, int) { return STAGE; }
+    static __host__ __device__ int extra_bytes(int) { return 0; }
+
+    static __device__ __forceinline__ int at(int r, int c) { return r * ROW + (SWZ ? (c ^ (r & 7)) : c) * 8; }
+
+    // Rows 0-7 of the A operand hold the first term of the (up to 8) heads, rows 8-15 the second;
+    // the third, where there is one, is a second A operand with its rows 8-15 zero.
+    __device__ __forceinline__ void init(const float *q, int heads, const attn_args &a, uint8_t *, int lane) {
+        const int hr = lane >> 2, qd = lane & 3;
+        const bool live = hr < heads;
+        const float *p = q + (size_t)(live ? hr : 0) * D;
+        float f = 1.f;
+        if constexpr (!BF) {
+            float mx = 0.f;
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) mx = fmaxf(mx, fabsf(p[16 * kk + 2 * qd + (e & 1) + (e >> 1) * 8]));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            // the largest magnitude to [2^12, 2^13)
+            if (mx > 0.f) f = exp2f((float)min(100, 12 - ilogbf(mx)));
+        }
+        sc = a.scale2 / f;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+            const int c0 = 16 * kk + 2 * qd, c1 = c0 + 8;
+            uint32_t t2 = 0, u2 = 0;
+            terms<BF>(live ? p[c0] * f : 0.f, live ? p[c0 + 1] * f : 0.f, qa[kk][0], qa[kk][1], t2);
+            terms<BF>(live ? p[c1] * f : 0.f, live ? p[c1 + 1] * f : 0.f, qa[kk][2], qa[kk][3], u2);
+            if constexpr (BF) {
+                ql[kk][0] = t2;
+                ql[kk][1] = u2;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = 0.f;
+        m = -INFINITY;
+        l = 0.f;
+    }
+
+    // off: lane r < KEYS holds the byte offset of key r's row in a pool, or -1.
+    static __device__ __forceinline__ void load(uint8_t *stage, const attn_args &a, long long off, int lane) {
+        auto *ks = reinterpret_cast<uint16_t *>(stage), *vs = ks + KEYS * ROW;
+#pragma unroll
+        for (int c = lane; c < KEYS * CH; c += 32) {
+            const int r = c / CH, ch = c % CH;
+            const long long b = __shfl_sync(0xffffffffu, off, r);
+            const size_t src = (b < 0 ? 0 : (size_t)b) + ch * 16;
+            cp_async(ks + at(r, ch), a.k + src, 16, b >= 0);
+            cp_async(vs + at(r, ch), a.v + src, 16, b >= 0);
+        }
+    }
+    // The newest token's row r of the tile, from f32; `dst` >= 0 also stores it in the pools.
+    static __device__ __forceinline__ void put_new(uint8_t *stage, const attn_args &a, int r, const float *kn, const float *vn,
+                                                   long long dst, bool store, int lane) {
+        auto *ks = reinterpret_cast<uint16_t *>(stage), *vs = ks + KEYS * ROW;
+        for (int d = lane; d < D; d += 32) {
+            const uint16_t kb = to16<BF>(kn[d]), vb = to16<BF>(vn[d]);
+            const int i = at(r, d >> 3) + (d & 7);
+            ks[i] = kb;
+            vs[i] = vb;
+            if (store) {
+                reinterpret_cast<uint16_t *>(a.k + dst)[d] = kb;
+                reinterpret_cast<uint16_t *>(a.v + dst)[d] = vb;
+            }
+        }
+        __syncwarp();
+    }
+
+    __device__ __forceinline__ void step(const uint8_t *stage, unsigned live, const attn_args &, uint8_t *, int lane) {
+        const auto *ks = reinterpret_cast<const uint16_t *>(stage), *vs = ks + KEYS * ROW;
+        const int qd = lane & 3, mi = lane >> 3;
+        float c0[2][4] = {}, c1[2][4] = {};
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+            uint32_t b[4];
+            ldsm4(b, ks + at(((mi >> 1) << 3) | (lane & 7), 2 * kk + (mi & 1)));
+            mma<BF>(c0[0], qa[kk][0], qa[kk][1], qa[kk][2], qa[kk][3], b[0], b[1]);
+            mma<BF>(c0[1], qa[kk][0], qa[kk][1], qa[kk][2], qa[kk][3], b[2], b[3]);
+            if constexpr (BF) {
+                mma<BF>(c1[0], ql[kk][0], 0u, ql[kk][1], 0u, b[0], b[1]);
+                mma<BF>(c1[1], ql[kk][0], 0u, ql[kk][1], 0u, b[2], b[3]);
+            }
+        }
+        // scores (in powers of two) of head lane / 4 for keys 2 qd, 2 qd + 1, 8 + 2 qd, 9 + 2 qd
+        float s[4];
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const float x = (c0[n][e] + (BF ? c0[n][e + 2] + c1[n][e] : c0[n][e + 2])) * sc;
+                s[2 * n + e] = live >> (8 * n + 2 * qd + e) & 1 ? x : -INFINITY;
+            }
+        float mt = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+        mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
+        mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 2));
+        const float mn = fmaxf(m, mt);
+        const float base = mn == -INFINITY ? 0.f : mn, corr = exp2f(m - base);
+        float p[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) p[e] = exp2f(s[e] - base);
+        l = l * corr + ((p[0] + p[1]) + (p[2] + p[3]));
+        m = mn;
+        uint32_t a0, a1, a2, a3, b0 = 0, b2 = 0;
+        terms<BF>(p[0] * PSCALE, p[1] * PSCALE, a0, a1, b0);
+        terms<BF>(p[2] * PSCALE, p[3] * PSCALE, a2, a3, b2);
+#pragma unroll
+        for (int dn = 0; dn < D / 16; ++dn) {
+            uint32_t b[4];
+            ldsm4t(b, vs + at(((mi & 1) << 3) | (lane & 7), 2 * dn + (mi >> 1)));
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float c[4] = {};
+                if constexpr (BF) mma<BF>(c, b0, 0u, b2, 0u, b[2 * h], b[2 * h + 1]);
+                mma<BF>(c, a0, a1, a2, a3, b[2 * h], b[2 * h + 1]);
+                o[2 * dn + h][0] = fmaf(o[2 * dn + h][0], corr, c[0] + c[2]);
+                o[2 * dn + h][1] = fmaf(o[2 * dn + h][1], corr, c[1] + c[3]);
+            }
+        }
+    }
+
+    // After the last tile: l summed over the head's lanes, o without its scale.
+    __device__ __forceinline__ void close(int) {
+        l += __shfl_xor_sync(0xffffffffu, l, 1);
+        l += __shfl_xor_sync(0xffffffffu, l, 2);
+        if constexpr (!BF) {
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i) {
+                o[i][0] *= 1.f / PSCALE;
+                o[i][1] *= 1.f / PSCALE;
+            }
+        }
+    }
+    // f(head, d, o, m, l) for every value this lane holds; one(head, m, l) once a head.
+    template <typename F, typename G>
+    __device__ __forceinline__ void each(int lane, const attn_args &, F &&f, G &&one) {
+        const int hr = lane >> 2, qd = lane & 3;
+        one(hr, m, l, qd == 0);
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+            f(hr, 8 * i + 2 * qd, o[i][0]);
+            f(hr, 8 * i + 2 * qd + 1, o[i][1]);
+        }
+    }
+};
+
+// ---- the CUDA-core tile (f32 caches, other head sizes) ----------------------------------------
+//
+// Eight keys a tile. Scores: lane (key, quarter) sums over every fourth group of four channels for
+// all GP heads, and the quarters are added so that each lane ends with GP / 4 heads of its key.
+// Values: a lane owns groups of four channels (lane + 32 i) of all GP heads, the weights come from
+// shared memory.
+
+template <typename T>
+__device__ __forceinline__ float4 four(const T *p) {
+    if constexpr (sizeof(T) == 4) {
+        return *reinterpret_cast<const float4 *>(p);
+    } else {
+        const uint2 u = *reinterpret_cast<const uint2 *>(p);
+        if constexpr (std::is_same<T, __half>::value) {
+            const float2 x = __half22float2(*reinterpret_cast<const __half2 *>(&u.x)), y = __half22float2(*reinterpret_cast<const __half2 *>(&u.y));
+            return make_float4(x.x, x.y, y.x, y.y);
+        } else {
+            return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
+                               __uint_as_float(u.y & 0xffff0000u));
+        }
+    }
+}
+__device__ __forceinline__ void round_to(float v, float &d) { d = v; }
+__device__ __forceinline__ void round_to(float v, __half &d) { d = __float2half_rn(v); }
+__device__ __forceinline__ void round_to(float v, __nv_bfloat16 &d) { d = __float2bfloat16_rn(v); }
+
+template <typename T, int NQ, int GP_>
+struct core_tile {
+    static constexpr int KEYS = 8, GP = GP_, WARPS = 8, NS = 0;  // NS 0: chosen by the shared memory a stage takes
+    float acc[NQ][GP][4], m[GP / 4], l[GP / 4];
+    unsigned heads_;
+
+    // A row in shared memory: an odd number of 16-byte chunks, so that eight keys meet eight bank
+    // groups; its tail past head_dim is zero.
+    static __host__ __device__ int row_bytes(int D) { return (((D * (int)sizeof(T) + 15) / 16) | 1) * 16; }
+    static __host__ __device__ int stage_bytes(int D, int) { return 2 * KEYS * row_bytes(D); }
+    static __host__ __device__ int dpad(int D) { return (D + 3) & ~3; }
+    // per warp beside the stages: q, the tile's weights, the heads' corrections
+    static __host__ __device__ int extra_bytes(int D) { return (GP * dpad(D) + KEYS * GP + GP) * 4; }
+
+    __device__ __forceinline__ void init(const float *q, int heads, const attn_args &a, uint8_t *extra, int lane) {
+        auto *qs = reinterpret_cast<float *>(extra);
+        const int dp = dpad(a.D);
+        __syncwarp();
+        for (int i = lane; i < GP * dp; i += 32) {
+            const int h = i / dp, d = i - h * dp;
+            qs[i] = h < heads && d < a.D ? q[(size_t)h * a.D + d] : 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < NQ; ++i)
+#pragma unroll
+            for (int h = 0; h < GP; ++h) acc[i][h][0] = acc[i][h][1] = acc[i][h][2] = acc[i][h][3] = 0.f;
+#pragma unroll
+        for (int h = 0; h < GP / 4; ++h) {
+            m[h] = -INFINITY;
+            l[h] = 0.f;
+        }
+        __syncwarp();
+    }
+    static __device__ __forceinline__ void load(uint8_t *stage, const attn_args &a, long long off, int lane) {
+        const int rb = row_bytes(a.D), bytes = a.D * (int)sizeof(T);
+        const int align = (int)((reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) | (uintptr_t)bytes) & 15);
+        // rows start where their size and the pools allow: 16- or 4-byte copies, else element by element
+        const int w = align == 0 ? 16 : (align & 3) == 0 ? 4 : 2;
+        for (int r = 0; r < KEYS; ++r) {
+            const long long b = __shfl_sync(0xffffffffu, off, r);
+            const size_t src = b < 0 ? 0 : (size_t)b;
+            uint8_t *kr = stage + r * rb, *vr = stage + (KEYS + r) * rb;
+            if (w > 2) {
+                for (int c = lane * w; c < bytes; c += 32 * w) {
+                    cp_async(kr + c, a.k + src + c, w, b >= 0);
+                    cp_async(vr + c, a.v + src + c, w, b >= 0);
+                }
+            } else {
+                for (int c = lane * 2; c < bytes; c += 64) {
+                    *reinterpret_cast<uint16_t *>(kr + c) = b >= 0 ? *reinterpret_cast<const uint16_t *>(a.k + src + c) : uint16_t(0);
+                    *reinterpret_cast<uint16_t *>(vr + c) = b >= 0 ? *reinterpret_cast<const uint16_t *>(a.v + src + c) : uint16_t(0);
+                }
+            }
+        }
+    }
+    static __device__ __forceinline__ void put_new(uint8_t *stage, const attn_args &a, int r, const float *kn, const float *vn,
+                                                   long long dst, bool store, int lane) {
+        const int rb = row_bytes(a.D);
+        auto *kr = reinterpret_cast<T *>(stage + r * rb), *vr = reinterpret_cast<T *>(stage + (KEYS + r) * rb);
+        for (int d = lane; d < a.D; d += 32) {
+            round_to(kn[d], kr[d]);
+            round_to(vn[d], vr[d]);
+            if (store) {
+                reinterpret_cast<T *>(a.k + dst)[d] = kr[d];
+                reinterpret_cast<T *>(a.v + dst)[d] = vr[d];
+            }
+        }
+        __syncwarp();
+    }
+    __device__ __forceinline__ void step(const uint8_t *stage, unsigned live, const attn_args &a, uint8_t *extra, int lane) {
+        const int D = a.D, dp = dpad(D), rb = row_bytes(D);
+        auto *qs = reinterpret_cast<float *>(extra), *ps = qs + GP * dp, *cs = ps + KEYS * GP;
+        const int key = lane >> 2, cl = lane & 3;
+        const T *kr = reinterpret_cast<const T *>(stage + key * rb);
+        float s[GP];
+#pragma unroll
+        for (int h = 0; h < GP; ++h) s[h] = 0.f;
+        for (int c = 4 * cl; c < dp; c += 16) {
+            const float4 kv = four(kr + c);
+#pragma unroll
+            for (int h = 0; h < GP; ++h) {
+                const float4 qv = *reinterpret_cast<const float4 *>(qs + h * dp + c);
+                s[h] = fmaf(qv.x, kv.x, fmaf(qv.y, kv.y, fmaf(qv.z, kv.z, fmaf(qv.w, kv.w, s[h]))));
+            }
+        }
+        // heads cl GP / 4 + (0 .. GP / 4 - 1) of the key, summed over the quarters
+        float t[GP / 2], x[GP / 4];
+#pragma unroll
+        for (int h = 0; h < GP / 2; ++h) {
+            const float mine = cl & 2 ? s[h + GP / 2] : s[h], other = cl & 2 ? s[h] : s[h + GP / 2];
+            t[h] = mine + __shfl_xor_sync(0xffffffffu, other, 2);
+        }
+#pragma unroll
+        for (int h = 0; h < GP / 4; ++h) {
+            const float mine = cl & 1 ? t[h + GP / 4] : t[h], other = cl & 1 ? t[h] : t[h + GP / 4];
+            x[h] = mine + __shfl_xor_sync(0xffffffffu, other, 1);
+        }
+        const bool in = live >> key & 1;
+#pragma unroll
+        for (int h = 0; h < GP / 4; ++h) {
+            const float sv = in ? x[h] * a.scale2 : -INFINITY;
+            float mt = sv;
+            mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 4));
+            mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 8));
+            mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 16));
+            const float mn = fmaxf(m[h], mt), base = mn == -INFINITY ? 0.f : mn;
+            const float corr = exp2f(m[h] - base), p = exp2f(sv - base);
+            l[h] = l[h] * corr + p;
+            m[h] = mn;
+            ps[key * GP + cl * (GP / 4) + h] = p;
+            if (key == 0) cs[cl * (GP / 4) + h] = corr;
+        }
+        __syncwarp();
+#pragma unroll
+        for (int h = 0; h < GP; ++h) {
+            const float corr = cs[h];
+#pragma unroll
+            for (int i = 0; i < NQ; ++i) {
+                acc[i][h][0] *= corr;
+                acc[i][h][1] *= corr;
+                acc[i][h][2] *= corr;
+                acc[i][h][3] *= corr;
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < KEYS; ++k) {
+            const T *vr = reinterpret_cast<const T *>(stage + (KEYS + k) * rb);
+            float p[GP];
+#pragma unroll
+            for (int h = 0; h < GP; h += 4) {
+                const float4 v = *reinterpret_cast<const float4 *>(ps + k * GP + h);
+                p[h] = v.x;
+                p[h + 1] = v.y;
+                p[h + 2] = v.z;
+                p[h + 3] = v.w;
+            }
+#pragma unroll
+            for (int i = 0; i < NQ; ++i) {
+                const int c = 4 * (lane + 32 * i);
+                if (c < dp) {
+                    const float4 v = four(vr + c);
+#pragma unroll
+                    for (int h = 0; h < GP; ++h) {
+                        acc[i][h][0] = fmaf(p[h], v.x, acc[i][h][0]);
+                        acc[i][h][1] = fmaf(p[h], v.y, acc[i][h][1]);
+                        acc[i][h][2] = fmaf(p[h], v.z, acc[i][h][2]);
+                        acc[i][h][3] = fmaf(p[h], v.w, acc[i][h][3]);
+                    }
+                }
+            }
+        }
+        __syncwarp();
+    }
+    __device__ __forceinline__ void close(int) {
+#pragma unroll
+        for (int h = 0; h < GP / 4; ++h) {
+            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 4);
+            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 8);
+            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 16);
+        }
+    }
+    template <typename F, typename G>
+    __device__ __forceinline__ void each(int lane, const attn_args &a, F &&f, G &&one) {
+#pragma unroll
+        for (int h = 0; h < GP / 4; ++h) one((lane & 3) * (GP / 4) + h, m[h], l[h], lane < 4);
+#pragma unroll
+        for (int i = 0; i < NQ; ++i)
+#pragma unroll
+            for (int h = 0; h < GP; ++h)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int d = 4 * (lane + 32 * i) + e;
+                    if (d < a.D) f(h, d, acc[i][h][e]);
+                }
+    }
+};
+
+// ---- the kernel over the line of tiles --------------------------------------------------------
+
+// Shared memory: the tile prefix, then per warp its stages, then per warp the heads' sums, the
+// stages' live masks and what the tile keeps (q), then the accumulators that warps of one head add.
+struct smem_layout {
+    int ring, warp, warp_bytes, merge, total;
+};
+__host__ __device__ inline smem_layout layout_of(int n_seq, int warps, int ns, int stage, int extra, int gp, int merge_warps, int D) {
+    smem_layout s;
+    s.ring = (((n_seq + 31) & ~31) + 1) * 4 + 127 & ~127;
+    s.warp = s.ring + warps * ns * stage;
+    s.warp_bytes = (3 * gp * 4 + 16 + extra + 15) & ~15;
+    s.merge = s.warp + warps * s.warp_bytes;
+    s.total = s.merge + merge_warps * gp * D * 4;
+    return s;
+}
+
+template <class Tile, int MINB>
+__global__ void __launch_bounds__(Tile::WARPS * 32, MINB)
+    k_attn_batch(const __grid_constant__ attn_args a, const __grid_constant__ seq_list L, int ns) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ int sums[32];
+    constexpr int KEYS = Tile::KEYS, GP = Tile::GP;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    const int D = a.D, HG = a.hg, R = a.rsplit, hs = warp % HG, r = warp / HG;
+    if constexpr (Tile::NS > 0) ns = Tile::NS;
+    const int stage_bytes = Tile::stage_bytes(D, 0);
+    const smem_layout S = layout_of((int)a.n_seq, warps, ns, stage_bytes, Tile::extra_bytes(D), GP, warps - HG, D);
+    int *pre = reinterpret_cast<int *>(smem);
+    uint8_t *ring = smem + S.ring + warp * ns * stage_bytes;
+    auto warp_heads = [&](int w) { return reinterpret_cast<float *>(smem + S.warp + w * S.warp_bytes); };
+    float *hm = warp_heads(warp), *hl = hm + GP, *ff = hl + GP;
+    unsigned *masks = reinterpret_cast<unsigned *>(ff + GP);
+    uint8_t *extra = reinterpret_cast<uint8_t *>(masks + 4);
+    if constexpr (Tile::NS == 0) {  // rows' tails past head_dim stay zero
+        for (int i = threadIdx.x * 16; i < warps * ns * stage_bytes; i += blockDim.x * 16)
+            *reinterpret_cast<uint4 *>(smem + S.ring + i) = make_uint4(0, 0, 0, 0);
+    }
+    pdl_trigger();
+    pdl_wait();
+
+    // The line of tiles: R x KEYS keys each, rows in batch order, the head groups one after another.
+    int run = 0;
+    for (unsigned b = 0; b < a.n_seq; b += blockDim.x) {
+        const unsigned i = b + threadIdx.x;
+        unsigned row, lo = 0, hi = 0;
+        if (i < a.n_seq) span_of(a, L, i, row, lo, hi);
+        int total;
+        const int upto = block_scan((int)((hi - lo + R * KEYS - 1) / (R * KEYS)), sums, &total);
+        if (i < a.n_seq) pre[i + 1] = run + upto;
+        run += total;
+    }
+    if (threadIdx.x == 0) pre[0] = 0;
+    __syncthreads();
+    const long line = run, T = line * a.nhg;
+    const int ctas = (int)min((long)gridDim.x, max(1L, (T + a.min_tiles - 1) / a.min_tiles));
+    if (blockIdx.x == 0)
+        for (unsigned i = threadIdx.x; i < a.n_seq + 2; i += blockDim.x) a.pre[i] = i <= a.n_seq ? pre[i] : ctas;
+    if ((int)blockIdx.x >= ctas || T == 0) return;
+    const long g0 = run_start(T, ctas, (int)blockIdx.x), g1 = run_start(T, ctas, (int)blockIdx.x + 1);
+
+    int s0;
+    {
+        const int x = (int)(g0 % line);
+        int lo = 0, hi = (int)a.n_seq;  // pre[lo] <= x < pre[hi]
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (pre[mid] <= x) lo = mid;
+            else hi = mid;
+        }
+        s0 = lo;
+    }
+    auto next_row = [&](int &s, int &h) {
+        do {
+            if (++s == (int)a.n_seq) {
+                s = 0;
+                ++h;
+            }
+        } while (pre[s + 1] == pre[s]);
+    };
+
+    // The loading side runs ns - 1 tiles ahead of the computing side, across rows.
+    long lg = g0, lend;
+    int ls = s0, lh = (int)(g0 / line), lstage = 0;
+    unsigned lrow, llo, lhi, lslot = 0, lpage = NO_PAGE;
+    const unsigned *ltab;
+    size_t lhead;
+    auto enter = [&]() {
+        span_of(a, L, (unsigned)ls, lrow, llo, lhi);
+        ltab = a.tables + (size_t)lrow * a.max_pages;
+        lhead = (size_t)((lh * HG + hs) / a.subs) * a.head_bytes;
+        lend = lh * line + pre[ls + 1];
+    };
+    // the table entry of the next tile's key, asked for one tile early
+    auto look_up = [&]() {
+        const unsigned t = (unsigned)(lg - lh * line - pre[ls]);
+        const unsigned j = llo + (t * R + r) * KEYS + lane;
+        lpage = NO_PAGE;
+        if (lane < KEYS && j < lhi) {
+            const unsigned e = j / a.pt;
+            lslot = j - e * a.pt;
+            lpage = ltab[e];
+        }
+    };
+    auto issue = [&]() {
+        if (lg < g1) {
+            const bool in = lpage < a.n_pages;
+            const long long off = in ? (long long)(((size_t)lpage * a.pt + lslot) * a.token_bytes + lhead) : -1;
+            const unsigned mask = __ballot_sync(0xffffffffu, in);
+            if (lane == 0) masks[lstage] = mask;
+            Tile::load(ring + lstage * stage_bytes, a, off, lane);
+            lstage = lstage + 1 == ns ? 0 : lstage + 1;
+            if (++lg < g1) {
+                if (lg == lend) {
+                    next_row(ls, lh);
+                    enter();
+                }
+                look_up();
+            }
+        }
+        cp_commit();
+    };
+    enter();
+    look_up();
+    for (int i = 0; i < ns - 1; ++i) issue();
+
+    Tile tile;
+    int s = s0, h = (int)(g0 / line), cstage = 0;
+    for (long g = g0; g < g1; next_row(s, h)) {
+        const long u0 = h * line + pre[s], u1 = h * line + pre[s + 1], first = g, end = min(u1, g1);
+        unsigned row, lo, hi;
+        span_of(a, L, (unsigned)s, row, lo, hi);
+        const int vh = h * HG + hs, kvh = vh / a.subs, sub = vh - kvh * a.subs;
+        const int h0 = kvh * a.group + sub * GP, heads = min(GP, a.group - sub * GP);
+        const unsigned newest = a.k_new ? a.n_kv[row] - 1 : 0xffffffffu;
+        tile.init(a.q + (size_t)s * a.q_stride + (size_t)h0 * D, heads, a, extra, lane);
+        for (; g < end; ++g) {
+            issue();
+            if (ns == 3) cp_wait<2>();
+            else cp_wait<1>();
+            __syncwarp();
+            uint8_t *stage = ring + cstage * stage_bytes;
+            const unsigned live = masks[cstage];
+            const unsigned j0 = lo + ((unsigned)(g - u0) * R + r) * KEYS;
+            if (newest >= j0 && newest - j0 < KEYS && (live >> (newest - j0) & 1)) {
+                const unsigned page = a.tables[(size_t)row * a.max_pages + newest / a.pt];
+                const size_t head = (size_t)kvh * a.head_bytes;
+                const long long dst = (long long)(((size_t)page * a.pt + newest % a.pt) * a.token_bytes + head);
+                const size_t src = (size_t)s * a.new_stride + (size_t)kvh * D;
+                Tile::put_new(stage, a, (int)(newest - j0), a.k_new + src, a.v_new + src, dst, sub == 0, lane);
+            }
+            if (live) tile.step(stage, live, a, extra, lane);
+            __syncwarp();
+            cstage = cstage + 1 == ns ? 0 : cstage + 1;
+        }
+
+        // Close the row or its part: the head's warps are added into its first, which writes.
+        tile.close(lane);
+        tile.each(lane, a, [](int, int, float &) {}, [&](int hd, float m, float l, bool mine) {
+            if (mine) {
+                hm[hd] = m;
+                hl[hd] = l;
+            }
+        });
+        __syncwarp();
+        auto merge_of = [&](int rr) { return reinterpret_cast<float *>(smem + S.merge) + ((size_t)(rr - 1) * HG + hs) * GP * D; };
+        if (R > 1) {
+            if (r > 0) {
+                float *b = merge_of(r);
+                tile.each(lane, a, [&](int hd, int d, float &o) { b[hd * D + d] = o; }, [](int, float, float, bool) {});
+            }
+            __syncthreads();
+            if (r == 0) {
+                if (lane < GP) {
+                    float M = -INFINITY, sum = 0.f;
+                    for (int w = 0; w < R; ++w) M = fmaxf(M, warp_heads(w * HG + hs)[lane]);
+                    for (int w = 0; w < R; ++w) {
+                        float *o = warp_heads(w * HG + hs);
+                        const float f = o[lane] == -INFINITY ? 0.f : exp2f(o[lane] - M);
+                        sum += o[GP + lane] * f;
+                        o[2 * GP + lane] = f;
+                    }
+                    hm[lane] = M;
+                    hl[lane] = sum;
+                }
+                __syncwarp();
+                tile.each(lane, a, [&](int hd, int d, float &o) {
+                    float v = o * ff[hd];
+                    for (int w = 1; w < R; ++w) v = fmaf(merge_of(w)[hd * D + d], warp_heads(w * HG + hs)[2 * GP + hd], v);
+                    o = v;
+                }, [](int, float, float, bool) {});
+                __syncwarp();
+            }
+        }
+        if (r == 0) {
+            const bool whole = first == u0 && end == u1;
+            float *part = nullptr;
+            if (whole) {
+                if (lane < heads) {
+                    float M = hm[lane], sum = hl[lane], f = 1.f;
+                    if (a.sinks) {
+                        const float sk = a.sinks[h0 + lane] * LOG2E, top = fmaxf(M, sk);
+                        f = M == -INFINITY ? 0.f : exp2f(M - top);
+                        sum = sum * f + (sk == -INFINITY ? 0.f : exp2f(sk - top));
+                    }
+                    ff[lane] = sum == 0.f ? 0.f : f / sum;
+                }
+            } else {
+                part = a.part + (((size_t)blockIdx.x * 2 + (first == g0 ? 0 : 1)) * HG + hs) * GP * (D + 2);
+                if (lane < GP) {
+                    part[GP * D + 2 * lane] = hm[lane];
+                    part[GP * D + 2 * lane + 1] = hl[lane];
+                }
+            }
+            __syncwarp();
+            float *out = a.out + ((size_t)s * a.n_heads + h0) * D;
+            tile.each(lane, a, [&](int hd, int d, float &o) {
+                if (!whole) part[hd * D + d] = o;
+                else if (hd < heads) out[(size_t)hd * D + d] = o * ff[hd];
+            }, [](int, float, float, bool) {});
+        }
+        if (R > 1) __syncthreads();  // the sums and accumulators are free for the next row
+        else __syncwarp();
+    }
+    cp_wait<0>();
+}
+
+// Joins the rows that several CTAs had a part of, in tile order, and writes zeros to empty rows.
+// CTA (batch row, virtual head).
+constexpr int JOIN_THREADS = 256;
+template <int GP>
+__global__ void __launch_bounds__(JOIN_THREADS) k_attn_join(const __grid_constant__ attn_args a) {
+    extern __shared__ float wgt[];  // [GP][parts]
+    __shared__ float inv[GP];
+    pdl_trigger();
+    pdl_wait();
+    const int i = blockIdx.x, vh = blockIdx.y, D = a.D, HG = a.hg;
+    const int hgi = vh / HG, hs = vh - hgi * HG, kvh = vh / a.subs, sub = vh - kvh * a.subs;
+    const int h0 = kvh * a.group + sub * GP, heads = min(GP, a.group - sub * GP);
+    float *out = a.out + ((size_t)i * a.n_heads + h0) * D;
+    const long line = a.pre[a.n_seq], T = line * a.nhg, u0 = hgi * line + a.pre[i], u1 = hgi * line + a.pre[i + 1];
+    if (u0 == u1) {
+        for (int e = threadIdx.x; e < heads * D; e += JOIN_THREADS) out[e] = 0.f;
+        return;
+    }
+    const int ctas = a.pre[a.n_seq + 1], c0 = run_owner(T, ctas, u0), c1 = run_owner(T, ctas, u1 - 1), n = c1 - c0 + 1;
+    if (n == 1) return;
+    const size_t rec = (size_t)GP * (D + 2);
+    // the first CTA's part is its second record unless its run begins inside the row
+    auto part_of = [&](int k) {
+        const int c = c0 + k, slot = k > 0 || run_start(T, ctas, c) >= u0 ? 0 : 1;
+        return a.part + (((size_t)c * 2 + slot) * HG + hs) * rec;
+    };
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int hd = warp; hd < heads; hd += JOIN_THREADS / 32) {
+        const float sk = a.sinks ? a.sinks[h0 + hd] * LOG2E : -INFINITY;
+        float M = sk;
+        for (int k = lane; k < n; k += 32) {
+            const float m = part_of(k)[GP * D + 2 * hd];
+            wgt[hd * n + k] = m;
+            M = fmaxf(M, m);
+        }
+        M = warp_max(M);
+        float sum = 0.f;
+        for (int k = lane; k < n; k += 32) {
+            const float m = wgt[hd * n + k], f = m == -INFINITY ? 0.f : exp2f(m - M);
+            wgt[hd * n + k] = f;
+            sum += part_of(k)[GP * D + 2 * hd + 1] * f;
+        }
+        sum = warp_sum(sum);
+        if (lane == 0) {
+            sum += sk == -INFINITY ? 0.f : exp2f(sk - M);
+            inv[hd] = sum == 0.f ? 0.f : 1.f / sum;
+        }
+    }
+    __syncthreads();
+    const float *rest = n > 1 ? part_of(1) : nullptr;  // parts after the first are 2 HG rec apart
+    const size_t step = (size_t)2 * HG * rec;
+    for (int e = threadIdx.x; e < heads * D; e += JOIN_THREADS) {
+        const int hd = e / D;
+        const float *w = wgt + hd * n;
+        float v = part_of(0)[e] * w[0];
+#pragma unroll 8
+        for (int k = 1; k < n; ++k) v = fmaf(rest[(size_t)(k - 1) * step + e], w[k], v);
+        out[e] = v * inv[hd];
+    }
+}
+
+// ---- host side --------------------------------------------------------------------------------
+
+// How a shape is cut: virtual heads and warps per CTA, stages, shared memory and the grid.
+struct attn_plan {
+    bool mma;
+    int gp, keys, subs, hg, rsplit, nhg, warps, ns, smem, grid;
+};
+
+bool mma_dim(unsigned D) { return D == 64 || D == 80 || D == 96 || D == 128 || D == 256; }
+
+template <class Tile>
+bool cut(attn_plan &p, int warps, int ns, int minb, int n_heads, int n_kv, int D, int n_seq, int sms) {
+    p.gp = Tile::GP;
+    p.keys = Tile::KEYS;
+    const int group = n_heads / n_kv;
+    p.subs = (group + p.gp - 1) / p.gp;
+    const int V = n_kv * p.subs;
+    p.hg = 1;
+    for (int d = 2; d <= warps; ++d)
+        if (V % d == 0) p.hg = d;
+    p.rsplit = warps / p.hg;
+    p.nhg = V / p.hg;
+    p.warps = p.hg * p.rsplit;
+    p.ns = ns;
+    p.smem = layout_of(n_seq, p.warps, ns, Tile::stage_bytes(D, 0), Tile::extra_bytes(D), p.gp, p.warps - p.hg, D).total;
+    if (p.smem > MAX_SMEM - 512) return false;
+    p.grid = sms * std::max(1, std::min(minb, 233472 / (p.smem + 1536)));
+    return true;
+}
+
+template <class Tile>
+bool cut_core(attn_plan &p, int n_heads, int n_kv, int D, int n_seq, int sms) {
+    // three stages where eight warps have them, else two, else fewer warps
+    for (int warps = 8; warps >= 1; warps /= 2)
+        for (int ns = 3; ns >= 2; --ns)
+            if (cut<Tile>(p, warps, ns, 2, n_heads, n_kv, D, n_seq, sms)) return true;
+    return false;
+}
+
+// f(Tile, MINB) for the tile that serves a shape.
+template <typename F>
+auto with_tile(bool mma, unsigned kv_type, unsigned D, F &&f) {
+#define MMA_CASE(d, mb)                                                                       \
+    if (D == d)                                                                               \
+        return kv_type == T_BF16 ? f((mma_tile<d, true> *)nullptr, std::integral_constant<int, mb>()) \
+                                 : f((mma_tile<d, false> *)nullptr, std::integral_constant<int, mb>());
+    if (mma) {
+        MMA_CASE(64, 2)
+        MMA_CASE(80, 1)
+        MMA_CASE(96, 1)
+        MMA_CASE(128, 1)
+        MMA_CASE(256, 1)
+    }
+#undef MMA_CASE
+#define CORE_CASE(T)                                                                                  \
+    if (D <= 128) return f((core_tile<T, 1, 8> *)nullptr, std::integral_constant<int, 2>());          \
+    if (D <= 256) return f((core_tile<T, 2, 8> *)nullptr, std::integral_constant<int, 1>());          \
+    if (D <= 512) return f((core_tile<T, 4, 4> *)nullptr, std::integral_constant<int, 1>());          \
+    return f((core_tile<T, 8, 4> *)nullptr, std::integral_constant<int, 1>());
+    if (kv_type == T_F32) {
+        CORE_CASE(float)
+    } else if (kv_type == T_F16) {
+        CORE_CASE(__half)
+    }
+    CORE_CASE(__nv_bfloat16)
+#undef CORE_CASE
+}
+
+bool plan_of(attn_plan &p, bool mma, unsigned kv_type, int n_heads, int n_kv, int D, int n_seq, int sms) {
+    p.mma = mma;
+    return with_tile(mma, kv_type, (unsigned)D, [&](auto *t, auto minb) {
+        using Tile = std::remove_pointer_t<decltype(t)>;
+        if constexpr (Tile::NS > 0) return cut<Tile>(p, Tile::WARPS, Tile::NS, minb(), n_heads, n_kv, D, n_seq, sms);
+        else return cut_core<Tile>(p, n_heads, n_kv, D, n_seq, sms);
+    });
+}
+
+constexpr size_t PRE_BYTES = ((KV_LIST + 2) * 4 + 255) / 256 * 256;
+size_t attn_bytes(const attn_plan &p, int D) { return PRE_BYTES + (size_t)p.grid * 2 * p.hg * p.gp * (D + 2) * 4; }
+
+template <class Tile, int MINB>
+cudaError_t launch(moearc_ctx *c, const attn_plan &p, const attn_args &a, const seq_list &L) {
+    static std::atomic<bool> done[MOEARC_MAX_DEVICES];
+    cudaError_t e = once_per_device(done, [] { return set_smem(k_attn_batch<Tile, MINB>, MAX_SMEM - 512); });
+    if (e == cudaSuccess)
+        e = launch_pdl(k_attn_batch<Tile, MINB>, dim3((unsigned)p.grid), dim3((unsigned)p.warps * 32), (size_t)p.smem, c->stream, a, L, p.ns);
+    if (e == cudaSuccess)
+        e = launch_pdl(k_attn_join<Tile::GP>, dim3(a.n_seq, (unsigned)(p.hg * p.nhg)), dim3(JOIN_THREADS),
+                       (size_t)Tile::GP * p.grid * 4, c->stream, a);
+    return e;
+}
+
+}  // namespace
+
+extern "C" {
+
+unsigned long moearc_x_kv_work_bytes(moearc_ctx *c, const moearc_x_kv_cache *kv, unsigned int n_heads) {
+    if (!c || !kv || !kv_shape_ok(*kv)) return 0;
+    size_t need = kv_page_work_bytes(kv->n_pages);
+    if (n_heads) {
+        if (n_heads > 65535 || n_heads % kv->n_kv_heads) return 0;
+        // the cut goes by the batch (its prefix takes shared memory) and, for 16-bit caches, by the
+        // pools' alignment: the largest of them all
+        const int D = (int)kv->head_dim;
+        attn_plan p;
+        for (int n = 32; n <= (int)KV_LIST; n += 32) {
+            if (!plan_of(p, false, kv->kv_type, (int)n_heads, (int)kv->n_kv_heads, D, n, c->sm_count)) return 0;
+            need = std::max(need, attn_bytes(p, D));
+            if (kv->kv_type == T_F32 || !mma_dim(kv->head_dim)) continue;
+            if (!plan_of(p, true, kv->kv_type, (int)n_heads, (int)kv->n_kv_heads, D, n, c->sm_count)) return 0;
+            need = std::max(need, attn_bytes(p, D));
+        }
+    }
+    return need;
+}
+
+int moearc_x_attn_decode_batch(moearc_ctx *c, const moearc_x_kv_cache *kv, unsigned int layer, float *out, const float *q,
+                               unsigned long q_stride, const float *k_new, const float *v_new, unsigned long new_stride,
+                               const unsigned int *seqs, const unsigned int *kv_begin, const float *sinks, unsigned int n_seq,
+                               unsigned int n_heads, float scale) {
+    const int rc = kv_check(c, kv);
+    if (rc) return rc;
+    if (!out || !q || (!k_new) != (!v_new)) return ERR;
+    if (layer >= kv->n_layer || n_heads == 0 || n_heads > 65535 || n_heads % kv->n_kv_heads || n_seq > KV_LIST) return ERR_ARG;
+    if (n_seq == 0) return OK;
+    const size_t D = kv->head_dim;
+    if (q_stride < n_heads * D || (k_new && new_stride < kv->n_kv_heads * D)) return ERR_ARG;
+    if (!(scale == scale) || scale - scale != 0.f) return ERR_ARG;
+    seq_list L;
+    if (seqs) {
+        kv_rows_seen seen(kv->max_seq);
+        for (unsigned i = 0; i < n_seq; ++i) {
+            if (!seen.add(seqs[i], kv->max_seq)) return ERR_ARG;
+            L.row[i] = seqs[i];
+        }
+    } else if (n_seq > kv->max_seq) {
+        return ERR_ARG;
+    }
+    const uintptr_t align = reinterpret_cast<uintptr_t>(kv->k_pages[layer]) | reinterpret_cast<uintptr_t>(kv->v_pages[layer]);
+    const bool mma = kv->kv_type != T_F32 && mma_dim(kv->head_dim) && (align & 15) == 0;
+    attn_plan p;
+    if (!plan_of(p, mma, kv->kv_type, (int)n_heads, (int)kv->n_kv_heads, (int)D, (int)n_seq, c->sm_count)) return ERR_ARG;
+    if (kv->work_bytes < attn_bytes(p, (int)D)) return ERR_ARG;
+    const unsigned cap = kv->max_pages * kv->page_tokens;
+    if ((unsigned long long)n_seq * (cap / (unsigned)(p.keys * p.rsplit) + 1) >= (1ull << 31)) return ERR_ARG;
+
+    attn_args a;
+    a.out = out;
+    a.q = q;
+    a.k_new = k_new;
+    a.v_new = v_new;
+    a.sinks = sinks;
+    a.k = static_cast<uint8_t *>(kv->k_pages[layer]);
+    a.v = static_cast<uint8_t *>(kv->v_pages[layer]);
+    a.tables = kv->tables;
+    a.n_kv = kv->n_kv;
+    a.begin = kv_begin;
+    a.q_stride = q_stride;
+    a.new_stride = new_stride;
+    a.token_bytes = (size_t)kv->n_kv_heads * D * kv_elem_bytes(kv->kv_type);
+    a.head_bytes = D * kv_elem_bytes(kv->kv_type);
+    a.n_seq = n_seq;
+    a.max_pages = kv->max_pages;
+    a.n_pages = kv->n_pages;
+    a.pt = kv->page_tokens;
+    a.cap = cap;
+    a.listed = seqs != nullptr;
+    a.n_heads = (int)n_heads;
+    a.group = (int)(n_heads / kv->n_kv_heads);
+    a.D = (int)D;
+    a.subs = p.subs;
+    a.hg = p.hg;
+    a.rsplit = p.rsplit;
+    a.nhg = p.nhg;
+    a.min_tiles = 1;
+    a.scale2 = scale * LOG2E;
+    a.pre = static_cast<int *>(kv->work);
+    a.part = reinterpret_cast<float *>(static_cast<uint8_t *>(kv->work) + PRE_BYTES);
+    device_guard g(c->device);
+    if (!g.ok) return ERR;
+    launch_scope ls(c, "attn_decode_batch", n_seq, n_heads);
+    const cudaError_t e = with_tile(mma, kv->kv_type, kv->head_dim, [&](auto *t, auto minb) {
+        return launch<std::remove_pointer_t<decltype(t)>, decltype(minb)::value>(c, p, a, L);
+    });
+    if (e != cudaSuccess) cudaGetLastError();  // the failed launch's error, not left for an unrelated later check
+    const int rc2 = ls.finish();
+    return e != cudaSuccess ? ERR : rc2;
+}
+
+}  // extern "C"

@@ -1,0 +1,414 @@
+// logprobs.cu — log probabilities of given tokens under rows of logits, with each row's entropy and
+// its k likeliest tokens, in one pass over the logits.
+//
+// With x = scale logit, M = max x, L = sum e^(x - M) and S = sum e^(x - M) (x - M):
+//
+//   logprob(t) = (x_t - M) - log L,      entropy = log L - S / L,
+//
+// both from running (M, L, S) triples, joined as S' = f (S + (m - M) L) with f = e^(m - M) when the
+// maximum moves from m to M. The pass reads each logit once and is bound by HBM; for 16-bit logits the
+// exponentials (16 a clock and SM) come close behind.
+//
+// A row is one CTA, or a cluster of up to 16 where there are too few rows to fill the GPU; the
+// cluster's CTAs join over distributed shared memory, so there is no second kernel and no
+// workspace, and the order of the sums depends on the sizes alone.
+//
+// The k likeliest: a thread's running maximum is the largest of the elements it read, so the k-th
+// largest of a CTA's thread maxima is a bound that k elements reach. Only the elements of threads
+// at or above it (about k of 256 threads) are read again, from L2, and those that reach the bound
+// are ranked by counting. Should more reach it than the list holds (equal values), the k-th of the
+// listed ones becomes the next bound. A key is the value's bits in order, then the complement of
+// the index: no two are equal, and ties go to the lowest index.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+
+#include "kvcache.cuh"
+
+namespace cg = cooperative_groups;
+using namespace moearc;
+
+namespace {
+
+constexpr int TH = 256, WARPS = TH / 32, UNROLL = 4, MAX_K = MAX_TOPK, LIST = 512;
+constexpr float LOG2E = 1.4426950408889634f;
+
+typedef unsigned long long u64;
+
+struct lp_args {
+    const void *logits;
+    const unsigned *tokens;
+    size_t row_stride;
+    unsigned n_vocab, k;
+    float scale;
+    float *logprob, *entropy, *top_lp;
+    unsigned *top_id;
+};
+
+// 2^x, subnormal results as 0.
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// max that keeps a NaN
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+
+struct triple {
+    float m, l, s;
+};
+// a and b joined; the smaller maximum's sums are moved to the larger. An empty side (m -inf, l 0)
+// adds nothing; a NaN sum stays.
+__device__ __forceinline__ triple join(triple a, triple b) {
+    triple r;
+    r.m = fmaxf(a.m, b.m);
+    if (r.m == -INFINITY) return triple{-INFINITY, a.l + b.l, a.s + b.s};
+    const float da = fmaxf(a.m - r.m, -200.f), db = fmaxf(b.m - r.m, -200.f);
+    const float fa = ex2(da * LOG2E), fb = ex2(db * LOG2E);
+    r.l = a.l * fa + b.l * fb;
+    r.s = fa * fmaf(da, a.l, a.s) + fb * fmaf(db, b.l, b.s);
+    return r;
+}
+
+// Values in order as unsigned bits; a NaN ranks with -inf, -0 with +0.
+__device__ __forceinline__ u64 key_of(float x, unsigned i) {
+    const float v = x != x ? -INFINITY : x + 0.f;
+    const unsigned b = __float_as_uint(v);
+    return (u64)(b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u)) << 32 | (0xffffffffu - i);
+}
+__device__ __forceinline__ float value_of(u64 key) {
+    const unsigned o = (unsigned)(key >> 32);
+    return __uint_as_float(o ^ ((o >> 31) ? 0x80000000u : 0xffffffffu));
+}
+
+template <typename T>
+struct vec {
+    static constexpr int N = 16 / sizeof(T);
+    float v[N];
+};
+__device__ __forceinline__ uint4 ld16(const void *p) {
+    uint4 u;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "l"(p));
+    return u;
+}
+template <typename T>
+__device__ __forceinline__ void unpack(uint4 u, float *v) {
+    const unsigned w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(T) == 4) {
+            v[i] = __uint_as_float(w[i]);
+        } else if constexpr (std::is_same<T, __half>::value) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+            v[2 * i] = f.x;
+            v[2 * i + 1] = f.y;
+        } else {
+            v[2 * i] = __uint_as_float(w[i] << 16);
+            v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+    }
+}
+__device__ __forceinline__ float one(const float *p) { return *p; }
+__device__ __forceinline__ float one(const __half *p) { return __half2float(*p); }
+__device__ __forceinline__ float one(const __nv_bfloat16 *p) { return __bfloat162float(*p); }
+
+// N values into a running triple: one look at the maximum for all of them.
+template <int N>
+__device__ __forceinline__ void take(triple &r, const float (&x)[N]) {
+    float b = x[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) b = fmaxf(b, x[i]);
+    if (b > r.m) {
+        if (r.m != -INFINITY) {
+            const float d = fmaxf(r.m - b, -200.f), f = ex2(d * LOG2E);
+            r.s = f * fmaf(d, r.l, r.s);
+            r.l *= f;
+        }
+        r.m = b;
+    }
+    const float base = r.m == -INFINITY ? 0.f : r.m;
+    float l0 = 0.f, l1 = 0.f, s0 = 0.f, s1 = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        // below -200 the weight is 0 in f32; the floor keeps 0 x -inf out of S
+        const float d = max_nan(x[i] - base, -200.f), e = ex2(d * LOG2E);
+        if (i & 1) {
+            l1 += e;
+            s1 = fmaf(e, d, s1);
+        } else {
+            l0 += e;
+            s0 = fmaf(e, d, s0);
+        }
+    }
+    r.l += l0 + l1;
+    r.s += s0 + s1;
+}
+
+// The CTA's run [c0, c1) of a row: single elements up to a 16-byte boundary, whole vectors, the
+// rest. Thread t reads element t of the first and last, vectors t, t + TH, ...
+template <typename T>
+struct run {
+    const T *row;
+    unsigned c0, head, nv, c1;
+    __device__ run(const T *r, unsigned a, unsigned b) : row(r), c0(a), c1(b) {
+        constexpr int V = vec<T>::N;
+        const unsigned off = (unsigned)(reinterpret_cast<uintptr_t>(r + a) & 15) / sizeof(T);
+        head = min((V - off) % V, c1 - c0);
+        nv = (c1 - c0 - head) / V;
+    }
+    __device__ unsigned body() const { return c0 + head; }
+    __device__ unsigned tail() const { return body() + nv * vec<T>::N; }
+};
+
+struct shared_lists {
+    triple part[WARPS], whole;
+    float warp_bound[WARPS];
+    float max_v[TH];
+    unsigned max_t[TH];
+    unsigned n_max, n_sub, sub[TH], n_list, n_top;
+    float bound;
+    u64 bound_key;
+    u64 list[LIST], top[MAX_K];
+};
+
+// The largest min(k, n) of list[0, n) in order, into top; rank by counting.
+__device__ void rank_list(const u64 *list, unsigned n, unsigned k, u64 *top) {
+    for (unsigned i = threadIdx.x; i < n; i += TH) {
+        const u64 key = list[i];
+        unsigned rank = 0;
+        for (unsigned j = 0; j < n; ++j) rank += list[j] > key;
+        if (rank < k) top[rank] = key;
+    }
+}
+
+// The largest min(k, elements) keys of the CTA's run, in order, in sh.top; m: the thread's maximum.
+template <typename T>
+__device__ void top_of_run(const run<T> &R, float m, float scale, unsigned k, shared_lists &sh) {
+    constexpr int V = vec<T>::N;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    // a first bound: each warp has ceil(k / WARPS) lanes at or above its own, so k threads of the
+    // CTA are at or above the least of them
+    float v = m, last = m;
+    for (unsigned q = 0; q < (k + WARPS - 1) / WARPS; ++q) {
+        last = warp_max(v);
+        const unsigned who = __ballot_sync(0xffffffffu, v == last);
+        if (lane == __ffs(who) - 1) v = -INFINITY;
+    }
+    if (lane == 0) sh.warp_bound[warp] = last;
+    if (threadIdx.x == 0) sh.n_max = sh.n_sub = 0;
+    __syncthreads();
+    float bound = sh.warp_bound[0];
+#pragma unroll
+    for (int w = 1; w < WARPS; ++w) bound = fminf(bound, sh.warp_bound[w]);
+    if (m >= bound) {
+        const unsigned i = atomicAdd(&sh.n_max, 1u);
+        sh.max_v[i] = m;
+        sh.max_t[i] = threadIdx.x;
+    }
+    __syncthreads();
+    // the k-th largest of the listed maxima (ties in any order give the same value)
+    const unsigned n_max = sh.n_max;
+    if (threadIdx.x < n_max) {
+        const float mine = sh.max_v[threadIdx.x];
+        unsigned rank = 0;
+        for (unsigned j = 0; j < n_max; ++j) rank += sh.max_v[j] > mine || (sh.max_v[j] == mine && j < threadIdx.x);
+        if (rank == k - 1) sh.bound = mine;
+    }
+    __syncthreads();
+    bound = sh.bound;
+    if (m >= bound) sh.sub[atomicAdd(&sh.n_sub, 1u)] = threadIdx.x;
+    u64 least = key_of(bound, 0xffffffffu);
+    for (;;) {
+        if (threadIdx.x == 0) sh.n_list = 0;
+        __syncthreads();
+        auto see = [&](float x, unsigned i) {
+            const u64 key = key_of(x, i);
+            if (key >= least) {
+                const unsigned at = atomicAdd(&sh.n_list, 1u);
+                if (at < LIST) sh.list[at] = key;
+            }
+        };
+        const unsigned n_sub = sh.n_sub;
+        for (unsigned w = warp; w < n_sub; w += WARPS) {
+            const unsigned t = sh.sub[w];
+            if (lane == 0 && t < R.head) see(one(R.row + R.c0 + t) * scale, R.c0 + t);
+            if (lane == 1 && R.tail() + t < R.c1) see(one(R.row + R.tail() + t) * scale, R.tail() + t);
+            for (unsigned j = t + lane * TH; j < R.nv; j += 32 * TH) {
+                float x[V];
+                unpack<T>(ld16(R.row + R.body() + (size_t)j * V), x);
+#pragma unroll
+                for (int e = 0; e < V; ++e) see(x[e] * scale, R.body() + j * V + e);
+            }
+        }
+        __syncthreads();
+        const unsigned n = min(sh.n_list, (unsigned)LIST);
+        const bool over = sh.n_list > LIST;
+        rank_list(sh.list, n, k, sh.top);
+        if (threadIdx.x == 0) sh.n_top = min(n, k);
+        __syncthreads();
+        if (!over) return;
+        least = sh.top[k - 1];  // k listed elements reach it: the next bound, above the last
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(TH, 4) k_logprobs(const lp_args a) {
+    constexpr int V = vec<T>::N;
+    __shared__ shared_lists sh;
+    cg::cluster_group cluster = cg::this_cluster();
+    const unsigned size = cluster.num_blocks(), rank = cluster.block_rank();
+    const unsigned row = blockIdx.x / size;
+    pdl_trigger();
+    pdl_wait();
+    const T *p = static_cast<const T *>(a.logits) + (size_t)row * a.row_stride;
+    const unsigned share = ((a.n_vocab + size - 1) / size + V - 1) / V * V;
+    const unsigned c0 = min(rank * share, a.n_vocab), c1 = min(c0 + share, a.n_vocab);
+    const run<T> R(p, c0, c1);
+    const float scale = a.scale;
+
+    triple r{-INFINITY, 0.f, 0.f};
+    unsigned j = threadIdx.x;
+    for (; j + (UNROLL - 1) * TH < R.nv; j += UNROLL * TH) {
+        uint4 u[UNROLL];
+#pragma unroll
+        for (int i = 0; i < UNROLL; ++i) u[i] = ld16(R.row + R.body() + (size_t)(j + i * TH) * V);
+        float x[UNROLL * V];
+#pragma unroll
+        for (int i = 0; i < UNROLL; ++i) unpack<T>(u[i], x + i * V);
+#pragma unroll
+        for (int i = 0; i < UNROLL * V; ++i) x[i] *= scale;
+        take(r, x);
+    }
+    for (; j < R.nv; j += TH) {
+        float x[V];
+        unpack<T>(ld16(R.row + R.body() + (size_t)j * V), x);
+#pragma unroll
+        for (int i = 0; i < V; ++i) x[i] *= scale;
+        take(r, x);
+    }
+    if (threadIdx.x < R.head) {
+        const float x[1] = {one(R.row + R.c0 + threadIdx.x) * scale};
+        take(r, x);
+    }
+    if (R.tail() + threadIdx.x < R.c1) {
+        const float x[1] = {one(R.row + R.tail() + threadIdx.x) * scale};
+        take(r, x);
+    }
+    const float mine = r.m;
+
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const triple b{__shfl_xor_sync(0xffffffffu, r.m, o), __shfl_xor_sync(0xffffffffu, r.l, o), __shfl_xor_sync(0xffffffffu, r.s, o)};
+        r = join(r, b);
+    }
+    if (lane == 0) sh.part[warp] = r;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        r = sh.part[0];
+        for (int w = 1; w < WARPS; ++w) r = join(r, sh.part[w]);
+        sh.whole = r;
+    }
+    if (a.k) top_of_run(R, mine, scale, a.k, sh);
+    if (size > 1) cluster.sync();
+    else __syncthreads();
+    if (rank == 0) {
+        r = sh.whole;
+        for (unsigned c = 1; c < size; ++c) r = join(r, cluster.map_shared_rank(&sh, c)->whole);
+        const float log_l = logf(r.l);
+        const bool none = r.m == -INFINITY && r.l == 0.f;  // every logit -inf
+        if (threadIdx.x == 0) {
+            if (a.entropy) a.entropy[row] = none ? 0.f : log_l - r.s / r.l;
+            if (a.logprob) {
+                const unsigned t = a.tokens[row];
+                a.logprob[row] = t >= a.n_vocab ? 0.f : none ? -INFINITY : (one(p + t) * scale - r.m) - log_l;
+            }
+        }
+        if (a.k) {
+            u64 *top = sh.top;
+            if (size > 1) {
+                __shared__ u64 every[16 * MAX_K], best[MAX_K];
+                __shared__ unsigned at[17];
+                if (threadIdx.x == 0) {
+                    at[0] = 0;
+                    for (unsigned c = 0; c < size; ++c) at[c + 1] = at[c] + cluster.map_shared_rank(&sh, c)->n_top;
+                }
+                __syncthreads();
+                for (unsigned i = threadIdx.x; i < size * MAX_K; i += TH) {
+                    const unsigned c = i / MAX_K, e = i - c * MAX_K;
+                    if (e < at[c + 1] - at[c]) every[at[c] + e] = cluster.map_shared_rank(&sh, c)->top[e];
+                }
+                __syncthreads();
+                rank_list(every, at[size], a.k, best);
+                __syncthreads();
+                top = best;
+            }
+            if (threadIdx.x < a.k) {
+                const u64 key = top[threadIdx.x];
+                const float v = value_of(key);
+                a.top_id[(size_t)row * a.k + threadIdx.x] = 0xffffffffu - (unsigned)key;
+                a.top_lp[(size_t)row * a.k + threadIdx.x] = none ? -INFINITY : (v - r.m) - log_l;
+            }
+        }
+    }
+    if (size > 1) cluster.sync();  // the other CTAs' lists are read until here
+}
+
+template <typename T>
+cudaError_t launch(moearc_ctx *c, const lp_args &a, unsigned n_rows) {
+    static std::atomic<bool> done[MOEARC_MAX_DEVICES];
+    cudaError_t e = once_per_device(done, [] {
+        return cudaFuncSetAttribute(k_logprobs<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    });
+    if (e != cudaSuccess) return e;
+    // CTAs for twice the SMs, but at least 8 vectors a thread of each; 16 CTAs only where 8 leave
+    // most SMs idle
+    const unsigned most = std::max(1u, a.n_vocab / (TH * 8 * (unsigned)vec<T>::N));
+    unsigned size = 1;
+    while (size < 16 && n_rows * size < (unsigned)c->sm_count * 2 && size * 2 <= most) size *= 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(n_rows * size);
+    cfg.blockDim = dim3(TH);
+    cfg.stream = c->stream;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = size;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, k_logprobs<T>, a);
+}
+
+}  // namespace
+
+extern "C" {
+
+int moearc_x_token_logprobs(moearc_ctx *c, const void *logits, unsigned int type, unsigned long row_stride, unsigned int n_rows,
+                            unsigned int n_vocab, float scale, const unsigned int *tokens, float *logprob, float *entropy,
+                            unsigned int k, unsigned int *top_ids, float *top_logprobs) {
+    if (!c || !logits || (!tokens) != (!logprob)) return ERR;
+    if (k && (!top_ids || !top_logprobs)) return ERR;
+    if (!kv_elem_bytes(type)) return ERR_ARG;
+    if (n_vocab == 0 || n_vocab > (1u << 30) || row_stride < n_vocab || k > MAX_TOPK || k > n_vocab || n_rows > (1u << 26)) return ERR_ARG;
+    if (!(scale > 0.f) || scale - scale != 0.f) return ERR_ARG;
+    if (reinterpret_cast<uintptr_t>(logits) % kv_elem_bytes(type)) return ERR_ARG;
+    if (n_rows == 0) return OK;
+    const lp_args a{logits, tokens, row_stride, n_vocab, k, scale, logprob, entropy, top_logprobs, top_ids};
+    device_guard g(c->device);
+    if (!g.ok) return ERR;
+    launch_scope ls(c, "token_logprobs", n_rows, n_vocab);
+    const cudaError_t e = type == T_F32   ? launch<float>(c, a, n_rows)
+                          : type == T_F16 ? launch<__half>(c, a, n_rows)
+                                          : launch<__nv_bfloat16>(c, a, n_rows);
+    if (e != cudaSuccess) cudaGetLastError();  // the failed launch's error, not left for an unrelated later check
+    const int rc = ls.finish();
+    return e != cudaSuccess ? ERR : rc;
+}
+
+}  // extern "C"

@@ -321,6 +321,22 @@ class Context:
         self._finish(self.lib.moearc_topk_router(self.raw, idx.ptr, weights.ptr, logits.ptr, n_tokens,
                                                  n_expert, k, gating), "topk_router")
 
+    def token_logprobs(self, logits, ty: int, n_rows: int, n_vocab: int, *, tokens=None, logprob=None, entropy=None,
+                       k: int = 0, top_ids=None, top_logprobs=None, row_stride: int | None = None,
+                       scale: float = 1.0) -> None:
+        """Log probabilities of `tokens` (u32 [n_rows]) under rows of logits (F32, F16 or BF16), each row's
+        entropy and its k likeliest tokens (moearc_x_token_logprobs); outputs that are None are left out."""
+        stride = n_vocab if row_stride is None else row_stride
+        if ty in KV_ELEM_BYTES and n_rows:
+            logits.require("logits", KV_ELEM_BYTES[ty] * ((n_rows - 1) * stride + n_vocab))
+        for b, what, each in ((tokens, "tokens", 1), (logprob, "log probability output", 1), (entropy, "entropy output", 1),
+                              (top_ids, "alternatives' ids", k), (top_logprobs, "alternatives' output", k)):
+            if b is not None:
+                b.require(what, 4 * n_rows * each)
+        self._finish(self.lib.moearc_x_token_logprobs(self.raw, logits.ptr, ty, stride, n_rows, n_vocab, scale, _p(tokens),
+                                                      _p(logprob), _p(entropy), k, _p(top_ids), _p(top_logprobs)),
+                     "token_logprobs")
+
     def synth(self, dst: DeviceBuffer, n: int, kind: int, seed: int, sigma: float = 1.0, lo: int = -8,
               hi: int = -4) -> None:
         self._finish(self.lib.moearc_x_synth(self.raw, dst.ptr, n, kind, seed, sigma, lo, hi), "synth")
