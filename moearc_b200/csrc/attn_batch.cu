@@ -44,6 +44,9 @@ namespace {
 
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int MAX_SMEM = 227 * 1024;
+// A row's weights are taken against a reference that follows its maximum only once that is this much
+// above (in powers of two): most tiles then rescale nothing, and weights stay below 2^8.
+constexpr float LAZY = 8.f;
 
 struct seq_list {
     unsigned row[KV_LIST];
@@ -56,6 +59,8 @@ struct attn_args {
     const unsigned *tables, *n_kv, *begin;
     size_t q_stride, new_stride, token_bytes, head_bytes;  // bytes: n_kv_heads x head_dim elements, head_dim elements
     unsigned n_seq, max_pages, n_pages, pt, cap;
+    unsigned unit;  // bytes of one copy: 16 where rows start on 16-byte boundaries, else 4 or 2
+    int one_page;   // tiles never cross a page
     int listed;  // rows come from the list (else row i is batch row i)
     int n_heads, group, D, subs;  // subs: virtual heads a kv head (its query heads by GP)
     int hg, rsplit, nhg;          // virtual heads a CTA, warps a head, head groups
@@ -79,16 +84,27 @@ __device__ __forceinline__ int run_owner(long total, int ctas, long g) {
     return (int)(g < r * (b + 1) ? g / (b + 1) : r + (g - r * (b + 1)) / b);
 }
 
-__device__ __forceinline__ void cp_async(void *smem, const void *gmem, int bytes, bool valid) {
-    const unsigned s = (unsigned)__cvta_generic_to_shared(smem);
-    if (bytes == 16)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(s), "l"(gmem), "r"(valid ? 16 : 0) : "memory");
-    else
-        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(s), "l"(gmem), "r"(valid ? 4 : 0) : "memory");
+// 16 (or 4) bytes global -> shared, zeros in their place where the source is not to be read.
+__device__ __forceinline__ void cp_async16(unsigned dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async16z(unsigned dst, const void *src, bool valid) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async4z(unsigned dst, const void *src, bool valid) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(dst), "l"(src), "r"(valid ? 4 : 0) : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory"); }
+__device__ __forceinline__ unsigned smem_u32(const void *p) { return (unsigned)__cvta_generic_to_shared(p); }
+
+// 2^x, subnormal results as 0.
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 
 // ---- the tensor-core tile (16-bit caches) -----------------------------------------------------
 
@@ -101,13 +117,13 @@ __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uin
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], const void *p) {
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], unsigned p) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"((unsigned)__cvta_generic_to_shared(p)) : "memory");
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(p) : "memory");
 }
-__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], const void *p) {
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], unsigned p) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"((unsigned)__cvta_generic_to_shared(p)) : "memory");
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(p) : "memory");
 }
 
 template <bool BF>
@@ -120,36 +136,97 @@ __device__ __forceinline__ float from16(uint16_t b) {
     if constexpr (BF) return bf16_bits_to_f32(b);
     else return f16_bits_to_f32(b);
 }
+// Two values rounded to 16 bits and packed, and a packed pair's values.
+template <bool BF>
+__device__ __forceinline__ uint32_t pack(float x, float y) {
+    if constexpr (BF) {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
+        return *reinterpret_cast<const uint32_t *>(&v);
+    } else {
+        const __half2 v = __floats2half2_rn(x, y);
+        return *reinterpret_cast<const uint32_t *>(&v);
+    }
+}
+template <bool BF>
+__device__ __forceinline__ float2 unpack(uint32_t u) {
+    if constexpr (BF) return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+    else return __half22float2(*reinterpret_cast<const __half2 *>(&u));
+}
 // Two values as packed pairs of 16-bit terms: x = t0 + t1 (+ t2), each term the rounding of what
 // the ones before it leave.
 template <bool BF>
 __device__ __forceinline__ void terms(float x, float y, uint32_t &t0, uint32_t &t1, uint32_t &t2) {
-    const uint16_t x0 = to16<BF>(x), y0 = to16<BF>(y);
-    const float xr = x - from16<BF>(x0), yr = y - from16<BF>(y0);
-    const uint16_t x1 = to16<BF>(xr), y1 = to16<BF>(yr);
-    t0 = x0 | (uint32_t)y0 << 16;
-    t1 = x1 | (uint32_t)y1 << 16;
-    if constexpr (BF) t2 = to16<BF>(xr - from16<BF>(x1)) | (uint32_t)to16<BF>(yr - from16<BF>(y1)) << 16;
+    t0 = pack<BF>(x, y);
+    const float2 a = unpack<BF>(t0);
+    t1 = pack<BF>(x - a.x, y - a.y);
+    if constexpr (BF) {
+        const float2 b = unpack<BF>(t1);
+        t2 = pack<BF>(x - a.x - b.x, y - a.y - b.y);
+    }
 }
 
 template <int D_, bool BF>
 struct mma_tile {
-    static constexpr int KEYS = 16, GP = 8, D = D_, WARPS = D_ > 128 ? 4 : 8, NS = 3;
+    static constexpr int KEYS = 16, GP = 8, ELEM = 2, D = D_, WARPS = D_ > 128 ? 4 : 8;
     // Rows of a stage: chunk c of row r lies at c ^ (r & 7) where a row is whole 128-byte lines,
     // else rows are padded by one chunk to an odd number of them, so that the eight rows of an
     // ldmatrix meet eight different bank groups.
     static constexpr bool SWZ = D % 64 == 0;
     static constexpr int CH = D / 8, ROW = SWZ ? D : D + 8;
-    static constexpr int STAGE = 2 * KEYS * ROW * 2;  // bytes: K rows, then V rows
-    static constexpr float PSCALE = BF ? 1.f : 4096.f;  // f16 weights scaled away from subnormals
+    // f16 weights are scaled away from subnormals (and stay below 65504 with the 2^8 of LAZY)
+    static constexpr float PSCALE = BF ? 1.f : 64.f;
+    // Tiles whose P V the tensor core sums before they are added to o (its sums truncate: a few
+    // are within f32's rounding, a long row's are not). Above 128 channels registers allow one.
+    static constexpr int CHAIN = D <= 128 ? 8 : 1;
 
     uint32_t qa[D / 16][4], ql[BF ? D / 16 : 1][2];
-    float o[D / 8][2], m, l, sc;
-    static __host__ __device__ int stage_bytes(int, int) { return STAGE; }
+    float o[D / 8][2], c[CHAIN > 1 ? D / 8 : 1][4], m, l, sc;
+    int chained;
+    static __host__ __device__ int row_bytes(int) { return ROW * 2; }
     static __host__ __device__ int extra_bytes(int) { return 0; }
+    // byte offset of chunk c of row r
+    static __device__ __forceinline__ int at(int r, int c) { return r * ROW * 2 + (SWZ ? (c ^ (r & 7)) : c) * 16; }
 
-    static __device__ __forceinline__ int at(int r, int c) { return r * ROW + (SWZ ? (c ^ (r & 7)) : c) * 8; }
-
+    // A whole tile of consecutive slots: `src` is the first key's row in the K pool, `to_v` the way
+    // from the K pool to the V pool.
+    static __device__ __forceinline__ void load_run(uint8_t *stage, const uint8_t *src, long long to_v, const attn_args &a, int lane) {
+        const unsigned s0 = smem_u32(stage);
+        if constexpr (32 % CH == 0) {  // a lane keeps its chunk and takes every 32 / CH-th row
+            constexpr int RW = 32 / CH;
+            const int rr = lane / CH, ch = lane % CH;
+            const uint8_t *p = src + (size_t)rr * a.token_bytes + ch * 16;
+            const size_t step = a.token_bytes * RW;
+            const unsigned d0 = s0 + at(rr, ch);
+#pragma unroll
+            for (int i = 0; i < KEYS / RW; ++i, p += step) {
+                const unsigned d = (d0 ^ (SWZ ? (i * RW & 7) << 4 : 0)) + i * RW * ROW * 2;
+                cp_async16(d, p);
+                cp_async16(d + KEYS * ROW * 2, p + to_v);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < KEYS * CH / 32; ++i) {
+                const int c = lane + 32 * i, r = c / CH, ch = c % CH;
+                const uint8_t *p = src + (size_t)r * a.token_bytes + ch * 16;
+                const unsigned d = s0 + at(r, ch);
+                cp_async16(d, p);
+                cp_async16(d + KEYS * ROW * 2, p + to_v);
+            }
+        }
+    }
+    // Any tile: lane r holds the byte offset of key r's row in a pool, or -1 for zeros.
+    static __device__ __forceinline__ void load_rows(uint8_t *stage, long long off, const attn_args &a, int lane) {
+        const unsigned s0 = smem_u32(stage);
+#pragma unroll 4
+        for (int i = 0; i < KEYS * CH / 32; ++i) {
+            const int c = lane + 32 * i, r = c / CH, ch = c % CH;
+            const long long b = __shfl_sync(0xffffffffu, off, r);
+            const size_t src = (b < 0 ? 0 : (size_t)b) + ch * 16;
+            const unsigned d = s0 + at(r, ch);
+            cp_async16z(d, a.k + src, b >= 0);
+            cp_async16z(d + KEYS * ROW * 2, a.v + src, b >= 0);
+        }
+    }
     // Rows 0-7 of the A operand hold the first term of the (up to 8) heads, rows 8-15 the second;
     // the third, where there is one, is a second A operand with its rows 8-15 zero.
     __device__ __forceinline__ void init(const float *q, int heads, const attn_args &a, uint8_t *, int lane) {
@@ -181,48 +258,53 @@ struct mma_tile {
             }
         }
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = 0.f;
+        for (int i = 0; i < D / 8; ++i) {
+            o[i][0] = o[i][1] = 0.f;
+            if constexpr (CHAIN > 1) c[i][0] = c[i][1] = c[i][2] = c[i][3] = 0.f;
+        }
         m = -INFINITY;
         l = 0.f;
+        chained = 0;
     }
-
-    // off: lane r < KEYS holds the byte offset of key r's row in a pool, or -1.
-    static __device__ __forceinline__ void load(uint8_t *stage, const attn_args &a, long long off, int lane) {
-        auto *ks = reinterpret_cast<uint16_t *>(stage), *vs = ks + KEYS * ROW;
+    // o takes the chained sums, both scaled.
+    __device__ __forceinline__ void flush(float f) {
+        if constexpr (CHAIN > 1) {
 #pragma unroll
-        for (int c = lane; c < KEYS * CH; c += 32) {
-            const int r = c / CH, ch = c % CH;
-            const long long b = __shfl_sync(0xffffffffu, off, r);
-            const size_t src = (b < 0 ? 0 : (size_t)b) + ch * 16;
-            cp_async(ks + at(r, ch), a.k + src, 16, b >= 0);
-            cp_async(vs + at(r, ch), a.v + src, 16, b >= 0);
-        }
-    }
-    // The newest token's row r of the tile, from f32; `dst` >= 0 also stores it in the pools.
-    static __device__ __forceinline__ void put_new(uint8_t *stage, const attn_args &a, int r, const float *kn, const float *vn,
-                                                   long long dst, bool store, int lane) {
-        auto *ks = reinterpret_cast<uint16_t *>(stage), *vs = ks + KEYS * ROW;
-        for (int d = lane; d < D; d += 32) {
-            const uint16_t kb = to16<BF>(kn[d]), vb = to16<BF>(vn[d]);
-            const int i = at(r, d >> 3) + (d & 7);
-            ks[i] = kb;
-            vs[i] = vb;
-            if (store) {
-                reinterpret_cast<uint16_t *>(a.k + dst)[d] = kb;
-                reinterpret_cast<uint16_t *>(a.v + dst)[d] = vb;
+            for (int i = 0; i < D / 8; ++i) {
+                o[i][0] = (o[i][0] + (c[i][0] + c[i][2])) * f;
+                o[i][1] = (o[i][1] + (c[i][1] + c[i][3])) * f;
+                c[i][0] = c[i][1] = c[i][2] = c[i][3] = 0.f;
+            }
+            chained = 0;
+        } else {
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i) {
+                o[i][0] *= f;
+                o[i][1] *= f;
             }
         }
-        __syncwarp();
+    }
+
+    // Row r of the stage (keys, then values) from f32, and into its slot where that is given.
+    static __device__ __forceinline__ void round_row(const float *x, uint8_t *stage, int r, uint8_t *slot, const attn_args &, int lane) {
+        for (int d = lane; d < D; d += 32) {
+            const uint16_t b = to16<BF>(x[d]);
+            *reinterpret_cast<uint16_t *>(stage + at(r, d >> 3) + (d & 7) * 2) = b;
+            if (slot) reinterpret_cast<uint16_t *>(slot)[d] = b;
+        }
     }
 
     __device__ __forceinline__ void step(const uint8_t *stage, unsigned live, const attn_args &, uint8_t *, int lane) {
-        const auto *ks = reinterpret_cast<const uint16_t *>(stage), *vs = ks + KEYS * ROW;
         const int qd = lane & 3, mi = lane >> 3;
+        // this lane's rows of the ldmatrix operands: keys (non-transposed) and values (transposed).
+        // Stages start on whole rows, so chunk c + 2 i of a swizzled row is chunk c's address xor 32 i.
+        const unsigned kb = smem_u32(stage) + at(((mi >> 1) << 3) | (lane & 7), mi & 1);
+        const unsigned vb = smem_u32(stage) + KEYS * ROW * 2 + at(((mi & 1) << 3) | (lane & 7), mi >> 1);
         float c0[2][4] = {}, c1[2][4] = {};
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
             uint32_t b[4];
-            ldsm4(b, ks + at(((mi >> 1) << 3) | (lane & 7), 2 * kk + (mi & 1)));
+            ldsm4(b, SWZ ? kb ^ (kk * 32) : kb + kk * 32);
             mma<BF>(c0[0], qa[kk][0], qa[kk][1], qa[kk][2], qa[kk][3], b[0], b[1]);
             mma<BF>(c0[1], qa[kk][0], qa[kk][1], qa[kk][2], qa[kk][3], b[2], b[3]);
             if constexpr (BF) {
@@ -232,52 +314,57 @@ struct mma_tile {
         }
         // scores (in powers of two) of head lane / 4 for keys 2 qd, 2 qd + 1, 8 + 2 qd, 9 + 2 qd
         float s[4];
+        const unsigned in = live >> (2 * qd);
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const float x = (c0[n][e] + (BF ? c0[n][e + 2] + c1[n][e] : c0[n][e + 2])) * sc;
-                s[2 * n + e] = live >> (8 * n + 2 * qd + e) & 1 ? x : -INFINITY;
+                s[2 * n + e] = in >> (8 * n + e) & 1 ? x : -INFINITY;
             }
         float mt = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
-        mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
-        mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 2));
-        const float mn = fmaxf(m, mt);
-        const float base = mn == -INFINITY ? 0.f : mn, corr = exp2f(m - base);
+        if (__any_sync(0xffffffffu, mt > m + LAZY)) {
+            mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
+            mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 2));
+            const float mn = fmaxf(m, mt), corr = ex2(m - (mn == -INFINITY ? 0.f : mn));
+            flush(corr);
+            l *= corr;
+            m = mn;
+        }
+        const float base = m == -INFINITY ? 0.f : m;
         float p[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) p[e] = exp2f(s[e] - base);
-        l = l * corr + ((p[0] + p[1]) + (p[2] + p[3]));
-        m = mn;
+        for (int e = 0; e < 4; ++e) p[e] = ex2(s[e] - base);
+        l += (p[0] + p[1]) + (p[2] + p[3]);
         uint32_t a0, a1, a2, a3, b0 = 0, b2 = 0;
         terms<BF>(p[0] * PSCALE, p[1] * PSCALE, a0, a1, b0);
         terms<BF>(p[2] * PSCALE, p[3] * PSCALE, a2, a3, b2);
 #pragma unroll
         for (int dn = 0; dn < D / 16; ++dn) {
             uint32_t b[4];
-            ldsm4t(b, vs + at(((mi & 1) << 3) | (lane & 7), 2 * dn + (mi >> 1)));
+            ldsm4t(b, SWZ ? vb ^ (dn * 32) : vb + dn * 32);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                float c[4] = {};
-                if constexpr (BF) mma<BF>(c, b0, 0u, b2, 0u, b[2 * h], b[2 * h + 1]);
-                mma<BF>(c, a0, a1, a2, a3, b[2 * h], b[2 * h + 1]);
-                o[2 * dn + h][0] = fmaf(o[2 * dn + h][0], corr, c[0] + c[2]);
-                o[2 * dn + h][1] = fmaf(o[2 * dn + h][1], corr, c[1] + c[3]);
+                if constexpr (CHAIN > 1) {
+                    if constexpr (BF) mma<BF>(c[2 * dn + h], b0, 0u, b2, 0u, b[2 * h], b[2 * h + 1]);
+                    mma<BF>(c[2 * dn + h], a0, a1, a2, a3, b[2 * h], b[2 * h + 1]);
+                } else {
+                    float t[4] = {};
+                    if constexpr (BF) mma<BF>(t, b0, 0u, b2, 0u, b[2 * h], b[2 * h + 1]);
+                    mma<BF>(t, a0, a1, a2, a3, b[2 * h], b[2 * h + 1]);
+                    o[2 * dn + h][0] += t[0] + t[2];
+                    o[2 * dn + h][1] += t[1] + t[3];
+                }
             }
         }
+        if (CHAIN > 1 && ++chained == CHAIN) flush(1.f);
     }
 
     // After the last tile: l summed over the head's lanes, o without its scale.
     __device__ __forceinline__ void close(int) {
         l += __shfl_xor_sync(0xffffffffu, l, 1);
         l += __shfl_xor_sync(0xffffffffu, l, 2);
-        if constexpr (!BF) {
-#pragma unroll
-            for (int i = 0; i < D / 8; ++i) {
-                o[i][0] *= 1.f / PSCALE;
-                o[i][1] *= 1.f / PSCALE;
-            }
-        }
+        flush(1.f / PSCALE);
     }
     // f(head, d, o, m, l) for every value this lane holds; one(head, m, l) once a head.
     template <typename F, typename G>
@@ -320,26 +407,23 @@ __device__ __forceinline__ void round_to(float v, __nv_bfloat16 &d) { d = __floa
 
 template <typename T, int NQ, int GP_>
 struct core_tile {
-    static constexpr int KEYS = 8, GP = GP_, WARPS = 8, NS = 0;  // NS 0: chosen by the shared memory a stage takes
+    static constexpr int KEYS = 8, GP = GP_, ELEM = sizeof(T), WARPS = NQ == 1 ? 16 : 8;
     float acc[NQ][GP][4], m[GP / 4], l[GP / 4];
-    unsigned heads_;
 
     // A row in shared memory: an odd number of 16-byte chunks, so that eight keys meet eight bank
     // groups; its tail past head_dim is zero.
     static __host__ __device__ int row_bytes(int D) { return (((D * (int)sizeof(T) + 15) / 16) | 1) * 16; }
-    static __host__ __device__ int stage_bytes(int D, int) { return 2 * KEYS * row_bytes(D); }
     static __host__ __device__ int dpad(int D) { return (D + 3) & ~3; }
     // per warp beside the stages: q, the tile's weights, the heads' corrections
     static __host__ __device__ int extra_bytes(int D) { return (GP * dpad(D) + KEYS * GP + GP) * 4; }
 
     __device__ __forceinline__ void init(const float *q, int heads, const attn_args &a, uint8_t *extra, int lane) {
+        // q as [four channels][head][4], so that a lane's loop has fixed offsets
         auto *qs = reinterpret_cast<float *>(extra);
-        const int dp = dpad(a.D);
         __syncwarp();
-        for (int i = lane; i < GP * dp; i += 32) {
-            const int h = i / dp, d = i - h * dp;
-            qs[i] = h < heads && d < a.D ? q[(size_t)h * a.D + d] : 0.f;
-        }
+        for (int d = lane; d < dpad(a.D); d += 32)
+#pragma unroll
+            for (int h = 0; h < GP; ++h) qs[(d >> 2) * (4 * GP) + h * 4 + (d & 3)] = h < heads && d < a.D ? q[(size_t)h * a.D + d] : 0.f;
 #pragma unroll
         for (int i = 0; i < NQ; ++i)
 #pragma unroll
@@ -351,41 +435,50 @@ struct core_tile {
         }
         __syncwarp();
     }
-    static __device__ __forceinline__ void load(uint8_t *stage, const attn_args &a, long long off, int lane) {
-        const int rb = row_bytes(a.D), bytes = a.D * (int)sizeof(T);
-        const int align = (int)((reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) | (uintptr_t)bytes) & 15);
-        // rows start where their size and the pools allow: 16- or 4-byte copies, else element by element
-        const int w = align == 0 ? 16 : (align & 3) == 0 ? 4 : 2;
+    static __device__ __forceinline__ void load_run(uint8_t *stage, const uint8_t *src, long long to_v, const attn_args &a, int lane) {
+        const int rb = row_bytes(a.D);
+        const unsigned s0 = smem_u32(stage);
+        for (unsigned c = lane * 16; c < a.head_bytes; c += 512) {
+            const uint8_t *p = src + c;
+#pragma unroll
+            for (int r = 0; r < KEYS; ++r, p += a.token_bytes) {
+                cp_async16(s0 + r * rb + c, p);
+                cp_async16(s0 + (KEYS + r) * rb + c, p + to_v);
+            }
+        }
+    }
+    static __device__ __forceinline__ void load_rows(uint8_t *stage, long long off, const attn_args &a, int lane) {
+        const int rb = row_bytes(a.D);
+#pragma unroll 1
         for (int r = 0; r < KEYS; ++r) {
             const long long b = __shfl_sync(0xffffffffu, off, r);
             const size_t src = b < 0 ? 0 : (size_t)b;
-            uint8_t *kr = stage + r * rb, *vr = stage + (KEYS + r) * rb;
-            if (w > 2) {
-                for (int c = lane * w; c < bytes; c += 32 * w) {
-                    cp_async(kr + c, a.k + src + c, w, b >= 0);
-                    cp_async(vr + c, a.v + src + c, w, b >= 0);
+            uint8_t *kr = stage + r * rb, *vr = kr + KEYS * rb;
+            if (a.unit == 16) {
+                for (unsigned c = lane * 16; c < a.head_bytes; c += 512) {
+                    cp_async16z(smem_u32(kr + c), a.k + src + c, b >= 0);
+                    cp_async16z(smem_u32(vr + c), a.v + src + c, b >= 0);
+                }
+            } else if (a.unit == 4) {
+                for (unsigned c = lane * 4; c < a.head_bytes; c += 128) {
+                    cp_async4z(smem_u32(kr + c), a.k + src + c, b >= 0);
+                    cp_async4z(smem_u32(vr + c), a.v + src + c, b >= 0);
                 }
             } else {
-                for (int c = lane * 2; c < bytes; c += 64) {
+                for (unsigned c = lane * 2; c < a.head_bytes; c += 64) {
                     *reinterpret_cast<uint16_t *>(kr + c) = b >= 0 ? *reinterpret_cast<const uint16_t *>(a.k + src + c) : uint16_t(0);
                     *reinterpret_cast<uint16_t *>(vr + c) = b >= 0 ? *reinterpret_cast<const uint16_t *>(a.v + src + c) : uint16_t(0);
                 }
             }
         }
     }
-    static __device__ __forceinline__ void put_new(uint8_t *stage, const attn_args &a, int r, const float *kn, const float *vn,
-                                                   long long dst, bool store, int lane) {
-        const int rb = row_bytes(a.D);
-        auto *kr = reinterpret_cast<T *>(stage + r * rb), *vr = reinterpret_cast<T *>(stage + (KEYS + r) * rb);
+    static __device__ __forceinline__ void round_row(const float *x, uint8_t *stage, int r, uint8_t *slot, const attn_args &a, int lane) {
         for (int d = lane; d < a.D; d += 32) {
-            round_to(kn[d], kr[d]);
-            round_to(vn[d], vr[d]);
-            if (store) {
-                reinterpret_cast<T *>(a.k + dst)[d] = kr[d];
-                reinterpret_cast<T *>(a.v + dst)[d] = vr[d];
-            }
+            T v;
+            round_to(x[d], v);
+            reinterpret_cast<T *>(stage + r * row_bytes(a.D))[d] = v;
+            if (slot) reinterpret_cast<T *>(slot)[d] = v;
         }
-        __syncwarp();
     }
     __device__ __forceinline__ void step(const uint8_t *stage, unsigned live, const attn_args &a, uint8_t *extra, int lane) {
         const int D = a.D, dp = dpad(D), rb = row_bytes(D);
@@ -395,11 +488,13 @@ struct core_tile {
         float s[GP];
 #pragma unroll
         for (int h = 0; h < GP; ++h) s[h] = 0.f;
-        for (int c = 4 * cl; c < dp; c += 16) {
+        const float *qc = qs + 4 * cl * GP;
+#pragma unroll 2
+        for (int c = 4 * cl; c < dp; c += 16, qc += 16 * GP) {
             const float4 kv = four(kr + c);
 #pragma unroll
             for (int h = 0; h < GP; ++h) {
-                const float4 qv = *reinterpret_cast<const float4 *>(qs + h * dp + c);
+                const float4 qv = *reinterpret_cast<const float4 *>(qc + 4 * h);
                 s[h] = fmaf(qv.x, kv.x, fmaf(qv.y, kv.y, fmaf(qv.z, kv.z, fmaf(qv.w, kv.w, s[h]))));
             }
         }
@@ -416,32 +511,44 @@ struct core_tile {
             x[h] = mine + __shfl_xor_sync(0xffffffffu, other, 1);
         }
         const bool in = live >> key & 1;
+        bool up = false;
 #pragma unroll
         for (int h = 0; h < GP / 4; ++h) {
-            const float sv = in ? x[h] * a.scale2 : -INFINITY;
-            float mt = sv;
-            mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 4));
-            mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 8));
-            mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 16));
-            const float mn = fmaxf(m[h], mt), base = mn == -INFINITY ? 0.f : mn;
-            const float corr = exp2f(m[h] - base), p = exp2f(sv - base);
-            l[h] = l[h] * corr + p;
-            m[h] = mn;
-            ps[key * GP + cl * (GP / 4) + h] = p;
-            if (key == 0) cs[cl * (GP / 4) + h] = corr;
+            x[h] = in ? x[h] * a.scale2 : -INFINITY;
+            up |= x[h] > m[h] + LAZY;
         }
-        __syncwarp();
+        if (__any_sync(0xffffffffu, up)) {
 #pragma unroll
-        for (int h = 0; h < GP; ++h) {
-            const float corr = cs[h];
+            for (int h = 0; h < GP / 4; ++h) {
+                float mt = x[h];
+                mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 4));
+                mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 8));
+                mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 16));
+                const float mn = fmaxf(m[h], mt), corr = ex2(m[h] - (mn == -INFINITY ? 0.f : mn));
+                l[h] *= corr;
+                m[h] = mn;
+                if (key == 0) cs[cl * (GP / 4) + h] = corr;
+            }
+            __syncwarp();
 #pragma unroll
-            for (int i = 0; i < NQ; ++i) {
-                acc[i][h][0] *= corr;
-                acc[i][h][1] *= corr;
-                acc[i][h][2] *= corr;
-                acc[i][h][3] *= corr;
+            for (int h = 0; h < GP; ++h) {
+                const float corr = cs[h];
+#pragma unroll
+                for (int i = 0; i < NQ; ++i) {
+                    acc[i][h][0] *= corr;
+                    acc[i][h][1] *= corr;
+                    acc[i][h][2] *= corr;
+                    acc[i][h][3] *= corr;
+                }
             }
         }
+#pragma unroll
+        for (int h = 0; h < GP / 4; ++h) {
+            const float p = ex2(x[h] - (m[h] == -INFINITY ? 0.f : m[h]));
+            l[h] += p;
+            ps[key * GP + cl * (GP / 4) + h] = p;
+        }
+        __syncwarp();
 #pragma unroll
         for (int k = 0; k < KEYS; ++k) {
             const T *vr = reinterpret_cast<const T *>(stage + (KEYS + k) * rb);
@@ -497,16 +604,18 @@ struct core_tile {
 
 // ---- the kernel over the line of tiles --------------------------------------------------------
 
-// Shared memory: the tile prefix, then per warp its stages, then per warp the heads' sums, the
-// stages' live masks and what the tile keeps (q), then the accumulators that warps of one head add.
+// Shared memory: scan words and the tile prefix, then per warp its stages (KEYS rows of K, KEYS of V), then per
+// warp the stages' live masks, the heads' sums and what the tile keeps (q), then the
+// accumulators that warps of one head add.
+constexpr int MAX_NS = 4;  // masks kept a warp
 struct smem_layout {
     int ring, warp, warp_bytes, merge, total;
 };
 __host__ __device__ inline smem_layout layout_of(int n_seq, int warps, int ns, int stage, int extra, int gp, int merge_warps, int D) {
     smem_layout s;
-    s.ring = (((n_seq + 31) & ~31) + 1) * 4 + 127 & ~127;
+    s.ring = (128 + (((n_seq + 31) & ~31) + 1) * 4 + 511) & ~511;  // rows of up to 512 bytes start on a multiple of their size
     s.warp = s.ring + warps * ns * stage;
-    s.warp_bytes = (3 * gp * 4 + 16 + extra + 15) & ~15;
+    s.warp_bytes = (MAX_NS * 4 + 3 * gp * 4 + extra + 15) & ~15;
     s.merge = s.warp + warps * s.warp_bytes;
     s.total = s.merge + merge_warps * gp * D * 4;
     return s;
@@ -515,35 +624,34 @@ __host__ __device__ inline smem_layout layout_of(int n_seq, int warps, int ns, i
 template <class Tile, int MINB>
 __global__ void __launch_bounds__(Tile::WARPS * 32, MINB)
     k_attn_batch(const __grid_constant__ attn_args a, const __grid_constant__ seq_list L, int ns) {
-    extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ int sums[32];
+    extern __shared__ __align__(1024) uint8_t smem[];
     constexpr int KEYS = Tile::KEYS, GP = Tile::GP;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     const int D = a.D, HG = a.hg, R = a.rsplit, hs = warp % HG, r = warp / HG;
-    if constexpr (Tile::NS > 0) ns = Tile::NS;
-    const int stage_bytes = Tile::stage_bytes(D, 0);
+    const int pitch = Tile::row_bytes(D), stage_bytes = 2 * KEYS * pitch;
     const smem_layout S = layout_of((int)a.n_seq, warps, ns, stage_bytes, Tile::extra_bytes(D), GP, warps - HG, D);
-    int *pre = reinterpret_cast<int *>(smem);
+    int *sums = reinterpret_cast<int *>(smem), *pre = sums + 32;
     uint8_t *ring = smem + S.ring + warp * ns * stage_bytes;
-    auto warp_heads = [&](int w) { return reinterpret_cast<float *>(smem + S.warp + w * S.warp_bytes); };
+    uint8_t *mine = smem + S.warp + warp * S.warp_bytes;
+    auto *masks = reinterpret_cast<unsigned *>(mine);
+    auto warp_heads = [&](int w) { return reinterpret_cast<float *>(smem + S.warp + w * S.warp_bytes + MAX_NS * 4); };
     float *hm = warp_heads(warp), *hl = hm + GP, *ff = hl + GP;
-    unsigned *masks = reinterpret_cast<unsigned *>(ff + GP);
-    uint8_t *extra = reinterpret_cast<uint8_t *>(masks + 4);
-    if constexpr (Tile::NS == 0) {  // rows' tails past head_dim stay zero
+    uint8_t *extra = reinterpret_cast<uint8_t *>(ff + GP);
+    // core rows' tails past head_dim hold zeros
+    if (D * (int)Tile::ELEM % 16)
         for (int i = threadIdx.x * 16; i < warps * ns * stage_bytes; i += blockDim.x * 16)
             *reinterpret_cast<uint4 *>(smem + S.ring + i) = make_uint4(0, 0, 0, 0);
-    }
     pdl_trigger();
     pdl_wait();
 
-    // The line of tiles: R x KEYS keys each, rows in batch order, the head groups one after another.
+    // The line of tiles: R x KEYS keys each, from a multiple of KEYS on, rows in batch order, the head groups one after another.
     int run = 0;
     for (unsigned b = 0; b < a.n_seq; b += blockDim.x) {
         const unsigned i = b + threadIdx.x;
         unsigned row, lo = 0, hi = 0;
         if (i < a.n_seq) span_of(a, L, i, row, lo, hi);
         int total;
-        const int upto = block_scan((int)((hi - lo + R * KEYS - 1) / (R * KEYS)), sums, &total);
+        const int upto = block_scan(lo < hi ? (int)((hi - lo / KEYS * KEYS + R * KEYS - 1) / (R * KEYS)) : 0, sums, &total);
         if (i < a.n_seq) pre[i + 1] = run + upto;
         run += total;
     }
@@ -588,12 +696,13 @@ __global__ void __launch_bounds__(Tile::WARPS * 32, MINB)
         lhead = (size_t)((lh * HG + hs) / a.subs) * a.head_bytes;
         lend = lh * line + pre[ls + 1];
     };
-    // the table entry of the next tile's key, asked for one tile early
+    // the table entry of the next tile's key `lane`, asked for one tile early
+    const long long to_v = a.v - a.k;
     auto look_up = [&]() {
         const unsigned t = (unsigned)(lg - lh * line - pre[ls]);
-        const unsigned j = llo + (t * R + r) * KEYS + lane;
+        const unsigned j = llo / KEYS * KEYS + (t * R + r) * KEYS + lane;
         lpage = NO_PAGE;
-        if (lane < KEYS && j < lhi) {
+        if (lane < KEYS && j >= llo && j < lhi) {
             const unsigned e = j / a.pt;
             lslot = j - e * a.pt;
             lpage = ltab[e];
@@ -604,8 +713,10 @@ __global__ void __launch_bounds__(Tile::WARPS * 32, MINB)
             const bool in = lpage < a.n_pages;
             const long long off = in ? (long long)(((size_t)lpage * a.pt + lslot) * a.token_bytes + lhead) : -1;
             const unsigned mask = __ballot_sync(0xffffffffu, in);
+            uint8_t *stage = ring + lstage * stage_bytes;
             if (lane == 0) masks[lstage] = mask;
-            Tile::load(ring + lstage * stage_bytes, a, off, lane);
+            if (a.one_page && mask == (1u << KEYS) - 1) Tile::load_run(stage, a.k + __shfl_sync(0xffffffffu, off, 0), to_v, a, lane);
+            else Tile::load_rows(stage, off, a, lane);
             lstage = lstage + 1 == ns ? 0 : lstage + 1;
             if (++lg < g1) {
                 if (lg == lend) {
@@ -637,14 +748,14 @@ __global__ void __launch_bounds__(Tile::WARPS * 32, MINB)
             else cp_wait<1>();
             __syncwarp();
             uint8_t *stage = ring + cstage * stage_bytes;
-            const unsigned live = masks[cstage];
-            const unsigned j0 = lo + ((unsigned)(g - u0) * R + r) * KEYS;
+            const unsigned live = masks[cstage], j0 = lo / KEYS * KEYS + ((unsigned)(g - u0) * R + r) * KEYS;
             if (newest >= j0 && newest - j0 < KEYS && (live >> (newest - j0) & 1)) {
-                const unsigned page = a.tables[(size_t)row * a.max_pages + newest / a.pt];
-                const size_t head = (size_t)kvh * a.head_bytes;
-                const long long dst = (long long)(((size_t)page * a.pt + newest % a.pt) * a.token_bytes + head);
+                const unsigned page = a.tables[(size_t)row * a.max_pages + newest / a.pt], at = newest - j0;
+                const size_t dst = ((size_t)page * a.pt + newest % a.pt) * a.token_bytes + (size_t)kvh * a.head_bytes;
                 const size_t src = (size_t)s * a.new_stride + (size_t)kvh * D;
-                Tile::put_new(stage, a, (int)(newest - j0), a.k_new + src, a.v_new + src, dst, sub == 0, lane);
+                Tile::round_row(a.k_new + src, stage, (int)at, sub == 0 ? a.k + dst : nullptr, a, lane);
+                Tile::round_row(a.v_new + src, stage, (int)(KEYS + at), sub == 0 ? a.v + dst : nullptr, a, lane);
+                __syncwarp();
             }
             if (live) tile.step(stage, live, a, extra, lane);
             __syncwarp();
@@ -673,7 +784,7 @@ __global__ void __launch_bounds__(Tile::WARPS * 32, MINB)
                     for (int w = 0; w < R; ++w) M = fmaxf(M, warp_heads(w * HG + hs)[lane]);
                     for (int w = 0; w < R; ++w) {
                         float *o = warp_heads(w * HG + hs);
-                        const float f = o[lane] == -INFINITY ? 0.f : exp2f(o[lane] - M);
+                        const float f = o[lane] == -INFINITY ? 0.f : ex2(o[lane] - M);
                         sum += o[GP + lane] * f;
                         o[2 * GP + lane] = f;
                     }
@@ -683,6 +794,7 @@ __global__ void __launch_bounds__(Tile::WARPS * 32, MINB)
                 __syncwarp();
                 tile.each(lane, a, [&](int hd, int d, float &o) {
                     float v = o * ff[hd];
+#pragma unroll 1
                     for (int w = 1; w < R; ++w) v = fmaf(merge_of(w)[hd * D + d], warp_heads(w * HG + hs)[2 * GP + hd], v);
                     o = v;
                 }, [](int, float, float, bool) {});
@@ -697,8 +809,8 @@ __global__ void __launch_bounds__(Tile::WARPS * 32, MINB)
                     float M = hm[lane], sum = hl[lane], f = 1.f;
                     if (a.sinks) {
                         const float sk = a.sinks[h0 + lane] * LOG2E, top = fmaxf(M, sk);
-                        f = M == -INFINITY ? 0.f : exp2f(M - top);
-                        sum = sum * f + (sk == -INFINITY ? 0.f : exp2f(sk - top));
+                        f = M == -INFINITY ? 0.f : ex2(M - top);
+                        sum = sum * f + (sk == -INFINITY ? 0.f : ex2(sk - top));
                     }
                     ff[lane] = sum == 0.f ? 0.f : f / sum;
                 }
@@ -719,7 +831,6 @@ __global__ void __launch_bounds__(Tile::WARPS * 32, MINB)
         if (R > 1) __syncthreads();  // the sums and accumulators are free for the next row
         else __syncwarp();
     }
-    cp_wait<0>();
 }
 
 // Joins the rows that several CTAs had a part of, in tile order, and writes zeros to empty rows.
@@ -760,13 +871,13 @@ __global__ void __launch_bounds__(JOIN_THREADS) k_attn_join(const __grid_constan
         M = warp_max(M);
         float sum = 0.f;
         for (int k = lane; k < n; k += 32) {
-            const float m = wgt[hd * n + k], f = m == -INFINITY ? 0.f : exp2f(m - M);
+            const float m = wgt[hd * n + k], f = m == -INFINITY ? 0.f : ex2(m - M);
             wgt[hd * n + k] = f;
             sum += part_of(k)[GP * D + 2 * hd + 1] * f;
         }
         sum = warp_sum(sum);
         if (lane == 0) {
-            sum += sk == -INFINITY ? 0.f : exp2f(sk - M);
+            sum += sk == -INFINITY ? 0.f : ex2(sk - M);
             inv[hd] = sum == 0.f ? 0.f : 1.f / sum;
         }
     }
@@ -791,6 +902,9 @@ struct attn_plan {
     int gp, keys, subs, hg, rsplit, nhg, warps, ns, smem, grid;
 };
 
+// f32 rows of up to 128 channels whose kv heads serve four query heads at most take half the
+// arithmetic with tiles of four heads.
+bool few_heads(unsigned D, int group) { return D <= 128 && group <= 4; }
 bool mma_dim(unsigned D) { return D == 64 || D == 80 || D == 96 || D == 128 || D == 256; }
 
 template <class Tile>
@@ -807,24 +921,24 @@ bool cut(attn_plan &p, int warps, int ns, int minb, int n_heads, int n_kv, int D
     p.nhg = V / p.hg;
     p.warps = p.hg * p.rsplit;
     p.ns = ns;
-    p.smem = layout_of(n_seq, p.warps, ns, Tile::stage_bytes(D, 0), Tile::extra_bytes(D), p.gp, p.warps - p.hg, D).total;
+    p.smem = layout_of(n_seq, p.warps, ns, 2 * Tile::KEYS * Tile::row_bytes(D), Tile::extra_bytes(D), p.gp, p.warps - p.hg, D).total;
     if (p.smem > MAX_SMEM - 512) return false;
     p.grid = sms * std::max(1, std::min(minb, 233472 / (p.smem + 1536)));
     return true;
 }
 
+// Three stages where the tile's warps have them, else two, else fewer warps.
 template <class Tile>
-bool cut_core(attn_plan &p, int n_heads, int n_kv, int D, int n_seq, int sms) {
-    // three stages where eight warps have them, else two, else fewer warps
-    for (int warps = 8; warps >= 1; warps /= 2)
+bool cut_any(attn_plan &p, int minb, int n_heads, int n_kv, int D, int n_seq, int sms) {
+    for (int warps = Tile::WARPS; warps >= 1; warps /= 2)
         for (int ns = 3; ns >= 2; --ns)
-            if (cut<Tile>(p, warps, ns, 2, n_heads, n_kv, D, n_seq, sms)) return true;
+            if (cut<Tile>(p, warps, ns, minb, n_heads, n_kv, D, n_seq, sms)) return true;
     return false;
 }
 
 // f(Tile, MINB) for the tile that serves a shape.
 template <typename F>
-auto with_tile(bool mma, unsigned kv_type, unsigned D, F &&f) {
+auto with_tile(bool mma, unsigned kv_type, unsigned D, int group, F &&f) {
 #define MMA_CASE(d, mb)                                                                       \
     if (D == d)                                                                               \
         return kv_type == T_BF16 ? f((mma_tile<d, true> *)nullptr, std::integral_constant<int, mb>()) \
@@ -838,7 +952,8 @@ auto with_tile(bool mma, unsigned kv_type, unsigned D, F &&f) {
     }
 #undef MMA_CASE
 #define CORE_CASE(T)                                                                                  \
-    if (D <= 128) return f((core_tile<T, 1, 8> *)nullptr, std::integral_constant<int, 2>());          \
+    if (few_heads(D, group)) return f((core_tile<T, 1, 4> *)nullptr, std::integral_constant<int, 1>()); \
+    if (D <= 128) return f((core_tile<T, 1, 8> *)nullptr, std::integral_constant<int, 1>());          \
     if (D <= 256) return f((core_tile<T, 2, 8> *)nullptr, std::integral_constant<int, 1>());          \
     if (D <= 512) return f((core_tile<T, 4, 4> *)nullptr, std::integral_constant<int, 1>());          \
     return f((core_tile<T, 8, 4> *)nullptr, std::integral_constant<int, 1>());
@@ -853,10 +968,9 @@ auto with_tile(bool mma, unsigned kv_type, unsigned D, F &&f) {
 
 bool plan_of(attn_plan &p, bool mma, unsigned kv_type, int n_heads, int n_kv, int D, int n_seq, int sms) {
     p.mma = mma;
-    return with_tile(mma, kv_type, (unsigned)D, [&](auto *t, auto minb) {
+    return with_tile(mma, kv_type, (unsigned)D, n_heads / n_kv, [&](auto *t, auto minb) {
         using Tile = std::remove_pointer_t<decltype(t)>;
-        if constexpr (Tile::NS > 0) return cut<Tile>(p, Tile::WARPS, Tile::NS, minb(), n_heads, n_kv, D, n_seq, sms);
-        else return cut_core<Tile>(p, n_heads, n_kv, D, n_seq, sms);
+        return cut_any<Tile>(p, minb(), n_heads, n_kv, D, n_seq, sms);
     });
 }
 
@@ -949,6 +1063,9 @@ int moearc_x_attn_decode_batch(moearc_ctx *c, const moearc_x_kv_cache *kv, unsig
     a.n_pages = kv->n_pages;
     a.pt = kv->page_tokens;
     a.cap = cap;
+    const uintptr_t rows = align | a.head_bytes;
+    a.unit = (rows & 15) == 0 ? 16 : (rows & 3) == 0 ? 4 : 2;
+    a.one_page = a.unit == 16 && kv->page_tokens % (unsigned)p.keys == 0;
     a.listed = seqs != nullptr;
     a.n_heads = (int)n_heads;
     a.group = (int)(n_heads / kv->n_kv_heads);
@@ -964,7 +1081,7 @@ int moearc_x_attn_decode_batch(moearc_ctx *c, const moearc_x_kv_cache *kv, unsig
     device_guard g(c->device);
     if (!g.ok) return ERR;
     launch_scope ls(c, "attn_decode_batch", n_seq, n_heads);
-    const cudaError_t e = with_tile(mma, kv->kv_type, kv->head_dim, [&](auto *t, auto minb) {
+    const cudaError_t e = with_tile(mma, kv->kv_type, kv->head_dim, a.group, [&](auto *t, auto minb) {
         return launch<std::remove_pointer_t<decltype(t)>, decltype(minb)::value>(c, p, a, L);
     });
     if (e != cudaSuccess) cudaGetLastError();  // the failed launch's error, not left for an unrelated later check
