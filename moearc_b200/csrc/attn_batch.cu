@@ -67,7 +67,8 @@ struct attn_args {
     int min_tiles;
     float scale2;  // scale x log2(e): scores are kept in powers of two
     float *part;   // [CTA][2][hg][GP][D + 2]
-    int *pre;      // [n_seq + 1] tile prefix, [n_seq + 1] = CTAs that work
+    int4 *info;    // [CTA] the row its run begins in: batch row, head group, first tile, the one after the last
+    int *shape;    // tiles, CTAs that work
 };
 
 // The keys [lo, hi) of batch row i in cache row `row`, hi cut to the table.
@@ -77,12 +78,16 @@ __device__ __forceinline__ void span_of(const attn_args &a, const seq_list &L, u
     lo = a.begin ? min(a.begin[i], hi) : 0;
 }
 
-// CTA c's run of the `total` tiles over `ctas` CTAs: the first total % ctas take one more.
-__device__ __forceinline__ long run_start(long total, int ctas, int c) { return total / ctas * c + min((long)c, total % ctas); }
-__device__ __forceinline__ int run_owner(long total, int ctas, long g) {
-    const long b = total / ctas, r = total % ctas;
-    return (int)(g < r * (b + 1) ? g / (b + 1) : r + (g - r * (b + 1)) / b);
-}
+// The line's tiles over `ctas` CTAs: each takes `each` of them, the first `more` one more.
+struct runs {
+    int each, more;
+    __device__ __forceinline__ runs(int total, int ctas) : each(total / ctas), more(total - total / ctas * ctas) {}
+    __device__ __forceinline__ int start(int c) const { return each * c + min(c, more); }
+    __device__ __forceinline__ int owner(int g) const {
+        const int cut = more * (each + 1);
+        return g < cut ? g / (each + 1) : more + (g - cut) / each;
+    }
+};
 
 // 16 (or 4) bytes global -> shared, zeros in their place where the source is not to be read.
 __device__ __forceinline__ void cp_async16(unsigned dst, const void *src) {
@@ -323,13 +328,18 @@ struct mma_tile {
                 s[2 * n + e] = in >> (8 * n + e) & 1 ? x : -INFINITY;
             }
         float mt = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
-        if (__any_sync(0xffffffffu, mt > m + LAZY)) {
-            mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
-            mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 2));
-            const float mn = fmaxf(m, mt), corr = ex2(m - (mn == -INFINITY ? 0.f : mn));
+        const bool up = __any_sync(0xffffffffu, mt > m + LAZY);
+        if (up || (CHAIN > 1 && chained == CHAIN)) {
+            float corr = 1.f;
+            if (up) {
+                mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
+                mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 2));
+                const float mn = fmaxf(m, mt);
+                corr = ex2(m - (mn == -INFINITY ? 0.f : mn));
+                l *= corr;
+                m = mn;
+            }
             flush(corr);
-            l *= corr;
-            m = mn;
         }
         const float base = m == -INFINITY ? 0.f : m;
         float p[4];
@@ -357,7 +367,7 @@ struct mma_tile {
                 }
             }
         }
-        if (CHAIN > 1 && ++chained == CHAIN) flush(1.f);
+        ++chained;
     }
 
     // After the last tile: l summed over the head's lanes, o without its scale.
@@ -605,9 +615,9 @@ struct core_tile {
 // ---- the kernel over the line of tiles --------------------------------------------------------
 
 // Shared memory: scan words and the tile prefix, then per warp its stages (KEYS rows of K, KEYS of V), then per
-// warp the stages' live masks, the heads' sums and what the tile keeps (q), then the
+// warp the the stages' live masks and the new token's place, the heads' sums and what the tile keeps (q), then the
 // accumulators that warps of one head add.
-constexpr int MAX_NS = 4;  // masks kept a warp
+constexpr int MAX_NS = 4;  // masks and places kept a warp
 struct smem_layout {
     int ring, warp, warp_bytes, merge, total;
 };
@@ -615,7 +625,7 @@ __host__ __device__ inline smem_layout layout_of(int n_seq, int warps, int ns, i
     smem_layout s;
     s.ring = (128 + (((n_seq + 31) & ~31) + 1) * 4 + 511) & ~511;  // rows of up to 512 bytes start on a multiple of their size
     s.warp = s.ring + warps * ns * stage;
-    s.warp_bytes = (MAX_NS * 4 + 3 * gp * 4 + extra + 15) & ~15;
+    s.warp_bytes = (MAX_NS * 12 + 3 * gp * 4 + extra + 15) & ~15;
     s.merge = s.warp + warps * s.warp_bytes;
     s.total = s.merge + merge_warps * gp * D * 4;
     return s;
@@ -633,8 +643,9 @@ __global__ void __launch_bounds__(Tile::WARPS * 32, MINB)
     int *sums = reinterpret_cast<int *>(smem), *pre = sums + 32;
     uint8_t *ring = smem + S.ring + warp * ns * stage_bytes;
     uint8_t *mine = smem + S.warp + warp * S.warp_bytes;
-    auto *masks = reinterpret_cast<unsigned *>(mine);
-    auto warp_heads = [&](int w) { return reinterpret_cast<float *>(smem + S.warp + w * S.warp_bytes + MAX_NS * 4); };
+    auto *slots = reinterpret_cast<long long *>(mine);  // the new token's place in a pool, where its tile is
+    auto *masks = reinterpret_cast<unsigned *>(slots + MAX_NS);
+    auto warp_heads = [&](int w) { return reinterpret_cast<float *>(smem + S.warp + w * S.warp_bytes + MAX_NS * 12); };
     float *hm = warp_heads(warp), *hl = hm + GP, *ff = hl + GP;
     uint8_t *extra = reinterpret_cast<uint8_t *>(ff + GP);
     // core rows' tails past head_dim hold zeros
@@ -657,16 +668,23 @@ __global__ void __launch_bounds__(Tile::WARPS * 32, MINB)
     }
     if (threadIdx.x == 0) pre[0] = 0;
     __syncthreads();
-    const long line = run, T = line * a.nhg;
-    const int ctas = (int)min((long)gridDim.x, max(1L, (T + a.min_tiles - 1) / a.min_tiles));
-    if (blockIdx.x == 0)
-        for (unsigned i = threadIdx.x; i < a.n_seq + 2; i += blockDim.x) a.pre[i] = i <= a.n_seq ? pre[i] : ctas;
+    const int line = run, T = line * a.nhg;  // below 2^31: the host has seen to it
+    const int ctas = min((int)gridDim.x, max(1, (T + a.min_tiles - 1) / a.min_tiles));
+    // rows without keys are zero
+    for (int i = blockIdx.x; i < (int)a.n_seq; i += gridDim.x)
+        if (pre[i] == pre[i + 1])
+            for (int e = threadIdx.x; e < a.n_heads * D; e += blockDim.x) a.out[(size_t)i * a.n_heads * D + e] = 0.f;
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        a.shape[0] = T;
+        a.shape[1] = ctas;
+    }
     if ((int)blockIdx.x >= ctas || T == 0) return;
-    const long g0 = run_start(T, ctas, (int)blockIdx.x), g1 = run_start(T, ctas, (int)blockIdx.x + 1);
+    const runs parts(T, ctas);
+    const int g0 = parts.start((int)blockIdx.x), g1 = parts.start((int)blockIdx.x + 1);
 
     int s0;
     {
-        const int x = (int)(g0 % line);
+        const int x = g0 % line;
         int lo = 0, hi = (int)a.n_seq;  // pre[lo] <= x < pre[hi]
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
@@ -675,6 +693,8 @@ __global__ void __launch_bounds__(Tile::WARPS * 32, MINB)
         }
         s0 = lo;
     }
+    const int h0g = g0 / line;
+    if (threadIdx.x == 0) a.info[blockIdx.x] = make_int4(s0, h0g, h0g * line + pre[s0], h0g * line + pre[s0 + 1]);
     auto next_row = [&](int &s, int &h) {
         do {
             if (++s == (int)a.n_seq) {
@@ -685,9 +705,8 @@ __global__ void __launch_bounds__(Tile::WARPS * 32, MINB)
     };
 
     // The loading side runs ns - 1 tiles ahead of the computing side, across rows.
-    long lg = g0, lend;
-    int ls = s0, lh = (int)(g0 / line), lstage = 0;
-    unsigned lrow, llo, lhi, lslot = 0, lpage = NO_PAGE;
+    int lg = g0, lend, ls = s0, lh = h0g, lstage = 0;
+    unsigned lrow, llo, lhi, lslot = 0, lpage = NO_PAGE, lnew;
     const unsigned *ltab;
     size_t lhead;
     auto enter = [&]() {
@@ -695,16 +714,18 @@ __global__ void __launch_bounds__(Tile::WARPS * 32, MINB)
         ltab = a.tables + (size_t)lrow * a.max_pages;
         lhead = (size_t)((lh * HG + hs) / a.subs) * a.head_bytes;
         lend = lh * line + pre[ls + 1];
+        lnew = a.k_new ? a.n_kv[lrow] - 1 : 0xffffffffu;
     };
     // the table entry of the next tile's key `lane`, asked for one tile early
     const long long to_v = a.v - a.k;
+    unsigned lj = 0;
     auto look_up = [&]() {
         const unsigned t = (unsigned)(lg - lh * line - pre[ls]);
-        const unsigned j = llo / KEYS * KEYS + (t * R + r) * KEYS + lane;
+        lj = llo / KEYS * KEYS + (t * R + r) * KEYS + lane;
         lpage = NO_PAGE;
-        if (lane < KEYS && j >= llo && j < lhi) {
-            const unsigned e = j / a.pt;
-            lslot = j - e * a.pt;
+        if (lane < KEYS && lj >= llo && lj < lhi) {
+            const unsigned e = lj / a.pt;
+            lslot = lj - e * a.pt;
             lpage = ltab[e];
         }
     };
@@ -715,6 +736,7 @@ __global__ void __launch_bounds__(Tile::WARPS * 32, MINB)
             const unsigned mask = __ballot_sync(0xffffffffu, in);
             uint8_t *stage = ring + lstage * stage_bytes;
             if (lane == 0) masks[lstage] = mask;
+            if (in && lj == lnew) slots[lstage] = off;
             if (a.one_page && mask == (1u << KEYS) - 1) Tile::load_run(stage, a.k + __shfl_sync(0xffffffffu, off, 0), to_v, a, lane);
             else Tile::load_rows(stage, off, a, lane);
             lstage = lstage + 1 == ns ? 0 : lstage + 1;
@@ -730,12 +752,11 @@ __global__ void __launch_bounds__(Tile::WARPS * 32, MINB)
     };
     enter();
     look_up();
-    for (int i = 0; i < ns - 1; ++i) issue();
 
     Tile tile;
-    int s = s0, h = (int)(g0 / line), cstage = 0;
-    for (long g = g0; g < g1; next_row(s, h)) {
-        const long u0 = h * line + pre[s], u1 = h * line + pre[s + 1], first = g, end = min(u1, g1);
+    int s = s0, h = h0g, cstage = 0, ahead = ns - 1;
+    for (int g = g0; g < g1; next_row(s, h)) {
+        const int u0 = h * line + pre[s], u1 = h * line + pre[s + 1], first = g, end = min(u1, g1);
         unsigned row, lo, hi;
         span_of(a, L, (unsigned)s, row, lo, hi);
         const int vh = h * HG + hs, kvh = vh / a.subs, sub = vh - kvh * a.subs;
@@ -743,15 +764,16 @@ __global__ void __launch_bounds__(Tile::WARPS * 32, MINB)
         const unsigned newest = a.k_new ? a.n_kv[row] - 1 : 0xffffffffu;
         tile.init(a.q + (size_t)s * a.q_stride + (size_t)h0 * D, heads, a, extra, lane);
         for (; g < end; ++g) {
-            issue();
+            for (; ahead >= 0; --ahead) issue();  // one a tile, ns before the first
+            ahead = 0;
             if (ns == 3) cp_wait<2>();
             else cp_wait<1>();
             __syncwarp();
             uint8_t *stage = ring + cstage * stage_bytes;
             const unsigned live = masks[cstage], j0 = lo / KEYS * KEYS + ((unsigned)(g - u0) * R + r) * KEYS;
             if (newest >= j0 && newest - j0 < KEYS && (live >> (newest - j0) & 1)) {
-                const unsigned page = a.tables[(size_t)row * a.max_pages + newest / a.pt], at = newest - j0;
-                const size_t dst = ((size_t)page * a.pt + newest % a.pt) * a.token_bytes + (size_t)kvh * a.head_bytes;
+                const unsigned at = newest - j0;
+                const size_t dst = (size_t)slots[cstage];
                 const size_t src = (size_t)s * a.new_stride + (size_t)kvh * D;
                 Tile::round_row(a.k_new + src, stage, (int)at, sub == 0 ? a.k + dst : nullptr, a, lane);
                 Tile::round_row(a.v_new + src, stage, (int)(KEYS + at), sub == 0 ? a.v + dst : nullptr, a, lane);
@@ -833,38 +855,34 @@ __global__ void __launch_bounds__(Tile::WARPS * 32, MINB)
     }
 }
 
-// Joins the rows that several CTAs had a part of, in tile order, and writes zeros to empty rows.
-// CTA (batch row, virtual head).
+// Joins the rows that several CTAs had a part of, in tile order. CTA (c, virtual head of the group,
+// share of the channels): the row that CTA c's run begins inside, if c is the first to do so.
 constexpr int JOIN_THREADS = 256;
 template <int GP>
-__global__ void __launch_bounds__(JOIN_THREADS) k_attn_join(const __grid_constant__ attn_args a) {
+__global__ void __launch_bounds__(JOIN_THREADS, 6) k_attn_join(const __grid_constant__ attn_args a) {
     extern __shared__ float wgt[];  // [GP][parts]
     __shared__ float inv[GP];
     pdl_trigger();
     pdl_wait();
-    const int i = blockIdx.x, vh = blockIdx.y, D = a.D, HG = a.hg;
-    const int hgi = vh / HG, hs = vh - hgi * HG, kvh = vh / a.subs, sub = vh - kvh * a.subs;
+    const int T = a.shape[0], ctas = a.shape[1], c = blockIdx.x + 1, hs = blockIdx.y;
+    if (c >= ctas) return;
+    const int4 at = a.info[c];  // batch row, head group, the row's first tile and the one after its last
+    const runs parts(T, ctas);
+    if (parts.start(c) == at.z || parts.start(c - 1) > at.z) return;
+    const int D = a.D, HG = a.hg, n = parts.owner(at.w - 1) - c + 2;
+    const int vh = at.y * HG + hs, kvh = vh / a.subs, sub = vh - kvh * a.subs;
     const int h0 = kvh * a.group + sub * GP, heads = min(GP, a.group - sub * GP);
-    float *out = a.out + ((size_t)i * a.n_heads + h0) * D;
-    const long line = a.pre[a.n_seq], T = line * a.nhg, u0 = hgi * line + a.pre[i], u1 = hgi * line + a.pre[i + 1];
-    if (u0 == u1) {
-        for (int e = threadIdx.x; e < heads * D; e += JOIN_THREADS) out[e] = 0.f;
-        return;
-    }
-    const int ctas = a.pre[a.n_seq + 1], c0 = run_owner(T, ctas, u0), c1 = run_owner(T, ctas, u1 - 1), n = c1 - c0 + 1;
-    if (n == 1) return;
-    const size_t rec = (size_t)GP * (D + 2);
-    // the first CTA's part is its second record unless its run begins inside the row
-    auto part_of = [&](int k) {
-        const int c = c0 + k, slot = k > 0 || run_start(T, ctas, c) >= u0 ? 0 : 1;
-        return a.part + (((size_t)c * 2 + slot) * HG + hs) * rec;
-    };
+    // CTA c - 1's part is its second record unless its run begins with the row; the others' their first
+    const size_t rec = (size_t)GP * (D + 2), step = (size_t)2 * HG * rec;
+    const float *rest = a.part + (size_t)c * step + hs * rec;
+    const float *part0 = rest - step + (parts.start(c - 1) == at.z ? 0 : HG * rec);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     for (int hd = warp; hd < heads; hd += JOIN_THREADS / 32) {
         const float sk = a.sinks ? a.sinks[h0 + hd] * LOG2E : -INFINITY;
+        const size_t ml = (size_t)GP * D + 2 * hd;
         float M = sk;
         for (int k = lane; k < n; k += 32) {
-            const float m = part_of(k)[GP * D + 2 * hd];
+            const float m = (k ? rest + (size_t)(k - 1) * step : part0)[ml];
             wgt[hd * n + k] = m;
             M = fmaxf(M, m);
         }
@@ -873,7 +891,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) k_attn_join(const __grid_constan
         for (int k = lane; k < n; k += 32) {
             const float m = wgt[hd * n + k], f = m == -INFINITY ? 0.f : ex2(m - M);
             wgt[hd * n + k] = f;
-            sum += part_of(k)[GP * D + 2 * hd + 1] * f;
+            sum += (k ? rest + (size_t)(k - 1) * step : part0)[ml + 1] * f;
         }
         sum = warp_sum(sum);
         if (lane == 0) {
@@ -882,12 +900,11 @@ __global__ void __launch_bounds__(JOIN_THREADS) k_attn_join(const __grid_constan
         }
     }
     __syncthreads();
-    const float *rest = n > 1 ? part_of(1) : nullptr;  // parts after the first are 2 HG rec apart
-    const size_t step = (size_t)2 * HG * rec;
-    for (int e = threadIdx.x; e < heads * D; e += JOIN_THREADS) {
+    float *out = a.out + ((size_t)at.x * a.n_heads + h0) * D;
+    for (int e = blockIdx.z * JOIN_THREADS + threadIdx.x; e < heads * D; e += gridDim.z * JOIN_THREADS) {
         const int hd = e / D;
         const float *w = wgt + hd * n;
-        float v = part_of(0)[e] * w[0];
+        float v = part0[e] * w[0];
 #pragma unroll 8
         for (int k = 1; k < n; ++k) v = fmaf(rest[(size_t)(k - 1) * step + e], w[k], v);
         out[e] = v * inv[hd];
@@ -974,17 +991,22 @@ bool plan_of(attn_plan &p, bool mma, unsigned kv_type, int n_heads, int n_kv, in
     });
 }
 
-constexpr size_t PRE_BYTES = ((KV_LIST + 2) * 4 + 255) / 256 * 256;
-size_t attn_bytes(const attn_plan &p, int D) { return PRE_BYTES + (size_t)p.grid * 2 * p.hg * p.gp * (D + 2) * 4; }
+// The work buffer: the line's shape, a note a CTA, the parts.
+size_t attn_bytes(const attn_plan &p, int D) { return 16 + (size_t)p.grid * 16 + (size_t)p.grid * 2 * p.hg * p.gp * (D + 2) * 4; }
 
 template <class Tile, int MINB>
 cudaError_t launch(moearc_ctx *c, const attn_plan &p, const attn_args &a, const seq_list &L) {
     static std::atomic<bool> done[MOEARC_MAX_DEVICES];
-    cudaError_t e = once_per_device(done, [] { return set_smem(k_attn_batch<Tile, MINB>, MAX_SMEM - 512); });
+    cudaError_t e = once_per_device(done, [] {
+        const cudaError_t e1 = set_smem(k_attn_batch<Tile, MINB>, MAX_SMEM - 512);
+        // the join's few KB under the same split of L1 and shared memory: with the default one its
+        // CTAs run one at a time on an SM
+        return e1 != cudaSuccess ? e1 : set_smem(k_attn_join<Tile::GP>, 40 * 1024);
+    });
     if (e == cudaSuccess)
         e = launch_pdl(k_attn_batch<Tile, MINB>, dim3((unsigned)p.grid), dim3((unsigned)p.warps * 32), (size_t)p.smem, c->stream, a, L, p.ns);
-    if (e == cudaSuccess)
-        e = launch_pdl(k_attn_join<Tile::GP>, dim3(a.n_seq, (unsigned)(p.hg * p.nhg)), dim3(JOIN_THREADS),
+    if (e == cudaSuccess && p.grid > 1)
+        e = launch_pdl(k_attn_join<Tile::GP>, dim3((unsigned)p.grid - 1, (unsigned)p.hg, (Tile::GP * a.D + 511) / 512), dim3(JOIN_THREADS),
                        (size_t)Tile::GP * p.grid * 4, c->stream, a);
     return e;
 }
@@ -1041,7 +1063,7 @@ int moearc_x_attn_decode_batch(moearc_ctx *c, const moearc_x_kv_cache *kv, unsig
     if (!plan_of(p, mma, kv->kv_type, (int)n_heads, (int)kv->n_kv_heads, (int)D, (int)n_seq, c->sm_count)) return ERR_ARG;
     if (kv->work_bytes < attn_bytes(p, (int)D)) return ERR_ARG;
     const unsigned cap = kv->max_pages * kv->page_tokens;
-    if ((unsigned long long)n_seq * (cap / (unsigned)(p.keys * p.rsplit) + 1) >= (1ull << 31)) return ERR_ARG;
+    if ((unsigned long long)n_seq * (cap / (unsigned)(p.keys * p.rsplit) + 2) * p.nhg >= (1ull << 31)) return ERR_ARG;
 
     attn_args a;
     a.out = out;
@@ -1076,8 +1098,9 @@ int moearc_x_attn_decode_batch(moearc_ctx *c, const moearc_x_kv_cache *kv, unsig
     a.nhg = p.nhg;
     a.min_tiles = 1;
     a.scale2 = scale * LOG2E;
-    a.pre = static_cast<int *>(kv->work);
-    a.part = reinterpret_cast<float *>(static_cast<uint8_t *>(kv->work) + PRE_BYTES);
+    a.shape = static_cast<int *>(kv->work);
+    a.info = reinterpret_cast<int4 *>(a.shape + 4);
+    a.part = reinterpret_cast<float *>(a.info + p.grid);
     device_guard g(c->device);
     if (!g.ok) return ERR;
     launch_scope ls(c, "attn_decode_batch", n_seq, n_heads);
