@@ -655,7 +655,8 @@ int moearc_x_attn_decode_static(moearc_ctx *c, float *out, const float *q, const
  * copied into the launch by value (a captured graph keeps them). What depends on device state is
  * checked there: a call that cannot be done has no effect at all and raises a bit of *status:
  * MOEARC_X_KV_FULL (too few free pages), MOEARC_X_KV_LONG (a row past its table), MOEARC_X_KV_TAKEN
- * (a fork onto a row that holds tokens). New pages are the free pages of lowest id, in list order.
+ * (a fork onto a row that holds tokens). MOEARC_X_KV_WAIT is none of these: a kernel's wait for its
+ * own copies ran out, and what it computed is invalid. New pages are the free pages of lowest id, in list order.
  * All calls are enqueued on the context's stream; the same cache must not be changed from two
  * streams at once, and calls that may overlap need a work buffer each. */
 #define MOEARC_X_NO_PAGE 0xFFFFFFFFu
@@ -664,6 +665,7 @@ int moearc_x_attn_decode_static(moearc_ctx *c, float *out, const float *q, const
 #define MOEARC_X_KV_FULL 1u
 #define MOEARC_X_KV_LONG 2u
 #define MOEARC_X_KV_TAKEN 4u
+#define MOEARC_X_KV_WAIT 8u
 typedef struct {
     void *const *k_pages;      /* HOST arrays of n_layer device pointers; a pool's pages hold */
     void *const *v_pages;      /* page_tokens x n_kv_heads x head_dim elements each */

@@ -32,7 +32,7 @@
 #include <cmath>
 #include <type_traits>
 
-#include "kvcache.cuh"
+#include "attn_batch.cuh"
 
 using namespace moearc;
 
@@ -41,75 +41,6 @@ size_t kv_page_work_bytes(unsigned n_pages);
 }
 
 namespace {
-
-constexpr float LOG2E = 1.4426950408889634f;
-constexpr int MAX_SMEM = 227 * 1024;
-// A row's weights are taken against a reference that follows its maximum only once that is this much
-// above (in powers of two): most tiles then rescale nothing, and weights stay below 2^8.
-constexpr float LAZY = 8.f;
-
-struct seq_list {
-    unsigned row[KV_LIST];
-};
-
-struct attn_args {
-    float *out;
-    const float *q, *k_new, *v_new, *sinks;
-    uint8_t *k, *v;  // the layer's pools
-    const unsigned *tables, *n_kv, *begin;
-    size_t q_stride, new_stride, token_bytes, head_bytes;  // bytes: n_kv_heads x head_dim elements, head_dim elements
-    unsigned n_seq, max_pages, n_pages, pt, cap;
-    unsigned unit;  // bytes of one copy: 16 where rows start on 16-byte boundaries, else 4 or 2
-    int one_page;   // tiles never cross a page
-    int listed;  // rows come from the list (else row i is batch row i)
-    int n_heads, group, D, subs;  // subs: virtual heads a kv head (its query heads by GP)
-    int hg, rsplit, nhg;          // virtual heads a CTA, warps a head, head groups
-    int min_tiles;
-    float scale2;  // scale x log2(e): scores are kept in powers of two
-    float *part;   // [CTA][2][hg][GP][D + 2]
-    int4 *info;    // [CTA] the row its run begins in: batch row, head group, first tile, the one after the last
-    int *shape;    // tiles, CTAs that work
-};
-
-// The keys [lo, hi) of batch row i in cache row `row`, hi cut to the table.
-__device__ __forceinline__ void span_of(const attn_args &a, const seq_list &L, unsigned i, unsigned &row, unsigned &lo, unsigned &hi) {
-    row = a.listed ? L.row[i] : i;
-    hi = min(a.n_kv[row], a.cap);
-    lo = a.begin ? min(a.begin[i], hi) : 0;
-}
-
-// The line's tiles over `ctas` CTAs: each takes `each` of them, the first `more` one more.
-struct runs {
-    int each, more;
-    __device__ __forceinline__ runs(int total, int ctas) : each(total / ctas), more(total - total / ctas * ctas) {}
-    __device__ __forceinline__ int start(int c) const { return each * c + min(c, more); }
-    __device__ __forceinline__ int owner(int g) const {
-        const int cut = more * (each + 1);
-        return g < cut ? g / (each + 1) : more + (g - cut) / each;
-    }
-};
-
-// 16 (or 4) bytes global -> shared, zeros in their place where the source is not to be read.
-__device__ __forceinline__ void cp_async16(unsigned dst, const void *src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async16z(unsigned dst, const void *src, bool valid) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_async4z(unsigned dst, const void *src, bool valid) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(dst), "l"(src), "r"(valid ? 4 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory"); }
-__device__ __forceinline__ unsigned smem_u32(const void *p) { return (unsigned)__cvta_generic_to_shared(p); }
-
-// 2^x, subnormal results as 0.
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 
 // ---- the tensor-core tile (16-bit caches) -----------------------------------------------------
 
@@ -129,45 +60,6 @@ __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], unsigned p) {
 __device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], unsigned p) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(p) : "memory");
-}
-
-template <bool BF>
-__device__ __forceinline__ uint16_t to16(float v) {
-    if constexpr (BF) return f32_to_bf16_bits(v);
-    else return __half_as_ushort(__float2half_rn(v));
-}
-template <bool BF>
-__device__ __forceinline__ float from16(uint16_t b) {
-    if constexpr (BF) return bf16_bits_to_f32(b);
-    else return f16_bits_to_f32(b);
-}
-// Two values rounded to 16 bits and packed, and a packed pair's values.
-template <bool BF>
-__device__ __forceinline__ uint32_t pack(float x, float y) {
-    if constexpr (BF) {
-        const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
-        return *reinterpret_cast<const uint32_t *>(&v);
-    } else {
-        const __half2 v = __floats2half2_rn(x, y);
-        return *reinterpret_cast<const uint32_t *>(&v);
-    }
-}
-template <bool BF>
-__device__ __forceinline__ float2 unpack(uint32_t u) {
-    if constexpr (BF) return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
-    else return __half22float2(*reinterpret_cast<const __half2 *>(&u));
-}
-// Two values as packed pairs of 16-bit terms: x = t0 + t1 (+ t2), each term the rounding of what
-// the ones before it leave.
-template <bool BF>
-__device__ __forceinline__ void terms(float x, float y, uint32_t &t0, uint32_t &t1, uint32_t &t2) {
-    t0 = pack<BF>(x, y);
-    const float2 a = unpack<BF>(t0);
-    t1 = pack<BF>(x - a.x, y - a.y);
-    if constexpr (BF) {
-        const float2 b = unpack<BF>(t1);
-        t2 = pack<BF>(x - a.x - b.x, y - a.y - b.y);
-    }
 }
 
 template <int D_, bool BF>
@@ -674,11 +566,10 @@ __global__ void __launch_bounds__(Tile::WARPS * 32, MINB)
     for (int i = blockIdx.x; i < (int)a.n_seq; i += gridDim.x)
         if (pre[i] == pre[i + 1])
             for (int e = threadIdx.x; e < a.n_heads * D; e += blockDim.x) a.out[(size_t)i * a.n_heads * D + e] = 0.f;
-    if (blockIdx.x == 0 && threadIdx.x == 0) {
-        a.shape[0] = T;
-        a.shape[1] = ctas;
+    if ((int)blockIdx.x >= ctas || T == 0) {
+        if (threadIdx.x == 0) a.notes[blockIdx.x] = make_int4(0, 0, 0, 0);
+        return;
     }
-    if ((int)blockIdx.x >= ctas || T == 0) return;
     const runs parts(T, ctas);
     const int g0 = parts.start((int)blockIdx.x), g1 = parts.start((int)blockIdx.x + 1);
 
@@ -694,7 +585,7 @@ __global__ void __launch_bounds__(Tile::WARPS * 32, MINB)
         s0 = lo;
     }
     const int h0g = g0 / line;
-    if (threadIdx.x == 0) a.info[blockIdx.x] = make_int4(s0, h0g, h0g * line + pre[s0], h0g * line + pre[s0 + 1]);
+    if (threadIdx.x == 0) a.notes[blockIdx.x] = note_of(parts, (int)blockIdx.x, s0, h0g * HG, h0g * line + pre[s0], h0g * line + pre[s0 + 1]);
     auto next_row = [&](int &s, int &h) {
         do {
             if (++s == (int)a.n_seq) {
@@ -855,62 +746,6 @@ __global__ void __launch_bounds__(Tile::WARPS * 32, MINB)
     }
 }
 
-// Joins the rows that several CTAs had a part of, in tile order. CTA (c, virtual head of the group,
-// share of the channels): the row that CTA c's run begins inside, if c is the first to do so.
-constexpr int JOIN_THREADS = 256;
-template <int GP>
-__global__ void __launch_bounds__(JOIN_THREADS, 6) k_attn_join(const __grid_constant__ attn_args a) {
-    extern __shared__ float wgt[];  // [GP][parts]
-    __shared__ float inv[GP];
-    pdl_trigger();
-    pdl_wait();
-    const int T = a.shape[0], ctas = a.shape[1], c = blockIdx.x + 1, hs = blockIdx.y;
-    if (c >= ctas) return;
-    const int4 at = a.info[c];  // batch row, head group, the row's first tile and the one after its last
-    const runs parts(T, ctas);
-    if (parts.start(c) == at.z || parts.start(c - 1) > at.z) return;
-    const int D = a.D, HG = a.hg, n = parts.owner(at.w - 1) - c + 2;
-    const int vh = at.y * HG + hs, kvh = vh / a.subs, sub = vh - kvh * a.subs;
-    const int h0 = kvh * a.group + sub * GP, heads = min(GP, a.group - sub * GP);
-    // CTA c - 1's part is its second record unless its run begins with the row; the others' their first
-    const size_t rec = (size_t)GP * (D + 2), step = (size_t)2 * HG * rec;
-    const float *rest = a.part + (size_t)c * step + hs * rec;
-    const float *part0 = rest - step + (parts.start(c - 1) == at.z ? 0 : HG * rec);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    for (int hd = warp; hd < heads; hd += JOIN_THREADS / 32) {
-        const float sk = a.sinks ? a.sinks[h0 + hd] * LOG2E : -INFINITY;
-        const size_t ml = (size_t)GP * D + 2 * hd;
-        float M = sk;
-        for (int k = lane; k < n; k += 32) {
-            const float m = (k ? rest + (size_t)(k - 1) * step : part0)[ml];
-            wgt[hd * n + k] = m;
-            M = fmaxf(M, m);
-        }
-        M = warp_max(M);
-        float sum = 0.f;
-        for (int k = lane; k < n; k += 32) {
-            const float m = wgt[hd * n + k], f = m == -INFINITY ? 0.f : ex2(m - M);
-            wgt[hd * n + k] = f;
-            sum += (k ? rest + (size_t)(k - 1) * step : part0)[ml + 1] * f;
-        }
-        sum = warp_sum(sum);
-        if (lane == 0) {
-            sum += sk == -INFINITY ? 0.f : ex2(sk - M);
-            inv[hd] = sum == 0.f ? 0.f : 1.f / sum;
-        }
-    }
-    __syncthreads();
-    float *out = a.out + ((size_t)at.x * a.n_heads + h0) * D;
-    for (int e = blockIdx.z * JOIN_THREADS + threadIdx.x; e < heads * D; e += gridDim.z * JOIN_THREADS) {
-        const int hd = e / D;
-        const float *w = wgt + hd * n;
-        float v = part0[e] * w[0];
-#pragma unroll 8
-        for (int k = 1; k < n; ++k) v = fmaf(rest[(size_t)(k - 1) * step + e], w[k], v);
-        out[e] = v * inv[hd];
-    }
-}
-
 // ---- host side --------------------------------------------------------------------------------
 
 // How a shape is cut: virtual heads and warps per CTA, stages, shared memory and the grid.
@@ -991,23 +826,19 @@ bool plan_of(attn_plan &p, bool mma, unsigned kv_type, int n_heads, int n_kv, in
     });
 }
 
-// The work buffer: the line's shape, a note a CTA, the parts.
-size_t attn_bytes(const attn_plan &p, int D) { return 16 + (size_t)p.grid * 16 + (size_t)p.grid * 2 * p.hg * p.gp * (D + 2) * 4; }
+// The work buffer: a note a CTA, then the parts.
+size_t attn_bytes(int grid, int hg, int gp, int D) { return (size_t)grid * 16 + (size_t)grid * 2 * hg * gp * (D + 2) * 4; }
+size_t attn_bytes(const attn_plan &p, int D) { return attn_bytes(p.grid, p.hg, p.gp, D); }
 
 template <class Tile, int MINB>
 cudaError_t launch(moearc_ctx *c, const attn_plan &p, const attn_args &a, const seq_list &L) {
     static std::atomic<bool> done[MOEARC_MAX_DEVICES];
     cudaError_t e = once_per_device(done, [] {
-        const cudaError_t e1 = set_smem(k_attn_batch<Tile, MINB>, MAX_SMEM - 512);
-        // the join's few KB under the same split of L1 and shared memory: with the default one its
-        // CTAs run one at a time on an SM
-        return e1 != cudaSuccess ? e1 : set_smem(k_attn_join<Tile::GP>, 40 * 1024);
+        return set_smem(k_attn_batch<Tile, MINB>, MAX_SMEM - 512);
     });
     if (e == cudaSuccess)
         e = launch_pdl(k_attn_batch<Tile, MINB>, dim3((unsigned)p.grid), dim3((unsigned)p.warps * 32), (size_t)p.smem, c->stream, a, L, p.ns);
-    if (e == cudaSuccess && p.grid > 1)
-        e = launch_pdl(k_attn_join<Tile::GP>, dim3((unsigned)p.grid - 1, (unsigned)p.hg, (Tile::GP * a.D + 511) / 512), dim3(JOIN_THREADS),
-                       (size_t)Tile::GP * p.grid * 4, c->stream, a);
+    if (e == cudaSuccess) e = attn_join_launch<Tile::GP>(c, p.grid, a);
     return e;
 }
 
@@ -1031,6 +862,7 @@ unsigned long moearc_x_kv_work_bytes(moearc_ctx *c, const moearc_x_kv_cache *kv,
             if (!plan_of(p, true, kv->kv_type, (int)n_heads, (int)kv->n_kv_heads, D, n, c->sm_count)) return 0;
             need = std::max(need, attn_bytes(p, D));
         }
+        need = std::max(need, attn_bytes(attn_tc_grid(kv->head_dim, c->sm_count), 1, 8, D));
     }
     return need;
 }
@@ -1061,9 +893,11 @@ int moearc_x_attn_decode_batch(moearc_ctx *c, const moearc_x_kv_cache *kv, unsig
     const bool mma = kv->kv_type != T_F32 && mma_dim(kv->head_dim) && (align & 15) == 0;
     attn_plan p;
     if (!plan_of(p, mma, kv->kv_type, (int)n_heads, (int)kv->n_kv_heads, (int)D, (int)n_seq, c->sm_count)) return ERR_ARG;
-    if (kv->work_bytes < attn_bytes(p, (int)D)) return ERR_ARG;
+    const bool tc = mma && attn_tc_serves(*kv, layer);
+    const int tc_grid = attn_tc_grid(kv->head_dim, c->sm_count);
+    if (kv->work_bytes < (tc ? attn_bytes(tc_grid, 1, 8, (int)D) : attn_bytes(p, (int)D))) return ERR_ARG;
     const unsigned cap = kv->max_pages * kv->page_tokens;
-    if ((unsigned long long)n_seq * (cap / (unsigned)(p.keys * p.rsplit) + 2) * p.nhg >= (1ull << 31)) return ERR_ARG;
+    if ((unsigned long long)n_seq * (cap / (unsigned)(p.keys * p.rsplit) + 2) * p.nhg * p.hg >= (1ull << 31)) return ERR_ARG;
 
     attn_args a;
     a.out = out;
@@ -1098,13 +932,13 @@ int moearc_x_attn_decode_batch(moearc_ctx *c, const moearc_x_kv_cache *kv, unsig
     a.nhg = p.nhg;
     a.min_tiles = 1;
     a.scale2 = scale * LOG2E;
-    a.shape = static_cast<int *>(kv->work);
-    a.info = reinterpret_cast<int4 *>(a.shape + 4);
-    a.part = reinterpret_cast<float *>(a.info + p.grid);
+    a.status = kv->status;
+    a.notes = static_cast<int4 *>(kv->work);
+    a.part = reinterpret_cast<float *>(a.notes + (tc ? tc_grid : p.grid));
     device_guard g(c->device);
     if (!g.ok) return ERR;
     launch_scope ls(c, "attn_decode_batch", n_seq, n_heads);
-    const cudaError_t e = with_tile(mma, kv->kv_type, kv->head_dim, a.group, [&](auto *t, auto minb) {
+    const cudaError_t e = tc ? attn_tc_launch(c, *kv, a, L) : with_tile(mma, kv->kv_type, kv->head_dim, a.group, [&](auto *t, auto minb) {
         return launch<std::remove_pointer_t<decltype(t)>, decltype(minb)::value>(c, p, a, L);
     });
     if (e != cudaSuccess) cudaGetLastError();  // the failed launch's error, not left for an unrelated later check

@@ -24,8 +24,8 @@ from .kernels import KV_ELEM_BYTES, BadArgument, Context, DeviceBuffer, Failed, 
 
 NO_PAGE = 0xFFFFFFFF
 MAX_LIST = 1024
-# bits of status(): what a call without effect lacked
-FULL, LONG, TAKEN = 1, 2, 4
+# bits of status(): what a call without effect lacked; WAIT: a kernel's wait ran out, its output is invalid
+FULL, LONG, TAKEN, WAIT = 1, 2, 4, 8
 
 
 def _list(v) -> tuple[C.Array, int]:
@@ -130,7 +130,7 @@ class KvCache:
         self.ctx._finish(self.ctx.lib.moearc_x_kv_compact(self.ctx.raw, self._d, t.ptr, r.ptr, _p(n_live)), "kv_compact")
 
     def status(self) -> int:
-        """Waits; the FULL, LONG and TAKEN bits raised since the last look (0: every call took effect)."""
+        """Waits; the FULL, LONG, TAKEN and WAIT bits raised since the last look (0: every call took effect)."""
         v = self.ctx.lib.moearc_x_kv_status(self.ctx.raw, self._d)
         if v < 0:
             raise Failed("kv_status failed on the device")
