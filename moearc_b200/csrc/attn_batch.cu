@@ -286,7 +286,15 @@ struct mma_tile {
 // Eight keys a tile. Scores: lane (key, quarter) sums over every fourth group of four channels for
 // all GP heads, and the quarters are added so that each lane ends with GP / 4 heads of its key.
 // Values: a lane owns groups of four channels (lane + 32 i) of all GP heads, the weights come from
-// shared memory.
+// shared memory, each twice over: channels are multiplied in pairs (fma.rn.f32x2), which halves the
+// instructions, and those are what bounds it.
+
+// d += a b, two values at once.
+__device__ __forceinline__ void fma2(float2 &d, float2 a, float2 b) {
+    asm("{ .reg .b64 x, y, z; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; mov.b64 z, {%0, %1}; fma.rn.f32x2 z, x, y, z; mov.b64 {%0, %1}, z; }"
+        : "+f"(d.x), "+f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+}
 
 template <typename T>
 __device__ __forceinline__ float4 four(const T *p) {
@@ -310,14 +318,15 @@ __device__ __forceinline__ void round_to(float v, __nv_bfloat16 &d) { d = __floa
 template <typename T, int NQ, int GP_>
 struct core_tile {
     static constexpr int KEYS = 8, GP = GP_, ELEM = sizeof(T), WARPS = NQ == 1 ? 16 : 8;
-    float acc[NQ][GP][4], m[GP / 4], l[GP / 4];
+    float2 acc[NQ][GP][2];
+    float m[GP / 4], l[GP / 4];
 
     // A row in shared memory: an odd number of 16-byte chunks, so that eight keys meet eight bank
     // groups; its tail past head_dim is zero.
     static __host__ __device__ int row_bytes(int D) { return (((D * (int)sizeof(T) + 15) / 16) | 1) * 16; }
     static __host__ __device__ int dpad(int D) { return (D + 3) & ~3; }
     // per warp beside the stages: q, the tile's weights, the heads' corrections
-    static __host__ __device__ int extra_bytes(int D) { return (GP * dpad(D) + KEYS * GP + GP) * 4; }
+    static __host__ __device__ int extra_bytes(int D) { return (GP * dpad(D) + 2 * KEYS * GP + GP) * 4; }
 
     __device__ __forceinline__ void init(const float *q, int heads, const attn_args &a, uint8_t *extra, int lane) {
         // q as [four channels][head][4], so that a lane's loop has fixed offsets
@@ -329,7 +338,7 @@ struct core_tile {
 #pragma unroll
         for (int i = 0; i < NQ; ++i)
 #pragma unroll
-            for (int h = 0; h < GP; ++h) acc[i][h][0] = acc[i][h][1] = acc[i][h][2] = acc[i][h][3] = 0.f;
+            for (int h = 0; h < GP; ++h) acc[i][h][0] = acc[i][h][1] = make_float2(0.f, 0.f);
 #pragma unroll
         for (int h = 0; h < GP / 4; ++h) {
             m[h] = -INFINITY;
@@ -351,17 +360,28 @@ struct core_tile {
     }
     static __device__ __forceinline__ void load_rows(uint8_t *stage, long long off, const attn_args &a, int lane) {
         const int rb = row_bytes(a.D);
+        const unsigned s0 = smem_u32(stage);
+        if (a.unit == 16) {
+            for (unsigned c = lane * 16; c - lane * 16 < a.head_bytes; c += 512) {
+                const bool on = c < a.head_bytes;
+#pragma unroll
+                for (int r = 0; r < KEYS; ++r) {
+                    const long long b = __shfl_sync(0xffffffffu, off, r);
+                    const size_t src = (b < 0 ? 0 : (size_t)b) + c;
+                    if (on) {
+                        cp_async16z(s0 + r * rb + c, a.k + src, b >= 0);
+                        cp_async16z(s0 + (KEYS + r) * rb + c, a.v + src, b >= 0);
+                    }
+                }
+            }
+            return;
+        }
 #pragma unroll 1
-        for (int r = 0; r < KEYS; ++r) {
+        for (int r = 0; r < KEYS; ++r) {  // rows off a 16-byte boundary
             const long long b = __shfl_sync(0xffffffffu, off, r);
             const size_t src = b < 0 ? 0 : (size_t)b;
             uint8_t *kr = stage + r * rb, *vr = kr + KEYS * rb;
-            if (a.unit == 16) {
-                for (unsigned c = lane * 16; c < a.head_bytes; c += 512) {
-                    cp_async16z(smem_u32(kr + c), a.k + src + c, b >= 0);
-                    cp_async16z(smem_u32(vr + c), a.v + src + c, b >= 0);
-                }
-            } else if (a.unit == 4) {
+            if (a.unit == 4) {
                 for (unsigned c = lane * 4; c < a.head_bytes; c += 128) {
                     cp_async4z(smem_u32(kr + c), a.k + src + c, b >= 0);
                     cp_async4z(smem_u32(vr + c), a.v + src + c, b >= 0);
@@ -384,12 +404,12 @@ struct core_tile {
     }
     __device__ __forceinline__ void step(const uint8_t *stage, unsigned live, const attn_args &a, uint8_t *extra, int lane) {
         const int D = a.D, dp = dpad(D), rb = row_bytes(D);
-        auto *qs = reinterpret_cast<float *>(extra), *ps = qs + GP * dp, *cs = ps + KEYS * GP;
+        auto *qs = reinterpret_cast<float *>(extra), *ps = qs + GP * dp, *cs = ps + 2 * KEYS * GP;
         const int key = lane >> 2, cl = lane & 3;
         const T *kr = reinterpret_cast<const T *>(stage + key * rb);
-        float s[GP];
+        float2 s2[GP];
 #pragma unroll
-        for (int h = 0; h < GP; ++h) s[h] = 0.f;
+        for (int h = 0; h < GP; ++h) s2[h] = make_float2(0.f, 0.f);
         const float *qc = qs + 4 * cl * GP;
 #pragma unroll 2
         for (int c = 4 * cl; c < dp; c += 16, qc += 16 * GP) {
@@ -397,9 +417,13 @@ struct core_tile {
 #pragma unroll
             for (int h = 0; h < GP; ++h) {
                 const float4 qv = *reinterpret_cast<const float4 *>(qc + 4 * h);
-                s[h] = fmaf(qv.x, kv.x, fmaf(qv.y, kv.y, fmaf(qv.z, kv.z, fmaf(qv.w, kv.w, s[h]))));
+                fma2(s2[h], make_float2(qv.x, qv.y), make_float2(kv.x, kv.y));
+                fma2(s2[h], make_float2(qv.z, qv.w), make_float2(kv.z, kv.w));
             }
         }
+        float s[GP];
+#pragma unroll
+        for (int h = 0; h < GP; ++h) s[h] = s2[h].x + s2[h].y;
         // heads cl GP / 4 + (0 .. GP / 4 - 1) of the key, summed over the quarters
         float t[GP / 2], x[GP / 4];
 #pragma unroll
@@ -436,33 +460,27 @@ struct core_tile {
             for (int h = 0; h < GP; ++h) {
                 const float corr = cs[h];
 #pragma unroll
-                for (int i = 0; i < NQ; ++i) {
-                    acc[i][h][0] *= corr;
-                    acc[i][h][1] *= corr;
-                    acc[i][h][2] *= corr;
-                    acc[i][h][3] *= corr;
-                }
+                for (int i = 0; i < NQ; ++i)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        acc[i][h][e].x *= corr;
+                        acc[i][h][e].y *= corr;
+                    }
             }
         }
 #pragma unroll
         for (int h = 0; h < GP / 4; ++h) {
             const float p = ex2(x[h] - (m[h] == -INFINITY ? 0.f : m[h]));
             l[h] += p;
-            ps[key * GP + cl * (GP / 4) + h] = p;
+            *reinterpret_cast<float2 *>(ps + 2 * (key * GP + cl * (GP / 4) + h)) = make_float2(p, p);
         }
         __syncwarp();
 #pragma unroll
         for (int k = 0; k < KEYS; ++k) {
             const T *vr = reinterpret_cast<const T *>(stage + (KEYS + k) * rb);
-            float p[GP];
+            float4 p[GP / 2];  // the weights of two heads, each twice
 #pragma unroll
-            for (int h = 0; h < GP; h += 4) {
-                const float4 v = *reinterpret_cast<const float4 *>(ps + k * GP + h);
-                p[h] = v.x;
-                p[h + 1] = v.y;
-                p[h + 2] = v.z;
-                p[h + 3] = v.w;
-            }
+            for (int h = 0; h < GP / 2; ++h) p[h] = *reinterpret_cast<const float4 *>(ps + 2 * k * GP + 4 * h);
 #pragma unroll
             for (int i = 0; i < NQ; ++i) {
                 const int c = 4 * (lane + 32 * i);
@@ -470,10 +488,9 @@ struct core_tile {
                     const float4 v = four(vr + c);
 #pragma unroll
                     for (int h = 0; h < GP; ++h) {
-                        acc[i][h][0] = fmaf(p[h], v.x, acc[i][h][0]);
-                        acc[i][h][1] = fmaf(p[h], v.y, acc[i][h][1]);
-                        acc[i][h][2] = fmaf(p[h], v.z, acc[i][h][2]);
-                        acc[i][h][3] = fmaf(p[h], v.w, acc[i][h][3]);
+                        const float2 w = h & 1 ? make_float2(p[h / 2].z, p[h / 2].w) : make_float2(p[h / 2].x, p[h / 2].y);
+                        fma2(acc[i][h][0], w, make_float2(v.x, v.y));
+                        fma2(acc[i][h][1], w, make_float2(v.z, v.w));
                     }
                 }
             }
@@ -499,7 +516,7 @@ struct core_tile {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int d = 4 * (lane + 32 * i) + e;
-                    if (d < a.D) f(h, d, acc[i][h][e]);
+                    if (d < a.D) f(h, d, e & 1 ? acc[i][h][e / 2].y : acc[i][h][e / 2].x);
                 }
     }
 };
@@ -615,8 +632,8 @@ __global__ void __launch_bounds__(Tile::WARPS * 32, MINB)
         lj = llo / KEYS * KEYS + (t * R + r) * KEYS + lane;
         lpage = NO_PAGE;
         if (lane < KEYS && lj >= llo && lj < lhi) {
-            const unsigned e = lj / a.pt;
-            lslot = lj - e * a.pt;
+            unsigned e;
+            place_of(a, lj, e, lslot);
             lpage = ltab[e];
         }
     };
@@ -918,6 +935,7 @@ int moearc_x_attn_decode_batch(moearc_ctx *c, const moearc_x_kv_cache *kv, unsig
     a.max_pages = kv->max_pages;
     a.n_pages = kv->n_pages;
     a.pt = kv->page_tokens;
+    a.pt_inv = (unsigned)std::min(0xffffffffull, (1ull << 32) / kv->page_tokens);
     a.cap = cap;
     const uintptr_t rows = align | a.head_bytes;
     a.unit = (rows & 15) == 0 ? 16 : (rows & 3) == 0 ? 4 : 2;

@@ -24,7 +24,7 @@ struct attn_args {
     const unsigned *tables, *n_kv, *begin;
     unsigned *status;
     size_t q_stride, new_stride, token_bytes, head_bytes;  // bytes: n_kv_heads x head_dim elements, head_dim elements
-    unsigned n_seq, max_pages, n_pages, pt, cap;
+    unsigned n_seq, max_pages, n_pages, pt, pt_inv, cap;  // pt_inv: floor(2^32 / pt), at most 2^32 - 1
     unsigned unit;  // bytes of one copy: 16 where rows start on 16-byte boundaries, else 4 or 2
     int one_page;   // tiles never cross a page
     int listed;  // rows come from the list (else row i is batch row i)
@@ -41,6 +41,16 @@ __device__ __forceinline__ void span_of(const attn_args &a, const seq_list &L, u
     row = a.listed ? L.row[i] : i;
     hi = min(a.n_kv[row], a.cap);
     lo = a.begin ? min(a.begin[i], hi) : 0;
+}
+
+// Token j's table entry and slot: j / pt by its inverse, one short at most.
+__device__ __forceinline__ void place_of(const attn_args &a, unsigned j, unsigned &entry, unsigned &slot) {
+    entry = __umulhi(j, a.pt_inv);
+    slot = j - entry * a.pt;
+    if (slot >= a.pt) {
+        ++entry;
+        slot -= a.pt;
+    }
 }
 
 // The line's tiles over `ctas` CTAs: each takes `each` of them, the first `more` one more.

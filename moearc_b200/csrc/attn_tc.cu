@@ -217,8 +217,8 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 2 : 1)
                     const unsigned j = lo + (unsigned)(g - u0) * KEYS + r * 64 + t;
                     page[r] = NO_PAGE;
                     if (j < hi) {
-                        const unsigned e = j / a.pt;
-                        slot[r] = j - e * a.pt;
+                        unsigned e;
+                        place_of(a, j, e, slot[r]);
                         page[r] = tab[e];
                     }
                 }

@@ -19,12 +19,17 @@ constexpr int PLAN_THREADS = 1024;
 static_assert(PLAN_THREADS == KV_LIST, "one plan thread a list entry");
 constexpr int SWEEP = 16;  // refs a plan thread reads at once: four 16-byte loads in flight
 
+// Lists go into a launch by value; short ones in a shorter argument (a launch with 10 KB of them
+// held up the next one by 10 us).
+constexpr int SHORT_LIST = 64, SHORT_POOLS = 16;
+template <int N>
 struct row_list {
-    unsigned a[KV_LIST], b[KV_LIST];  // grow: row, add; fork: src, dst; free: row, keep
+    unsigned a[N], b[N];  // grow: row, add; fork: src, dst; free: row, keep
     unsigned n;
 };
+template <int N>
 struct pool_list {
-    void *p[2 * KV_LAYERS];
+    void *p[N];
     unsigned n;
 };
 struct cache_view {
@@ -35,8 +40,8 @@ struct cache_view {
 // The work buffer: a header, each list entry's first new page, the new pages, the moves and (for
 // compaction) where every page goes.
 struct plan_head {
-    unsigned ok, n_moves, n_live, pad;
-    unsigned off[KV_LIST + 4];
+    unsigned ok, n_moves, n_live, n;
+    unsigned off[KV_LIST], src[KV_LIST], dst[KV_LIST];  // a fork's list for the kernel after the plan
 };
 struct work_view {
     plan_head *head;
@@ -100,8 +105,8 @@ __device__ __forceinline__ unsigned entry_of(const unsigned *off, unsigned n, un
 
 // Plan of a grow (FORK false) or fork (true): the pages each entry needs, the free pages handed
 // out, the moves; a grow's tables, counts and lengths too. All or nothing.
-template <bool FORK>
-__global__ void __launch_bounds__(PLAN_THREADS) k_kv_plan(const __grid_constant__ row_list L, cache_view k, work_view w, int deep) {
+template <bool FORK, int N>
+__global__ void __launch_bounds__(PLAN_THREADS) k_kv_plan(const __grid_constant__ row_list<N> L, cache_view k, work_view w, int deep) {
     __shared__ unsigned long long sums64[32];
     __shared__ unsigned sums[32], off[KV_LIST + 1], bad, n_moves;
     const unsigned i = threadIdx.x;
@@ -173,9 +178,14 @@ __global__ void __launch_bounds__(PLAN_THREADS) k_kv_plan(const __grid_constant_
         __syncthreads();
     }
     if (!FORK && ok && i < L.n) k.n_kv[row] = cur + add;
-    if (FORK && ok && i < L.n) w.head->off[i] = total ? off[i] : 0;
+    if (FORK && ok && i < L.n) {
+        w.head->off[i] = total ? off[i] : 0;
+        w.head->src[i] = row;
+        w.head->dst[i] = L.b[i];
+    }
     if (i == 0) {
         w.head->ok = ok;
+        w.head->n = L.n;
         w.head->n_moves = ok ? n_moves : 0;
         if (!ok) atomicOr(k.status, flags ? flags : MOEARC_X_KV_FULL);
     }
@@ -184,8 +194,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) k_kv_plan(const __grid_constant_
 // Copy the planned pages in every pool: 256-thread CTAs over chunks of CHUNK elements of V.
 constexpr int COPY_THREADS = 256, COPY_UNROLL = 4, COPY_CHUNK = COPY_THREADS * COPY_UNROLL;
 
-template <typename V>
-__device__ void copy_pages(const uint2 *moves, unsigned n_moves, const pool_list &P, unsigned page_v) {
+template <typename V, int NP>
+__device__ void copy_pages(const uint2 *moves, unsigned n_moves, const pool_list<NP> &P, unsigned page_v) {
     const unsigned cpp = (page_v + COPY_CHUNK - 1) / COPY_CHUNK;  // chunks a page
     const unsigned long long items = (unsigned long long)n_moves * P.n * cpp;
     for (unsigned long long it = blockIdx.x; it < items; it += gridDim.x) {
@@ -205,8 +215,8 @@ __device__ void copy_pages(const uint2 *moves, unsigned n_moves, const pool_list
     }
 }
 
-template <typename V>
-__global__ void __launch_bounds__(COPY_THREADS) k_kv_copy(const __grid_constant__ pool_list P, work_view w, unsigned page_v) {
+template <typename V, int NP>
+__global__ void __launch_bounds__(COPY_THREADS) k_kv_copy(const __grid_constant__ pool_list<NP> P, work_view w, unsigned page_v) {
     pdl_trigger();
     pdl_wait();
     copy_pages<V>(w.moves, w.head->n_moves, P, page_v);
@@ -214,17 +224,17 @@ __global__ void __launch_bounds__(COPY_THREADS) k_kv_copy(const __grid_constant_
 
 // A fork's rows: dst's table from src's, its own pages in place, one more reference on each
 // shared page; then the copies. CTAs stride over the list.
-template <typename V>
-__global__ void __launch_bounds__(COPY_THREADS) k_kv_fork(const __grid_constant__ row_list L, const __grid_constant__ pool_list P,
-                                                          cache_view k, work_view w, unsigned page_v, int deep) {
+template <typename V, int NP>
+__global__ void __launch_bounds__(COPY_THREADS) k_kv_fork(const __grid_constant__ pool_list<NP> P, cache_view k, work_view w,
+                                                          unsigned page_v, int deep) {
     pdl_trigger();
     pdl_wait();
     if (!w.head->ok) return;
-    for (unsigned e = blockIdx.x; e < L.n; e += gridDim.x) {
-        const unsigned len = k.n_kv[L.a[e]], np = (len + k.pt - 1) / k.pt;
+    for (unsigned e = blockIdx.x; e < w.head->n; e += gridDim.x) {
+        const unsigned len = k.n_kv[w.head->src[e]], np = (len + k.pt - 1) / k.pt;
         const unsigned first = deep ? 0 : len / k.pt;  // pages from here on are the row's own
-        const unsigned *src = k.tables + (size_t)L.a[e] * k.max_pages;
-        unsigned *dst = k.tables + (size_t)L.b[e] * k.max_pages;
+        const unsigned *src = k.tables + (size_t)w.head->src[e] * k.max_pages;
+        unsigned *dst = k.tables + (size_t)w.head->dst[e] * k.max_pages;
         for (unsigned j = threadIdx.x; j < np; j += COPY_THREADS) {
             unsigned p = src[j];
             if (p < k.n_pages) {
@@ -233,12 +243,13 @@ __global__ void __launch_bounds__(COPY_THREADS) k_kv_fork(const __grid_constant_
             }
             dst[j] = p;
         }
-        if (threadIdx.x == 0) k.n_kv[L.b[e]] = len;
+        if (threadIdx.x == 0) k.n_kv[w.head->dst[e]] = len;
     }
     copy_pages<V>(w.moves, w.head->n_moves, P, page_v);
 }
 
-__global__ void __launch_bounds__(256) k_kv_free(const __grid_constant__ row_list L, cache_view k) {
+template <int N>
+__global__ void __launch_bounds__(256) k_kv_free(const __grid_constant__ row_list<N> L, cache_view k) {
     pdl_trigger();
     pdl_wait();
     const unsigned s = L.a[blockIdx.x], cur = k.n_kv[s], keep = min(cur, L.b[blockIdx.x]);
@@ -300,8 +311,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) k_kv_compact_plan(cache_view k, 
 
 // A compaction's copies, tables and counts. In place as well: a hole's count is written with its
 // page's, and every other element is written with what it holds or holds already.
-template <typename V>
-__global__ void __launch_bounds__(COPY_THREADS) k_kv_compact(const __grid_constant__ pool_list P, cache_view k, work_view w,
+template <typename V, int NP>
+__global__ void __launch_bounds__(COPY_THREADS) k_kv_compact(const __grid_constant__ pool_list<NP> P, cache_view k, work_view w,
                                                              unsigned page_v, unsigned *tables_out, unsigned *refs_out,
                                                              unsigned *n_live_out) {
     pdl_trigger();
@@ -331,19 +342,55 @@ cache_view view_of(const moearc_x_kv_cache &k) {
     return cache_view{k.tables, k.n_kv, k.refs, k.status, k.n_pages, k.page_tokens, k.max_pages, k.max_seq};
 }
 
-// The pools, and the widest element (16, 4 or 2 bytes) that every page of every pool starts on and
-// is a whole number of.
-unsigned pools_of(const moearc_x_kv_cache &k, pool_list &P, size_t &page_bytes) {
+// The widest element (16, 4 or 2 bytes) that every page of every pool starts on and is a whole number of.
+unsigned copy_width(const moearc_x_kv_cache &k, size_t &page_bytes) {
     page_bytes = (size_t)k.page_tokens * k.n_kv_heads * k.head_dim * kv_elem_bytes(k.kv_type);
     uintptr_t a = page_bytes;
-    P.n = 2 * k.n_layer;
-    for (unsigned l = 0; l < k.n_layer; ++l) {
-        P.p[2 * l] = k.k_pages[l];
-        P.p[2 * l + 1] = k.v_pages[l];
-        a |= reinterpret_cast<uintptr_t>(k.k_pages[l]) | reinterpret_cast<uintptr_t>(k.v_pages[l]);
-    }
+    for (unsigned l = 0; l < k.n_layer; ++l) a |= reinterpret_cast<uintptr_t>(k.k_pages[l]) | reinterpret_cast<uintptr_t>(k.v_pages[l]);
     return (a & 15) == 0 ? 16 : (a & 3) == 0 ? 4 : 2;
 }
+
+// f(V, pools, elements a page): the copy's element type and the pools in an argument of their size.
+template <typename F>
+cudaError_t with_pools(const moearc_x_kv_cache &k, F &&f) {
+    size_t page_bytes;
+    const unsigned width = copy_width(k, page_bytes), page_v = (unsigned)(page_bytes / width);
+    auto by_width = [&](auto &P) {
+        P.n = 2 * k.n_layer;
+        for (unsigned l = 0; l < k.n_layer; ++l) {
+            P.p[2 * l] = k.k_pages[l];
+            P.p[2 * l + 1] = k.v_pages[l];
+        }
+        return width == 16 ? f(uint4(), P, page_v) : width == 4 ? f(uint32_t(), P, page_v) : f(uint16_t(), P, page_v);
+    };
+    if (2 * k.n_layer <= SHORT_POOLS) {
+        pool_list<SHORT_POOLS> P;
+        return by_width(P);
+    }
+    pool_list<2 * KV_LAYERS> P;
+    return by_width(P);
+}
+// f(list): the rows in an argument of their size.
+template <typename F>
+cudaError_t with_rows(const unsigned *a, const unsigned *b, unsigned n, F &&f) {
+    auto fill = [&](auto &L) {
+        L.n = n;
+        for (unsigned i = 0; i < n; ++i) {
+            L.a[i] = a[i];
+            L.b[i] = b ? b[i] : 0;
+        }
+        return f(L);
+    };
+    if (n <= SHORT_LIST) {
+        row_list<SHORT_LIST> L;
+        return fill(L);
+    }
+    row_list<KV_LIST> L;
+    return fill(L);
+}
+
+// Eight CTAs an SM: 3 GB of pages in 503 us, against 562 with two.
+dim3 copy_grid(const moearc_ctx *c) { return dim3((unsigned)c->sm_count * 8); }
 
 int finish(moearc_ctx *c, cudaError_t e) {
     if (e != cudaSuccess) {
@@ -389,26 +436,21 @@ int moearc_x_kv_grow(moearc_ctx *c, const moearc_x_kv_cache *kv, const unsigned 
     if (!seqs || !add) return ERR;
     if (n > KV_LIST) return ERR_ARG;
     kv_rows_seen seen(kv->max_seq);
-    row_list L;
-    L.n = n;
-    for (unsigned i = 0; i < n; ++i) {
+    for (unsigned i = 0; i < n; ++i)
         if (!seen.add(seqs[i], kv->max_seq)) return ERR_ARG;
-        L.a[i] = seqs[i];
-        L.b[i] = add[i];
-    }
     device_guard g(c->device);
     if (!g.ok) return ERR;
-    pool_list P;
-    size_t page_bytes;
-    const unsigned width = pools_of(*kv, P, page_bytes), page_v = (unsigned)(page_bytes / width);
     const work_view w = work_of(kv->work, kv->n_pages);
     launch_scope ls(c, "kv_grow", n, kv->n_layer);
-    cudaError_t e = launch_pdl(k_kv_plan<false>, dim3(1), dim3(PLAN_THREADS), 0, c->stream, L, view_of(*kv), w, 0);
-    const dim3 grid((unsigned)c->sm_count * 2);
+    cudaError_t e = with_rows(seqs, add, n, [&](auto &L) {
+        constexpr int N = (int)(sizeof(L.a) / sizeof(unsigned));
+        return launch_pdl(k_kv_plan<false, N>, dim3(1), dim3(PLAN_THREADS), 0, c->stream, L, view_of(*kv), w, 0);
+    });
     if (e == cudaSuccess)
-        e = width == 16  ? launch_pdl(k_kv_copy<uint4>, grid, dim3(COPY_THREADS), 0, c->stream, P, w, page_v)
-            : width == 4 ? launch_pdl(k_kv_copy<uint32_t>, grid, dim3(COPY_THREADS), 0, c->stream, P, w, page_v)
-                         : launch_pdl(k_kv_copy<uint16_t>, grid, dim3(COPY_THREADS), 0, c->stream, P, w, page_v);
+        e = with_pools(*kv, [&](auto v, auto &P, unsigned page_v) {
+            constexpr int NP = (int)(sizeof(P.p) / sizeof(void *));
+            return launch_pdl(k_kv_copy<decltype(v), NP>, copy_grid(c), dim3(COPY_THREADS), 0, c->stream, P, w, page_v);
+        });
     const int rc2 = ls.finish();
     return e != cudaSuccess ? finish(c, e) : rc2;
 }
@@ -421,30 +463,24 @@ int moearc_x_kv_fork(moearc_ctx *c, const moearc_x_kv_cache *kv, const unsigned 
     if (!src || !dst) return ERR;
     if (n > KV_LIST) return ERR_ARG;
     kv_rows_seen seen(kv->max_seq);
-    row_list L;
-    L.n = n;
-    for (unsigned i = 0; i < n; ++i) {
+    for (unsigned i = 0; i < n; ++i)
         if (!seen.add(dst[i], kv->max_seq)) return ERR_ARG;
-        L.b[i] = dst[i];
-    }
-    for (unsigned i = 0; i < n; ++i) {
+    for (unsigned i = 0; i < n; ++i)
         if (src[i] >= kv->max_seq || seen.has(src[i])) return ERR_ARG;
-        L.a[i] = src[i];
-    }
     device_guard g(c->device);
     if (!g.ok) return ERR;
-    pool_list P;
-    size_t page_bytes;
-    const unsigned width = pools_of(*kv, P, page_bytes), page_v = (unsigned)(page_bytes / width);
     const work_view w = work_of(kv->work, kv->n_pages);
     const cache_view k = view_of(*kv);
     launch_scope ls(c, "kv_fork", n, kv->n_layer);
-    cudaError_t e = launch_pdl(k_kv_plan<true>, dim3(1), dim3(PLAN_THREADS), 0, c->stream, L, k, w, deep);
-    const dim3 grid((unsigned)c->sm_count * 2);
+    cudaError_t e = with_rows(src, dst, n, [&](auto &L) {
+        constexpr int N = (int)(sizeof(L.a) / sizeof(unsigned));
+        return launch_pdl(k_kv_plan<true, N>, dim3(1), dim3(PLAN_THREADS), 0, c->stream, L, k, w, deep);
+    });
     if (e == cudaSuccess)
-        e = width == 16  ? launch_pdl(k_kv_fork<uint4>, grid, dim3(COPY_THREADS), 0, c->stream, L, P, k, w, page_v, deep)
-            : width == 4 ? launch_pdl(k_kv_fork<uint32_t>, grid, dim3(COPY_THREADS), 0, c->stream, L, P, k, w, page_v, deep)
-                         : launch_pdl(k_kv_fork<uint16_t>, grid, dim3(COPY_THREADS), 0, c->stream, L, P, k, w, page_v, deep);
+        e = with_pools(*kv, [&](auto v, auto &P, unsigned page_v) {
+            constexpr int NP = (int)(sizeof(P.p) / sizeof(void *));
+            return launch_pdl(k_kv_fork<decltype(v), NP>, copy_grid(c), dim3(COPY_THREADS), 0, c->stream, P, k, w, page_v, deep);
+        });
     const int rc2 = ls.finish();
     return e != cudaSuccess ? finish(c, e) : rc2;
 }
@@ -456,17 +492,15 @@ int moearc_x_kv_free(moearc_ctx *c, const moearc_x_kv_cache *kv, const unsigned 
     if (!seqs) return ERR;
     if (n > KV_LIST) return ERR_ARG;
     kv_rows_seen seen(kv->max_seq);
-    row_list L;
-    L.n = n;
-    for (unsigned i = 0; i < n; ++i) {
+    for (unsigned i = 0; i < n; ++i)
         if (!seen.add(seqs[i], kv->max_seq)) return ERR_ARG;
-        L.a[i] = seqs[i];
-        L.b[i] = keep ? keep[i] : 0;
-    }
     device_guard g(c->device);
     if (!g.ok) return ERR;
     launch_scope ls(c, "kv_free", n, 1);
-    const cudaError_t e = launch_pdl(k_kv_free, dim3(n), dim3(256), 0, c->stream, L, view_of(*kv));
+    const cudaError_t e = with_rows(seqs, keep, n, [&](auto &L) {
+        constexpr int N = (int)(sizeof(L.a) / sizeof(unsigned));
+        return launch_pdl(k_kv_free<N>, dim3(n), dim3(256), 0, c->stream, L, view_of(*kv));
+    });
     const int rc2 = ls.finish();
     return e != cudaSuccess ? finish(c, e) : rc2;
 }
@@ -478,18 +512,16 @@ int moearc_x_kv_compact(moearc_ctx *c, const moearc_x_kv_cache *kv, unsigned int
     if (!tables_out || !refs_out) return ERR;
     device_guard g(c->device);
     if (!g.ok) return ERR;
-    pool_list P;
-    size_t page_bytes;
-    const unsigned width = pools_of(*kv, P, page_bytes), page_v = (unsigned)(page_bytes / width);
     const work_view w = work_of(kv->work, kv->n_pages);
     const cache_view k = view_of(*kv);
     launch_scope ls(c, "kv_compact", kv->n_pages, kv->n_layer);
     cudaError_t e = launch_pdl(k_kv_compact_plan, dim3(1), dim3(PLAN_THREADS), 0, c->stream, k, w);
-    const dim3 grid((unsigned)c->sm_count * 2), block(COPY_THREADS);
     if (e == cudaSuccess)
-        e = width == 16  ? launch_pdl(k_kv_compact<uint4>, grid, block, 0, c->stream, P, k, w, page_v, tables_out, refs_out, n_live)
-            : width == 4 ? launch_pdl(k_kv_compact<uint32_t>, grid, block, 0, c->stream, P, k, w, page_v, tables_out, refs_out, n_live)
-                         : launch_pdl(k_kv_compact<uint16_t>, grid, block, 0, c->stream, P, k, w, page_v, tables_out, refs_out, n_live);
+        e = with_pools(*kv, [&](auto v, auto &P, unsigned page_v) {
+            constexpr int NP = (int)(sizeof(P.p) / sizeof(void *));
+            return launch_pdl(k_kv_compact<decltype(v), NP>, copy_grid(c), dim3(COPY_THREADS), 0, c->stream, P, k, w, page_v, tables_out,
+                              refs_out, n_live);
+        });
     const int rc2 = ls.finish();
     return e != cudaSuccess ? finish(c, e) : rc2;
 }

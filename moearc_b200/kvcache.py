@@ -16,6 +16,7 @@ read back but ``status()``.
 from __future__ import annotations
 
 import ctypes as C
+from array import array
 
 import numpy as np
 
@@ -28,14 +29,18 @@ MAX_LIST = 1024
 FULL, LONG, TAKEN, WAIT = 1, 2, 4, 8
 
 
-def _list(v) -> tuple[C.Array, int]:
-    n = len(v)
-    if n > MAX_LIST:
-        raise BadArgument(f"a list of {n} rows: one call takes {MAX_LIST}")
-    for x in v:
-        if not 0 <= x <= 0xFFFFFFFF:
-            raise BadArgument(f"{x} in a row list")
-    return (C.c_uint * max(n, 1))(*v), n
+def _list(v) -> array:
+    try:
+        a = v if isinstance(v, array) and v.typecode == "I" else array("I", v)
+    except (OverflowError, TypeError) as e:
+        raise BadArgument(f"a row list of whole numbers is wanted: {e}") from None
+    if len(a) > MAX_LIST:
+        raise BadArgument(f"a list of {len(a)} rows: one call takes {MAX_LIST}")
+    return a
+
+
+def _at(a: array) -> int:
+    return a.buffer_info()[0]
 
 
 class KvCache:
@@ -94,29 +99,25 @@ class KvCache:
 
     def grow(self, seqs, add) -> None:
         """Row seqs[i] gains add[i] tokens."""
-        s, n = _list(seqs)
-        a, m = _list(add)
-        if n != m:
-            raise BadArgument(f"{n} rows and {m} counts")
-        self.ctx._finish(self.ctx.lib.moearc_x_kv_grow(self.ctx.raw, self._d, s, a, n), "kv_grow")
+        s, a = _list(seqs), _list(add)
+        if len(s) != len(a):
+            raise BadArgument(f"{len(s)} rows and {len(a)} counts")
+        self.ctx._finish(self.ctx.lib.moearc_x_kv_grow(self.ctx.raw, self._d, _at(s), _at(a), len(s)), "kv_grow")
 
     def fork(self, src, dst, deep: bool = False) -> None:
         """Empty row dst[i] becomes row src[i], sharing full pages (or, deep, copying every page)."""
-        s, n = _list(src)
-        t, m = _list(dst)
-        if n != m:
-            raise BadArgument(f"{n} rows to fork onto {m}")
-        self.ctx._finish(self.ctx.lib.moearc_x_kv_fork(self.ctx.raw, self._d, s, t, n, 1 if deep else 0), "kv_fork")
+        s, t = _list(src), _list(dst)
+        if len(s) != len(t):
+            raise BadArgument(f"{len(s)} rows to fork onto {len(t)}")
+        self.ctx._finish(self.ctx.lib.moearc_x_kv_fork(self.ctx.raw, self._d, _at(s), _at(t), len(s), 1 if deep else 0), "kv_fork")
 
     def free(self, seqs, keep=None) -> None:
         """Row seqs[i] keeps its first keep[i] tokens (None: no tokens)."""
-        s, n = _list(seqs)
-        k = None
-        if keep is not None:
-            k, m = _list(keep)
-            if n != m:
-                raise BadArgument(f"{n} rows and {m} lengths")
-        self.ctx._finish(self.ctx.lib.moearc_x_kv_free(self.ctx.raw, self._d, s, k, n), "kv_free")
+        s = _list(seqs)
+        k = None if keep is None else _list(keep)
+        if k is not None and len(s) != len(k):
+            raise BadArgument(f"{len(s)} rows and {len(k)} lengths")
+        self.ctx._finish(self.ctx.lib.moearc_x_kv_free(self.ctx.raw, self._d, _at(s), None if k is None else _at(k), len(s)), "kv_free")
 
     def compact(self, tables_out: DeviceBuffer | None = None, refs_out: DeviceBuffer | None = None,
                 n_live: DeviceBuffer | None = None) -> None:
@@ -161,9 +162,9 @@ class KvCache:
                 sinks.require("sinks", 4 * n_heads)
         rows = None
         if seqs is not None:
-            rows, n = _list(seqs)
-            if n != n_seq:
-                raise BadArgument(f"{n} rows for a batch of {n_seq}")
+            rows = _list(seqs)
+            if len(rows) != n_seq:
+                raise BadArgument(f"{len(rows)} rows for a batch of {n_seq}")
         self.ctx._finish(self.ctx.lib.moearc_x_attn_decode_batch(
-            self.ctx.raw, self._d, layer, out.ptr, q.ptr, qs, _p(k_new), _p(v_new), ns, rows, _p(kv_begin), _p(sinks), n_seq,
+            self.ctx.raw, self._d, layer, out.ptr, q.ptr, qs, _p(k_new), _p(v_new), ns, None if rows is None else _at(rows), _p(kv_begin), _p(sinks), n_seq,
             n_heads, scale), "attn_decode_batch")

@@ -127,7 +127,9 @@ def test_python_lists_are_checked():
         kvcache._list([1 << 32])
     with pytest.raises(BadArgument):
         kvcache._list(range(1025))
-    assert kvcache._list([])[1] == 0
+    with pytest.raises(BadArgument):
+        kvcache._list([0.5])
+    assert len(kvcache._list([])) == 0
 
 
 def test_the_model_keeps_its_rules():
