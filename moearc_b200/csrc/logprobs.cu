@@ -10,18 +10,19 @@
 // exponentials (16 a clock and SM) come close behind.
 //
 // A row is one CTA, or a cluster of up to 16 where there are too few rows to fill the GPU; the
-// cluster's CTAs join over distributed shared memory, so there is no second kernel and no
-// workspace, and the order of the sums depends on the sizes alone.
+// cluster's CTAs write what they found into the first one's shared memory, so there is no second
+// kernel and no workspace, and the order of the sums depends on the sizes alone.
 //
 // The k likeliest: a thread's running maximum is the largest of the elements it read, so the k-th
 // largest of a CTA's thread maxima is a bound that k elements reach. Only the elements of threads
-// at or above it (about k of 256 threads) are read again, from L2, and those that reach the bound
-// are ranked by counting. Should more reach it than the list holds (equal values), the k-th of the
+// at or above it (about k of 256 threads) are read again, from L2, all at once, and those that
+// reach the bound are ranked by counting. Should more reach it than the list holds (equal values), the k-th of the
 // listed ones becomes the next bound. A key is the value's bits in order, then the complement of
 // the index: no two are equal, and ties go to the lowest index.
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <cfloat>
 
 #include "kvcache.cuh"
 
@@ -116,36 +117,59 @@ __device__ __forceinline__ float one(const float *p) { return *p; }
 __device__ __forceinline__ float one(const __half *p) { return __half2float(*p); }
 __device__ __forceinline__ float one(const __nv_bfloat16 *p) { return __bfloat162float(*p); }
 
-// N values into a running triple: one look at the maximum for all of them.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{ .reg .b64 x, y, z; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; add.rn.f32x2 z, x, y; mov.b64 {%0, %1}, z; }" : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("{ .reg .b64 x, y, z; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; mul.rn.f32x2 z, x, y; mov.b64 {%0, %1}, z; }" : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ void fma2(float2 &d, float2 a, float2 b) {
+    asm("{ .reg .b64 x, y, z; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; mov.b64 z, {%0, %1}; fma.rn.f32x2 z, x, y, z; mov.b64 {%0, %1}, z; }"
+        : "+f"(d.x), "+f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+}
+
+// N logits, unscaled, into a running triple of unscaled m and s: one look at the maximum for all of
+// them, then two at a time. scale2: scale x log2(e).
 template <int N>
-__device__ __forceinline__ void take(triple &r, const float (&x)[N]) {
+__device__ __forceinline__ void take(triple &r, const float (&x)[N], float scale2) {
     float b = x[0];
 #pragma unroll
     for (int i = 1; i < N; ++i) b = fmaxf(b, x[i]);
     if (b > r.m) {
         if (r.m != -INFINITY) {
-            const float d = fmaxf(r.m - b, -200.f), f = ex2(d * LOG2E);
-            r.s = f * fmaf(d, r.l, r.s);
+            const float d = fmaxf(r.m - b, -FLT_MAX), f = ex2(d * scale2);
+            r.s = f * r.s + (f * d) * r.l;
             r.l *= f;
         }
         r.m = b;
     }
     const float base = r.m == -INFINITY ? 0.f : r.m;
-    float l0 = 0.f, l1 = 0.f, s0 = 0.f, s1 = 0.f;
+    const float2 mb = make_float2(-base, -base), sc = make_float2(scale2, scale2);
+    float2 l = make_float2(0.f, 0.f), t = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        // below -200 the weight is 0 in f32; the floor keeps 0 x -inf out of S
-        const float d = max_nan(x[i] - base, -200.f), e = ex2(d * LOG2E);
-        if (i & 1) {
-            l1 += e;
-            s1 = fmaf(e, d, s1);
-        } else {
-            l0 += e;
-            s0 = fmaf(e, d, s0);
-        }
+    for (int i = 0; i + 1 < N; i += 2) {
+        // the floor keeps 0 x -inf out of S: a weight that far down is 0 at any scale allowed
+        float2 d = add2(make_float2(x[i], x[i + 1]), mb);
+        d.x = max_nan(d.x, -FLT_MAX);
+        d.y = max_nan(d.y, -FLT_MAX);
+        float2 e = mul2(d, sc);
+        e.x = ex2(e.x);
+        e.y = ex2(e.y);
+        l = add2(l, e);
+        fma2(t, e, d);
     }
-    r.l += l0 + l1;
-    r.s += s0 + s1;
+    if constexpr (N & 1) {
+        const float d = max_nan(x[N - 1] - base, -FLT_MAX), e = ex2(d * scale2);
+        l.x += e;
+        t.x = fmaf(e, d, t.x);
+    }
+    r.l += l.x + l.y;
+    r.s += t.x + t.y;
 }
 
 // The CTA's run [c0, c1) of a row: single elements up to a 16-byte boundary, whole vectors, the
@@ -165,29 +189,39 @@ struct run {
 };
 
 struct shared_lists {
-    triple part[WARPS], whole;
+    triple part[WARPS];
     float warp_bound[WARPS];
-    float max_v[TH];
-    unsigned max_t[TH];
-    unsigned n_max, n_sub, sub[TH], n_list, n_top;
+    __align__(16) float max_v[TH];
+    unsigned max_t[TH], sub[TH];
+    unsigned n_max, n_sub, n_list;
     float bound;
-    u64 bound_key;
-    u64 list[LIST], top[MAX_K];
+    __align__(16) u64 list[LIST + 2];
+    // what the cluster's CTAs found, in the first one's copy: keys largest first, 0 past the last
+    triple whole[16];
+    __align__(16) u64 top[16][MAX_K];
+    u64 best[MAX_K];
 };
 
-// The largest min(k, n) of list[0, n) in order, into top; rank by counting.
+// The largest k of list[0, n) in order into top, 0 past the last; rank by counting. n is even (a
+// 0 fills up an odd one).
 __device__ void rank_list(const u64 *list, unsigned n, unsigned k, u64 *top) {
+    const auto *two = reinterpret_cast<const ulonglong2 *>(list);
     for (unsigned i = threadIdx.x; i < n; i += TH) {
         const u64 key = list[i];
         unsigned rank = 0;
-        for (unsigned j = 0; j < n; ++j) rank += list[j] > key;
-        if (rank < k) top[rank] = key;
+#pragma unroll 4
+        for (unsigned j = 0; j < n / 2; ++j) {
+            const ulonglong2 v = two[j];
+            rank += (v.x > key) + (v.y > key);
+        }
+        if (rank < k && key) top[rank] = key;
     }
 }
 
-// The largest min(k, elements) keys of the CTA's run, in order, in sh.top; m: the thread's maximum.
+// The largest min(k, elements) keys of the CTA's run, in order, into top, 0 past the last; m: the
+// thread's maximum, scaled.
 template <typename T>
-__device__ void top_of_run(const run<T> &R, float m, float scale, unsigned k, shared_lists &sh) {
+__device__ void top_of_run(const run<T> &R, float m, float scale, unsigned k, shared_lists &sh, u64 *top) {
     constexpr int V = vec<T>::N;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     // a first bound: each warp has ceil(k / WARPS) lanes at or above its own, so k threads of the
@@ -200,6 +234,7 @@ __device__ void top_of_run(const run<T> &R, float m, float scale, unsigned k, sh
     }
     if (lane == 0) sh.warp_bound[warp] = last;
     if (threadIdx.x == 0) sh.n_max = sh.n_sub = 0;
+    sh.max_v[threadIdx.x] = -INFINITY;
     __syncthreads();
     float bound = sh.warp_bound[0];
 #pragma unroll
@@ -210,20 +245,27 @@ __device__ void top_of_run(const run<T> &R, float m, float scale, unsigned k, sh
         sh.max_t[i] = threadIdx.x;
     }
     __syncthreads();
-    // the k-th largest of the listed maxima (ties in any order give the same value)
+    // the k-th largest of the listed maxima: fewer than k above it, at least k at or above
     const unsigned n_max = sh.n_max;
     if (threadIdx.x < n_max) {
         const float mine = sh.max_v[threadIdx.x];
-        unsigned rank = 0;
-        for (unsigned j = 0; j < n_max; ++j) rank += sh.max_v[j] > mine || (sh.max_v[j] == mine && j < threadIdx.x);
-        if (rank == k - 1) sh.bound = mine;
+        unsigned above = 0, at = 0;
+#pragma unroll 4
+        for (unsigned j = 0; j < (n_max + 3) / 4; ++j) {
+            const float4 o = reinterpret_cast<const float4 *>(sh.max_v)[j];
+            above += (o.x > mine) + (o.y > mine) + (o.z > mine) + (o.w > mine);
+            at += (o.x == mine) + (o.y == mine) + (o.z == mine) + (o.w == mine);
+        }
+        if (above < k && above + at >= k) sh.bound = mine;
     }
     __syncthreads();
     bound = sh.bound;
     if (m >= bound) sh.sub[atomicAdd(&sh.n_sub, 1u)] = threadIdx.x;
     u64 least = key_of(bound, 0xffffffffu);
+    const unsigned per = (R.nv + TH - 1) / TH;  // vectors a thread, at most
     for (;;) {
         if (threadIdx.x == 0) sh.n_list = 0;
+        if (threadIdx.x < MAX_K) top[threadIdx.x] = 0;
         __syncthreads();
         auto see = [&](float x, unsigned i) {
             const u64 key = key_of(x, i);
@@ -232,26 +274,41 @@ __device__ void top_of_run(const run<T> &R, float m, float scale, unsigned k, sh
                 if (at < LIST) sh.list[at] = key;
             }
         };
-        const unsigned n_sub = sh.n_sub;
-        for (unsigned w = warp; w < n_sub; w += WARPS) {
-            const unsigned t = sh.sub[w];
-            if (lane == 0 && t < R.head) see(one(R.row + R.c0 + t) * scale, R.c0 + t);
-            if (lane == 1 && R.tail() + t < R.c1) see(one(R.row + R.tail() + t) * scale, R.tail() + t);
-            for (unsigned j = t + lane * TH; j < R.nv; j += 32 * TH) {
-                float x[V];
-                unpack<T>(ld16(R.row + R.body() + (size_t)j * V), x);
+        const unsigned n_sub = sh.n_sub, n_vec = n_sub * per;
+        for (unsigned q = threadIdx.x; q < n_sub; q += TH) {
+            const unsigned t = sh.sub[q];
+            if (t < R.head) see(one(R.row + R.c0 + t) * scale, R.c0 + t);
+            if (R.tail() + t < R.c1) see(one(R.row + R.tail() + t) * scale, R.tail() + t);
+        }
+        for (unsigned q = threadIdx.x; q < n_vec; q += 2 * TH) {
+            uint4 u[2];
+            unsigned j[2];
 #pragma unroll
-                for (int e = 0; e < V; ++e) see(x[e] * scale, R.body() + j * V + e);
+            for (int e = 0; e < 2; ++e) {
+                const unsigned qe = q + e * TH, w = qe / per;
+                j[e] = qe < n_vec ? sh.sub[w] + (qe - w * per) * TH : R.nv;
+                if (j[e] < R.nv) u[e] = ld16(R.row + R.body() + (size_t)j[e] * V);
             }
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                if (j[e] < R.nv) {
+                    float x[V];
+                    unpack<T>(u[e], x);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) see(x[i] * scale, R.body() + j[e] * V + i);
+                }
         }
         __syncthreads();
-        const unsigned n = min(sh.n_list, (unsigned)LIST);
         const bool over = sh.n_list > LIST;
-        rank_list(sh.list, n, k, sh.top);
-        if (threadIdx.x == 0) sh.n_top = min(n, k);
+        unsigned n = min(sh.n_list, (unsigned)LIST);
+        if ((n & 1) && threadIdx.x == 0) sh.list[n] = 0;
+        n += n & 1;
+        __syncthreads();
+        rank_list(sh.list, n, k, top);
         __syncthreads();
         if (!over) return;
-        least = sh.top[k - 1];  // k listed elements reach it: the next bound, above the last
+        least = top[k - 1];  // k listed elements reach it: the next bound, above the last
+        __syncthreads();
     }
 }
 
@@ -262,13 +319,14 @@ __global__ void __launch_bounds__(TH, 4) k_logprobs(const lp_args a) {
     cg::cluster_group cluster = cg::this_cluster();
     const unsigned size = cluster.num_blocks(), rank = cluster.block_rank();
     const unsigned row = blockIdx.x / size;
+    if (size > 1) cluster.barrier_arrive();  // waited for before the first one's memory is written
     pdl_trigger();
     pdl_wait();
     const T *p = static_cast<const T *>(a.logits) + (size_t)row * a.row_stride;
     const unsigned share = ((a.n_vocab + size - 1) / size + V - 1) / V * V;
     const unsigned c0 = min(rank * share, a.n_vocab), c1 = min(c0 + share, a.n_vocab);
     const run<T> R(p, c0, c1);
-    const float scale = a.scale;
+    const float scale = a.scale, scale2 = a.scale * LOG2E;
 
     triple r{-INFINITY, 0.f, 0.f};
     unsigned j = threadIdx.x;
@@ -279,25 +337,23 @@ __global__ void __launch_bounds__(TH, 4) k_logprobs(const lp_args a) {
         float x[UNROLL * V];
 #pragma unroll
         for (int i = 0; i < UNROLL; ++i) unpack<T>(u[i], x + i * V);
-#pragma unroll
-        for (int i = 0; i < UNROLL * V; ++i) x[i] *= scale;
-        take(r, x);
+        take(r, x, scale2);
     }
     for (; j < R.nv; j += TH) {
         float x[V];
         unpack<T>(ld16(R.row + R.body() + (size_t)j * V), x);
-#pragma unroll
-        for (int i = 0; i < V; ++i) x[i] *= scale;
-        take(r, x);
+        take(r, x, scale2);
     }
     if (threadIdx.x < R.head) {
-        const float x[1] = {one(R.row + R.c0 + threadIdx.x) * scale};
-        take(r, x);
+        const float x[1] = {one(R.row + R.c0 + threadIdx.x)};
+        take(r, x, scale2);
     }
     if (R.tail() + threadIdx.x < R.c1) {
-        const float x[1] = {one(R.row + R.tail() + threadIdx.x) * scale};
-        take(r, x);
+        const float x[1] = {one(R.row + R.tail() + threadIdx.x)};
+        take(r, x, scale2);
     }
+    r.m *= scale;  // rounding keeps the order: this is the largest of the rounded products
+    r.s *= scale;
     const float mine = r.m;
 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -307,55 +363,51 @@ __global__ void __launch_bounds__(TH, 4) k_logprobs(const lp_args a) {
         r = join(r, b);
     }
     if (lane == 0) sh.part[warp] = r;
-    __syncthreads();
+    if (a.k) top_of_run(R, mine, scale, a.k, sh, size > 1 ? sh.best : sh.top[0]);
+    else __syncthreads();
+    if (size > 1) cluster.barrier_wait();
+    shared_lists &first = size > 1 ? *cluster.map_shared_rank(&sh, 0) : sh;
     if (threadIdx.x == 0) {
         r = sh.part[0];
         for (int w = 1; w < WARPS; ++w) r = join(r, sh.part[w]);
-        sh.whole = r;
+        first.whole[rank] = r;
     }
-    if (a.k) top_of_run(R, mine, scale, a.k, sh);
-    if (size > 1) cluster.sync();
-    else __syncthreads();
-    if (rank == 0) {
-        r = sh.whole;
-        for (unsigned c = 1; c < size; ++c) r = join(r, cluster.map_shared_rank(&sh, c)->whole);
-        const float log_l = logf(r.l);
-        const bool none = r.m == -INFINITY && r.l == 0.f;  // every logit -inf
-        if (threadIdx.x == 0) {
-            if (a.entropy) a.entropy[row] = none ? 0.f : log_l - r.s / r.l;
-            if (a.logprob) {
-                const unsigned t = a.tokens[row];
-                a.logprob[row] = t >= a.n_vocab ? 0.f : none ? -INFINITY : (one(p + t) * scale - r.m) - log_l;
-            }
-        }
-        if (a.k) {
-            u64 *top = sh.top;
-            if (size > 1) {
-                __shared__ u64 every[16 * MAX_K], best[MAX_K];
-                __shared__ unsigned at[17];
-                if (threadIdx.x == 0) {
-                    at[0] = 0;
-                    for (unsigned c = 0; c < size; ++c) at[c + 1] = at[c] + cluster.map_shared_rank(&sh, c)->n_top;
-                }
-                __syncthreads();
-                for (unsigned i = threadIdx.x; i < size * MAX_K; i += TH) {
-                    const unsigned c = i / MAX_K, e = i - c * MAX_K;
-                    if (e < at[c + 1] - at[c]) every[at[c] + e] = cluster.map_shared_rank(&sh, c)->top[e];
-                }
-                __syncthreads();
-                rank_list(every, at[size], a.k, best);
-                __syncthreads();
-                top = best;
-            }
-            if (threadIdx.x < a.k) {
-                const u64 key = top[threadIdx.x];
-                const float v = value_of(key);
-                a.top_id[(size_t)row * a.k + threadIdx.x] = 0xffffffffu - (unsigned)key;
-                a.top_lp[(size_t)row * a.k + threadIdx.x] = none ? -INFINITY : (v - r.m) - log_l;
-            }
+    if (size > 1) {
+        if (threadIdx.x < a.k) first.top[rank][threadIdx.x] = sh.best[threadIdx.x];
+        cluster.sync();
+        if (rank != 0) return;
+    } else {
+        __syncthreads();
+    }
+    r = sh.whole[0];
+    for (unsigned c = 1; c < size; ++c) r = join(r, sh.whole[c]);
+    const float log_l = logf(r.l);
+    const bool none = r.m == -INFINITY && r.l == 0.f;  // every logit -inf
+    if (threadIdx.x == 0) {
+        if (a.entropy) a.entropy[row] = none ? 0.f : log_l - r.s / r.l;
+        if (a.logprob) {
+            const unsigned t = a.tokens[row];
+            a.logprob[row] = t >= a.n_vocab ? 0.f : none ? -INFINITY : (one(p + t) * scale - r.m) - log_l;
         }
     }
-    if (size > 1) cluster.sync();  // the other CTAs' lists are read until here
+    if (a.k) {
+        if (size > 1) {
+            // every CTA's keys side by side (the unused end of a list is 0), then the best of them
+            for (unsigned i = threadIdx.x; i < size * a.k; i += TH) sh.list[i] = sh.top[i / a.k][i % a.k];
+            unsigned n = size * a.k;
+            if ((n & 1) && threadIdx.x == 0) sh.list[n] = 0;
+            n += n & 1;
+            __syncthreads();
+            rank_list(sh.list, n, a.k, sh.best);
+            __syncthreads();
+        }
+        if (threadIdx.x < a.k) {
+            const u64 key = size > 1 ? sh.best[threadIdx.x] : sh.top[0][threadIdx.x];
+            const float v = value_of(key);
+            a.top_id[(size_t)row * a.k + threadIdx.x] = 0xffffffffu - (unsigned)key;
+            a.top_lp[(size_t)row * a.k + threadIdx.x] = none ? -INFINITY : (v - r.m) - log_l;
+        }
+    }
 }
 
 template <typename T>
@@ -396,7 +448,7 @@ int moearc_x_token_logprobs(moearc_ctx *c, const void *logits, unsigned int type
     if (k && (!top_ids || !top_logprobs)) return ERR;
     if (!kv_elem_bytes(type)) return ERR_ARG;
     if (n_vocab == 0 || n_vocab > (1u << 30) || row_stride < n_vocab || k > MAX_TOPK || k > n_vocab || n_rows > (1u << 26)) return ERR_ARG;
-    if (!(scale > 0.f) || scale - scale != 0.f) return ERR_ARG;
+    if (!(scale >= 1e-30f && scale <= 1e30f)) return ERR_ARG;
     if (reinterpret_cast<uintptr_t>(logits) % kv_elem_bytes(type)) return ERR_ARG;
     if (n_rows == 0) return OK;
     const lp_args a{logits, tokens, row_stride, n_vocab, k, scale, logprob, entropy, top_logprobs, top_ids};
