@@ -31,7 +31,7 @@ using namespace moearc;
 
 namespace {
 
-constexpr int TH = 256, WARPS = TH / 32, UNROLL = 4, MAX_K = MAX_TOPK, LIST = 512;
+constexpr int TH = 256, WARPS = TH / 32, MAX_K = MAX_TOPK, LIST = 512;
 constexpr float LOG2E = 1.4426950408889634f;
 
 typedef unsigned long long u64;
@@ -225,14 +225,14 @@ __device__ void top_of_run(const run<T> &R, float m, float scale, unsigned k, sh
     constexpr int V = vec<T>::N;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     // a first bound: each warp has ceil(k / WARPS) lanes at or above its own, so k threads of the
-    // CTA are at or above the least of them
-    float v = m, last = m;
+    // CTA are at or above the least of them (as ordered bits, for the warp's maximum in one step)
+    unsigned v = (unsigned)(key_of(m, 0) >> 32), last = v;
     for (unsigned q = 0; q < (k + WARPS - 1) / WARPS; ++q) {
-        last = warp_max(v);
+        last = __reduce_max_sync(0xffffffffu, v);
         const unsigned who = __ballot_sync(0xffffffffu, v == last);
-        if (lane == __ffs(who) - 1) v = -INFINITY;
+        if (lane == __ffs(who) - 1) v = 0;
     }
-    if (lane == 0) sh.warp_bound[warp] = last;
+    if (lane == 0) sh.warp_bound[warp] = value_of((u64)last << 32);
     if (threadIdx.x == 0) sh.n_max = sh.n_sub = 0;
     sh.max_v[threadIdx.x] = -INFINITY;
     __syncthreads();
@@ -313,7 +313,7 @@ __device__ void top_of_run(const run<T> &R, float m, float scale, unsigned k, sh
 }
 
 template <typename T>
-__global__ void __launch_bounds__(TH, 4) k_logprobs(const lp_args a) {
+__global__ void __launch_bounds__(TH, sizeof(T) == 4 ? 4 : 5) k_logprobs(const lp_args a) {
     constexpr int V = vec<T>::N;
     __shared__ shared_lists sh;
     cg::cluster_group cluster = cg::this_cluster();
@@ -326,8 +326,17 @@ __global__ void __launch_bounds__(TH, 4) k_logprobs(const lp_args a) {
     const unsigned share = ((a.n_vocab + size - 1) / size + V - 1) / V * V;
     const unsigned c0 = min(rank * share, a.n_vocab), c1 = min(c0 + share, a.n_vocab);
     const run<T> R(p, c0, c1);
+    // the given token's logit, asked for before the pass
+    unsigned token = 0;
+    float given = 0.f;
+    if (a.logprob && rank == 0 && threadIdx.x == 0) {
+        token = a.tokens[row];
+        if (token < a.n_vocab) given = one(p + token);
+    }
     const float scale = a.scale, scale2 = a.scale * LOG2E;
 
+    // 16-byte loads: 32 f32 or 16 16-bit logits a look, as registers for four or five CTAs an SM allow
+    constexpr int UNROLL = sizeof(T) == 4 ? 8 : 2;
     triple r{-INFINITY, 0.f, 0.f};
     unsigned j = threadIdx.x;
     for (; j + (UNROLL - 1) * TH < R.nv; j += UNROLL * TH) {
@@ -379,16 +388,20 @@ __global__ void __launch_bounds__(TH, 4) k_logprobs(const lp_args a) {
     } else {
         __syncthreads();
     }
-    r = sh.whole[0];
-    for (unsigned c = 1; c < size; ++c) r = join(r, sh.whole[c]);
+    // the cluster's triples, joined in pairs by every warp
+    r = lane < (int)size ? sh.whole[lane] : triple{-INFINITY, 0.f, 0.f};
+    for (unsigned o = size >> 1; o > 0; o >>= 1) {
+        const triple b{__shfl_xor_sync(0xffffffffu, r.m, o), __shfl_xor_sync(0xffffffffu, r.l, o), __shfl_xor_sync(0xffffffffu, r.s, o)};
+        r = join(r, b);
+    }
+    r.m = __shfl_sync(0xffffffffu, r.m, 0);
+    r.l = __shfl_sync(0xffffffffu, r.l, 0);
+    r.s = __shfl_sync(0xffffffffu, r.s, 0);
     const float log_l = logf(r.l);
     const bool none = r.m == -INFINITY && r.l == 0.f;  // every logit -inf
     if (threadIdx.x == 0) {
         if (a.entropy) a.entropy[row] = none ? 0.f : log_l - r.s / r.l;
-        if (a.logprob) {
-            const unsigned t = a.tokens[row];
-            a.logprob[row] = t >= a.n_vocab ? 0.f : none ? -INFINITY : (one(p + t) * scale - r.m) - log_l;
-        }
+        if (a.logprob) a.logprob[row] = token >= a.n_vocab ? 0.f : none ? -INFINITY : (given * scale - r.m) - log_l;
     }
     if (a.k) {
         if (size > 1) {
@@ -417,11 +430,11 @@ cudaError_t launch(moearc_ctx *c, const lp_args &a, unsigned n_rows) {
         return cudaFuncSetAttribute(k_logprobs<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     });
     if (e != cudaSuccess) return e;
-    // CTAs for twice the SMs, but at least 8 vectors a thread of each; 16 CTAs only where 8 leave
-    // most SMs idle
-    const unsigned most = std::max(1u, a.n_vocab / (TH * 8 * (unsigned)vec<T>::N));
+    // CTAs for twice the SMs, but at least 16 vectors a thread of each; clusters of 16 only where they
+    // are few enough to run at once (16 rows of 131072 f32: 20 us with 16 CTAs a row, 11 with 8)
+    const unsigned most = std::max(1u, a.n_vocab / (TH * 16 * (unsigned)vec<T>::N));
     unsigned size = 1;
-    while (size < 16 && n_rows * size < (unsigned)c->sm_count * 2 && size * 2 <= most) size *= 2;
+    while (size < 16 && n_rows * size < (unsigned)c->sm_count * 2 && size * 2 <= most && (size < 8 || n_rows * 16 <= (unsigned)c->sm_count)) size *= 2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(n_rows * size);
     cfg.blockDim = dim3(TH);
