@@ -153,21 +153,35 @@ static __global__ void __launch_bounds__(JOIN_THREADS, 4) k_attn_join(const __gr
     const size_t rec = (size_t)GP * (D + 2), step = (size_t)2 * HG * rec;
     const float *rest = a.part + (size_t)c * step + hs * rec, *part0 = rest - step + (size_t)at.w * HG * rec;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int q = threadIdx.x & (JOIN_THREADS / JOIN_PARTS - 1), grp = threadIdx.x / (JOIN_THREADS / JOIN_PARTS);
+    const int k0 = n * grp / JOIN_PARTS, k1 = n * (grp + 1) / JOIN_PARTS;
+    auto part_at = [&](int k) { return k ? rest + (size_t)(k - 1) * step : part0; };
+    // this thread's first parts of its first channels, asked for before the weights are worked out
+    constexpr int AHEAD = 4;
+    float4 ahead[AHEAD];
+    const int e0 = blockIdx.z * JOIN_OUT + 4 * q;
+    const bool quads = D % 4 == 0;
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i)
+        if (quads && e0 < heads * D && k0 + i < k1) ahead[i] = *reinterpret_cast<const float4 *>(part_at(k0 + i) + e0);
     for (int hd = warp; hd < heads; hd += JOIN_THREADS / 32) {
         const float sk = a.sinks ? a.sinks[h0 + hd] * LOG2E : -INFINITY;
-        const size_t ml = (size_t)GP * D + 2 * hd;
+        const size_t ml = (size_t)GP * D + 2 * hd;  // even: max and sum are read together
+        // up to 32 parts are in registers, more are read again for the sum
+        float2 mine = make_float2(-INFINITY, 0.f);
         float M = sk;
         for (int k = lane; k < n; k += 32) {
-            const float m = (k ? rest + (size_t)(k - 1) * step : part0)[ml];
-            wgt[hd * n + k] = m;
-            M = fmaxf(M, m);
+            const float2 v = *reinterpret_cast<const float2 *>(part_at(k) + ml);
+            if (k < 32) mine = v;
+            M = fmaxf(M, v.x);
         }
         M = warp_max(M);
         float sum = 0.f;
         for (int k = lane; k < n; k += 32) {
-            const float m = wgt[hd * n + k], f = m == -INFINITY ? 0.f : ex2(m - M);
+            const float2 v = k < 32 ? mine : *reinterpret_cast<const float2 *>(part_at(k) + ml);
+            const float f = v.x == -INFINITY ? 0.f : ex2(v.x - M);
             wgt[hd * n + k] = f;
-            sum += (k ? rest + (size_t)(k - 1) * step : part0)[ml + 1] * f;
+            sum += v.y * f;
         }
         sum = warp_sum(sum);
         if (lane == 0) {
@@ -177,27 +191,31 @@ static __global__ void __launch_bounds__(JOIN_THREADS, 4) k_attn_join(const __gr
     }
     __syncthreads();
     float *out = a.out + ((size_t)at.x * a.n_heads + h0) * D;
-    const int q = threadIdx.x & (JOIN_THREADS / JOIN_PARTS - 1), grp = threadIdx.x / (JOIN_THREADS / JOIN_PARTS);
-    const int k0 = n * grp / JOIN_PARTS, k1 = n * (grp + 1) / JOIN_PARTS;
     for (int b = blockIdx.z * JOIN_OUT; b < heads * D; b += gridDim.z * JOIN_OUT) {
         const int e = b + 4 * q;
         float v[4] = {0.f, 0.f, 0.f, 0.f};
         // channels of one head where head_dim is a multiple of four; else each channel has its own
         const float *w0 = wgt + min(e, heads * D - 1) / D * n;
         if (e < heads * D) {
-            if (D % 4 == 0) {
-#pragma unroll 4
-                for (int k = k0; k < k1; ++k) {
-                    const float4 x = *reinterpret_cast<const float4 *>((k ? rest + (size_t)(k - 1) * step : part0) + e);
-                    const float w = w0[k];
+            if (quads) {
+                auto add = [&](float4 x, float w) {
                     v[0] = fmaf(x.x, w, v[0]);
                     v[1] = fmaf(x.y, w, v[1]);
                     v[2] = fmaf(x.z, w, v[2]);
                     v[3] = fmaf(x.w, w, v[3]);
+                };
+                int k = k0;
+                if (e == e0) {
+#pragma unroll
+                    for (int i = 0; i < AHEAD; ++i)
+                        if (k0 + i < k1) add(ahead[i], w0[k0 + i]);
+                    k += AHEAD;
                 }
+#pragma unroll 4
+                for (; k < k1; ++k) add(*reinterpret_cast<const float4 *>(part_at(k) + e), w0[k]);
             } else {
                 for (int k = k0; k < k1; ++k) {
-                    const float *p = k ? rest + (size_t)(k - 1) * step : part0;
+                    const float *p = part_at(k);
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
                         if (e + i < heads * D) v[i] = fmaf(p[e + i], wgt[(e + i) / D * n + k], v[i]);

@@ -45,10 +45,12 @@ struct tc_smem {
     static constexpr int Q = NT * D * 2, P = KEYS * NT * 2;
     static constexpr int STAGE = 2 * MAT;
     static constexpr int at_q = NS * STAGE, at_p = at_q + 2 * Q, at_bar = at_p + 2 * P;
-    static constexpr int at_meta = at_bar + 24 * 8, at_scale = at_meta + NS * (int)sizeof(tile_meta), at_red = at_scale + 4 * GP * 4;
+    static constexpr int at_meta = at_bar + 24 * 8, at_scale = at_meta + NS * (int)sizeof(tile_meta), at_red = at_scale + 4 * 2 * GP * 4;
     static constexpr int at_max = at_red + 2 * 4 * GP * 4, at_tok = at_max + 2 * 4 * GP * 4;
     static constexpr int at_scan = at_tok + NS * KEYS * 4, at_pre = at_scan + 128 + 16;
-    static constexpr int total(int n_seq) { return at_pre + (n_seq + 1) * 4 + 1024; }  // 1024: room to align the stages
+    // the tile prefix, then each row's first key and end (bit 31: the end was cut to the table); 1024:
+    // room to align the stages
+    static constexpr int total(int n_seq) { return at_pre + (3 * n_seq + 1) * 4 + 1024; }
 };
 
 // Descriptor of an operand whose M (or N) index is contiguous, K rows one after another: V in rows
@@ -83,6 +85,25 @@ __device__ __forceinline__ void cp_async16p(unsigned dst, const void *src, bool 
         "l"(src), "r"(valid ? 16 : 0), "r"((int)on)
         : "memory");
 }
+// Eight values a lane over the warp, by op: 9 exchanges, each step leaving a lane half as many. The
+// result of value (lane / 4) is in lanes 4 (lane / 4) ...
+template <typename Op>
+__device__ __forceinline__ float reduce8(const float (&v)[8], int lane, Op op) {
+    float a[4], b[2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float keep = lane & 16 ? v[i + 4] : v[i], give = lane & 16 ? v[i] : v[i + 4];
+        a[i] = op(keep, __shfl_xor_sync(0xffffffffu, give, 16));
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const float keep = lane & 8 ? a[i + 2] : a[i], give = lane & 8 ? a[i] : a[i + 2];
+        b[i] = op(keep, __shfl_xor_sync(0xffffffffu, give, 8));
+    }
+    float c = op(lane & 4 ? b[1] : b[0], __shfl_xor_sync(0xffffffffu, lane & 4 ? b[0] : b[1], 4));
+    c = op(c, __shfl_xor_sync(0xffffffffu, c, 2));
+    return op(c, __shfl_xor_sync(0xffffffffu, c, 1));
+}
 // Barrier of the four softmax warps, and with it whether any thread's `x` holds.
 __device__ __forceinline__ void load_sync(int st) {
     if (st) asm volatile("barrier.cta.sync 3, 64;" ::: "memory");
@@ -116,6 +137,7 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 2 : 1)
     volatile int *abort = scan + 32;
     auto *tslot = reinterpret_cast<uint32_t *>(scan + 33);
     int *pre = reinterpret_cast<int *>(smem + S::at_pre);
+    unsigned *first_key = reinterpret_cast<unsigned *>(pre + a.n_seq + 1), *end_key = first_key + a.n_seq;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int *status = reinterpret_cast<int *>(a.status);
     constexpr int WAIT = (int)MOEARC_X_KV_WAIT;
@@ -147,11 +169,15 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 2 : 1)
     int run = 0;
     for (unsigned b = 0; b < a.n_seq; b += blockDim.x) {
         const unsigned i = b + threadIdx.x;
-        unsigned row, lo = 0, hi = 0;
+        unsigned row = 0, lo = 0, hi = 0;
         if (i < a.n_seq) span_of(a, L, i, row, lo, hi);
         int total;
         const int upto = block_scan(lo < hi ? (int)((hi - lo + KEYS - 1) / KEYS) : 0, scan, &total);
-        if (i < a.n_seq) pre[i + 1] = run + upto;
+        if (i < a.n_seq) {
+            pre[i + 1] = run + upto;
+            first_key[i] = lo;
+            end_key[i] = hi | (hi < a.n_kv[row] ? 1u << 31 : 0);
+        }
         run += total;
     }
     if (threadIdx.x == 0) pre[0] = 0;
@@ -198,7 +224,7 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 2 : 1)
             const int st = (warp - 5) >> 1, t = threadIdx.x - 160 - st * LOADERS;
             auto *tok = reinterpret_cast<int *>(smem + S::at_tok) + st * KEYS;
             int s = s0, vh = vh0, u0 = unit_start(s, vh), u1 = u0 + pre[s + 1] - pre[s], was = -1;
-            unsigned row, lo = 0, hi = 0, newest = 0, page[2], slot[2];
+            unsigned lo = 0, hi = 0, newest = 0, page[2], slot[2];
             const unsigned *tab = nullptr;
             auto look_up = [&](int g) {  // keys t and 64 + t of tile g, one of the group's tiles early
                 while (g >= u1) {
@@ -208,9 +234,10 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 2 : 1)
                 }
                 if (s != was) {
                     was = s;
-                    span_of(a, L, (unsigned)s, row, lo, hi);
-                    tab = a.tables + (size_t)row * a.max_pages;
-                    newest = a.k_new ? a.n_kv[row] - 1 : 0xffffffffu;
+                    lo = first_key[s];
+                    hi = end_key[s] & 0x7fffffffu;
+                    tab = a.tables + (size_t)(a.listed ? L.row[s] : s) * a.max_pages;
+                    newest = a.k_new && !(end_key[s] >> 31) ? hi - 1 : 0xffffffffu;
                 }
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
@@ -400,7 +427,10 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 2 : 1)
                     for (int r = 0; r < TERMS; ++r)
                         *reinterpret_cast<uint4 *>(qs + (ch >> 3) * NT * 128 + (r * 8 + h) * 128 + (((ch & 7) ^ h) << 4)) =
                             make_uint4(w[r][0], w[r][1], w[r][2], w[r][3]);
-                    if (ch == 0) scales[(u & 3) * GP + h] = a.scale2 / f;
+                    if (ch == 0) {
+                        scales[(u & 3) * 2 * GP + h] = a.scale2 / f;
+                        scales[((u & 3) * 2 + 1) * GP + h] = a.sinks && h < heads ? a.sinks[h0 + h] * LOG2E : -INFINITY;
+                    }
                 }
                 fence_async();
                 tc::bar_arrive(qfull + (u & 1));
@@ -440,7 +470,7 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 2 : 1)
                     for (int h = 0; h < GP; ++h) {
                         O[h] = l[h] = 0.f;
                         m[h] = -INFINITY;
-                        sc[h] = scales[(u & 3) * GP + h];
+                        sc[h] = scales[(u & 3) * 2 * GP + h];
                     }
                     pending = false;
                 }
@@ -463,11 +493,8 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 2 : 1)
                         ok = flush(i - 1) && ok;
                         pending = false;
                     }
-#pragma unroll
-                    for (int h = 0; h < GP; ++h) {
-                        const float x = warp_max(s[h]);
-                        if (lane == 0) mxs[(st * 4 + warp) * GP + h] = x;
-                    }
+                    const float top = reduce8(s, lane, [](float x, float y) { return fmaxf(x, y); });
+                    if ((lane & 3) == 0) mxs[(st * 4 + warp) * GP + (lane >> 2)] = top;
                     soft_sync();
 #pragma unroll
                     for (int h = 0; h < GP; ++h) {
@@ -497,12 +524,9 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 2 : 1)
                 if (pending) ok = ok && flush(i - 1);
                 pending = true;
                 if (flags & LAST) {
+                    const float part_l = reduce8(l, lane, [](float x, float y) { return x + y; });
+                    if ((lane & 3) == 0) red[((u & 1) * 4 + warp) * GP + (lane >> 2)] = part_l;
                     ok = ok && flush(i);
-#pragma unroll
-                    for (int h = 0; h < GP; ++h) {
-                        const float x = warp_sum(l[h]);
-                        if (lane == 0) red[((u & 1) * 4 + warp) * GP + h] = x;
-                    }
                     soft_sync();
                     const int kvh = vh / a.subs, sub = vh - kvh * a.subs;
                     const int h0 = kvh * a.group + sub * GP, heads = min(GP, a.group - sub * GP);
@@ -518,10 +542,11 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 2 : 1)
                         for (int h = 0; h < GP; ++h) {
                             if (h >= heads) break;
                             float sum = l[h], f = 1.f;
-                            if (a.sinks) {
-                                const float sk = a.sinks[h0 + h] * LOG2E, top = fmaxf(m[h], sk);
+                            const float sk = scales[((u & 3) * 2 + 1) * GP + h];
+                            if (sk != -INFINITY) {
+                                const float top = fmaxf(m[h], sk);
                                 f = m[h] == -INFINITY ? 0.f : ex2(m[h] - top);
-                                sum = sum * f + (sk == -INFINITY ? 0.f : ex2(sk - top));
+                                sum = sum * f + ex2(sk - top);
                             }
                             if (t < D) out[h * D + t] = sum == 0.f ? 0.f : O[h] * (f / sum);
                         }
