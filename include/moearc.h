@@ -722,8 +722,8 @@ int moearc_x_kv_status(moearc_ctx *c, const moearc_x_kv_cache *kv);
  * a row without tokens in range stores nothing. seqs: HOST list of distinct rows, or NULL for rows
  * 0 .. n_seq - 1; kv_begin: device [n_seq] or NULL (0); sinks: device [n_heads] or NULL. Queries,
  * and keys and values in range, are finite; what lies in pages outside the range may be anything.
- * Results do not depend on timing: the same call gives the same bits. Enqueues two kernels, no
- * allocation; lengths and tables are read on the device, so a captured call follows them. */
+ * Results do not depend on timing: the same call gives the same bits. Enqueues two kernels (three
+ * with seqs), no allocation; lengths and tables are read on the device, so a captured call follows them. */
 int moearc_x_attn_decode_batch(moearc_ctx *c, const moearc_x_kv_cache *kv, unsigned int layer, float *out, const float *q,
                                unsigned long q_stride, const float *k_new, const float *v_new, unsigned long new_stride,
                                const unsigned int *seqs, const unsigned int *kv_begin, const float *sinks, unsigned int n_seq,

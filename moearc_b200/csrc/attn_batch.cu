@@ -542,7 +542,7 @@ __host__ __device__ inline smem_layout layout_of(int n_seq, int warps, int ns, i
 
 template <class Tile, int MINB>
 __global__ void __launch_bounds__(Tile::WARPS * 32, MINB)
-    k_attn_batch(const __grid_constant__ attn_args a, const __grid_constant__ seq_list L, int ns) {
+    k_attn_batch(const __grid_constant__ attn_args a, int ns) {
     extern __shared__ __align__(1024) uint8_t smem[];
     constexpr int KEYS = Tile::KEYS, GP = Tile::GP;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
@@ -569,7 +569,7 @@ __global__ void __launch_bounds__(Tile::WARPS * 32, MINB)
     for (unsigned b = 0; b < a.n_seq; b += blockDim.x) {
         const unsigned i = b + threadIdx.x;
         unsigned row, lo = 0, hi = 0;
-        if (i < a.n_seq) span_of(a, L, i, row, lo, hi);
+        if (i < a.n_seq) span_of(a, i, row, lo, hi);
         int total;
         const int upto = block_scan(lo < hi ? (int)((hi - lo / KEYS * KEYS + R * KEYS - 1) / (R * KEYS)) : 0, sums, &total);
         if (i < a.n_seq) pre[i + 1] = run + upto;
@@ -618,7 +618,7 @@ __global__ void __launch_bounds__(Tile::WARPS * 32, MINB)
     const unsigned *ltab;
     size_t lhead;
     auto enter = [&]() {
-        span_of(a, L, (unsigned)ls, lrow, llo, lhi);
+        span_of(a, (unsigned)ls, lrow, llo, lhi);
         ltab = a.tables + (size_t)lrow * a.max_pages;
         lhead = (size_t)((lh * HG + hs) / a.subs) * a.head_bytes;
         lend = lh * line + pre[ls + 1];
@@ -666,7 +666,7 @@ __global__ void __launch_bounds__(Tile::WARPS * 32, MINB)
     for (int g = g0; g < g1; next_row(s, h)) {
         const int u0 = h * line + pre[s], u1 = h * line + pre[s + 1], first = g, end = min(u1, g1);
         unsigned row, lo, hi;
-        span_of(a, L, (unsigned)s, row, lo, hi);
+        span_of(a, (unsigned)s, row, lo, hi);
         const int vh = h * HG + hs, kvh = vh / a.subs, sub = vh - kvh * a.subs;
         const int h0 = kvh * a.group + sub * GP, heads = min(GP, a.group - sub * GP);
         const unsigned newest = a.k_new ? a.n_kv[row] - 1 : 0xffffffffu;
@@ -763,6 +763,32 @@ __global__ void __launch_bounds__(Tile::WARPS * 32, MINB)
     }
 }
 
+// The rows of a listed batch into the work buffer: by value into a launch of their own, so that the
+// launches that have none to pass stay short.
+template <int N>
+struct seq_list {
+    unsigned row[N];
+};
+template <int N>
+__global__ void __launch_bounds__(KV_LIST) k_attn_rows(const __grid_constant__ seq_list<N> L, unsigned n, unsigned *rows) {
+    pdl_trigger();
+    pdl_wait();
+    if (threadIdx.x < n) rows[threadIdx.x] = L.row[threadIdx.x];
+}
+template <typename F>
+cudaError_t with_list(const unsigned *rows, unsigned n, F &&f) {
+    auto fill = [&](auto &L) {
+        std::copy(rows, rows + n, L.row);
+        return f(L);
+    };
+    if (n <= 64) {
+        seq_list<64> L;
+        return fill(L);
+    }
+    seq_list<KV_LIST> L;
+    return fill(L);
+}
+
 // ---- host side --------------------------------------------------------------------------------
 
 // How a shape is cut: virtual heads and warps per CTA, stages, shared memory and the grid.
@@ -843,18 +869,18 @@ bool plan_of(attn_plan &p, bool mma, unsigned kv_type, int n_heads, int n_kv, in
     });
 }
 
-// The work buffer: a note a CTA, then the parts.
-size_t attn_bytes(int grid, int hg, int gp, int D) { return (size_t)grid * 16 + (size_t)grid * 2 * hg * gp * (D + 2) * 4; }
+// The work buffer: the rows' list, a note a CTA, then the parts.
+size_t attn_bytes(int grid, int hg, int gp, int D) { return KV_LIST * 4 + (size_t)grid * 16 + (size_t)grid * 2 * hg * gp * (D + 2) * 4; }
 size_t attn_bytes(const attn_plan &p, int D) { return attn_bytes(p.grid, p.hg, p.gp, D); }
 
 template <class Tile, int MINB>
-cudaError_t launch(moearc_ctx *c, const attn_plan &p, const attn_args &a, const seq_list &L) {
+cudaError_t launch(moearc_ctx *c, const attn_plan &p, const attn_args &a) {
     static std::atomic<bool> done[MOEARC_MAX_DEVICES];
     cudaError_t e = once_per_device(done, [] {
         return set_smem(k_attn_batch<Tile, MINB>, MAX_SMEM - 512);
     });
     if (e == cudaSuccess)
-        e = launch_pdl(k_attn_batch<Tile, MINB>, dim3((unsigned)p.grid), dim3((unsigned)p.warps * 32), (size_t)p.smem, c->stream, a, L, p.ns);
+        e = launch_pdl(k_attn_batch<Tile, MINB>, dim3((unsigned)p.grid), dim3((unsigned)p.warps * 32), (size_t)p.smem, c->stream, a, p.ns);
     if (e == cudaSuccess) e = attn_join_launch<Tile::GP>(c, p.grid, a);
     return e;
 }
@@ -896,13 +922,10 @@ int moearc_x_attn_decode_batch(moearc_ctx *c, const moearc_x_kv_cache *kv, unsig
     const size_t D = kv->head_dim;
     if (q_stride < n_heads * D || (k_new && new_stride < kv->n_kv_heads * D)) return ERR_ARG;
     if (!(scale == scale) || scale - scale != 0.f) return ERR_ARG;
-    seq_list L;
     if (seqs) {
         kv_rows_seen seen(kv->max_seq);
-        for (unsigned i = 0; i < n_seq; ++i) {
+        for (unsigned i = 0; i < n_seq; ++i)
             if (!seen.add(seqs[i], kv->max_seq)) return ERR_ARG;
-            L.row[i] = seqs[i];
-        }
     } else if (n_seq > kv->max_seq) {
         return ERR_ARG;
     }
@@ -940,7 +963,6 @@ int moearc_x_attn_decode_batch(moearc_ctx *c, const moearc_x_kv_cache *kv, unsig
     const uintptr_t rows = align | a.head_bytes;
     a.unit = (rows & 15) == 0 ? 16 : (rows & 3) == 0 ? 4 : 2;
     a.one_page = a.unit == 16 && kv->page_tokens % (unsigned)p.keys == 0;
-    a.listed = seqs != nullptr;
     a.n_heads = (int)n_heads;
     a.group = (int)(n_heads / kv->n_kv_heads);
     a.D = (int)D;
@@ -951,13 +973,20 @@ int moearc_x_attn_decode_batch(moearc_ctx *c, const moearc_x_kv_cache *kv, unsig
     a.min_tiles = 1;
     a.scale2 = scale * LOG2E;
     a.status = kv->status;
-    a.notes = static_cast<int4 *>(kv->work);
+    a.rows = seqs ? static_cast<unsigned *>(kv->work) : nullptr;
+    a.notes = reinterpret_cast<int4 *>(static_cast<uint8_t *>(kv->work) + KV_LIST * 4);
     a.part = reinterpret_cast<float *>(a.notes + (tc ? tc_grid : p.grid));
     device_guard g(c->device);
     if (!g.ok) return ERR;
     launch_scope ls(c, "attn_decode_batch", n_seq, n_heads);
-    const cudaError_t e = tc ? attn_tc_launch(c, *kv, a, L) : with_tile(mma, kv->kv_type, kv->head_dim, a.group, [&](auto *t, auto minb) {
-        return launch<std::remove_pointer_t<decltype(t)>, decltype(minb)::value>(c, p, a, L);
+    cudaError_t e = cudaSuccess;
+    if (seqs)
+        e = with_list(seqs, n_seq, [&](auto &L) {
+            constexpr int N = (int)(sizeof(L.row) / sizeof(unsigned));
+            return launch_pdl(k_attn_rows<N>, dim3(1), dim3(KV_LIST), 0, c->stream, L, n_seq, static_cast<unsigned *>(kv->work));
+        });
+    if (e == cudaSuccess) e = tc ? attn_tc_launch(c, *kv, a) : with_tile(mma, kv->kv_type, kv->head_dim, a.group, [&](auto *t, auto minb) {
+        return launch<std::remove_pointer_t<decltype(t)>, decltype(minb)::value>(c, p, a);
     });
     if (e != cudaSuccess) cudaGetLastError();  // the failed launch's error, not left for an unrelated later check
     const int rc2 = ls.finish();

@@ -13,10 +13,6 @@ constexpr int MAX_SMEM = 227 * 1024;
 // above (in powers of two): most tiles then rescale nothing, and weights stay below 2^8.
 constexpr float LAZY = 8.f;
 
-struct seq_list {
-    unsigned row[KV_LIST];
-};
-
 struct attn_args {
     float *out;
     const float *q, *k_new, *v_new, *sinks;
@@ -27,7 +23,7 @@ struct attn_args {
     unsigned n_seq, max_pages, n_pages, pt, pt_inv, cap;  // pt_inv: floor(2^32 / pt), at most 2^32 - 1
     unsigned unit;  // bytes of one copy: 16 where rows start on 16-byte boundaries, else 4 or 2
     int one_page;   // tiles never cross a page
-    int listed;  // rows come from the list (else row i is batch row i)
+    const unsigned *rows;  // the batch rows' cache rows, or null: row i is i
     int n_heads, group, D, subs;  // subs: virtual heads a kv head (its query heads by GP)
     int hg, rsplit, nhg;          // virtual heads a CTA, warps a head, head groups
     int min_tiles;
@@ -37,8 +33,8 @@ struct attn_args {
 };
 
 // The keys [lo, hi) of batch row i in cache row `row`, hi cut to the table.
-__device__ __forceinline__ void span_of(const attn_args &a, const seq_list &L, unsigned i, unsigned &row, unsigned &lo, unsigned &hi) {
-    row = a.listed ? L.row[i] : i;
+__device__ __forceinline__ void span_of(const attn_args &a, unsigned i, unsigned &row, unsigned &lo, unsigned &hi) {
+    row = a.rows ? a.rows[i] : i;
     hi = min(a.n_kv[row], a.cap);
     lo = a.begin ? min(a.begin[i], hi) : 0;
 }
@@ -256,6 +252,6 @@ static cudaError_t attn_join_launch(moearc_ctx *c, int grid, const attn_args &a)
 // The tcgen05 kernel (attn_tc.cu): whether it serves a shape, its grid, and its launch.
 bool attn_tc_serves(const moearc_x_kv_cache &kv, unsigned layer);
 int attn_tc_grid(unsigned head_dim, int sms);
-cudaError_t attn_tc_launch(moearc_ctx *c, const moearc_x_kv_cache &kv, attn_args a, const seq_list &L);
+cudaError_t attn_tc_launch(moearc_ctx *c, const moearc_x_kv_cache &kv, attn_args a);
 
 }  // namespace moearc

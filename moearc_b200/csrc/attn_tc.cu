@@ -45,7 +45,7 @@ struct tc_smem {
     static constexpr int Q = NT * D * 2, P = KEYS * NT * 2;
     static constexpr int STAGE = 2 * MAT;
     static constexpr int at_q = NS * STAGE, at_p = at_q + 2 * Q, at_bar = at_p + 2 * P;
-    static constexpr int at_meta = at_bar + 24 * 8, at_scale = at_meta + NS * (int)sizeof(tile_meta), at_red = at_scale + 4 * 2 * GP * 4;
+    static constexpr int at_meta = at_bar + 24 * 8, at_scale = at_meta + NS * (int)sizeof(tile_meta), at_red = at_scale + 8 * 2 * GP * 4;
     static constexpr int at_max = at_red + 2 * 4 * GP * 4, at_tok = at_max + 2 * 4 * GP * 4;
     static constexpr int at_scan = at_tok + NS * KEYS * 4, at_pre = at_scan + 128 + 16;
     // the tile prefix, then each row's first key and end (bit 31: the end was cut to the table); 1024:
@@ -122,7 +122,7 @@ __device__ __forceinline__ bool soft_any(bool x) {
 
 template <int D, bool BF>
 __global__ void __launch_bounds__(THREADS, D == 64 ? 2 : 1)
-    k_attn_tc(const __grid_constant__ attn_args a, const __grid_constant__ seq_list L) {
+    k_attn_tc(const __grid_constant__ attn_args a) {
     using S = tc_smem<D>;
     constexpr int CH = D / 8, TERMS = BF ? 3 : 2;
     constexpr float PSCALE = BF ? 1.f : 64.f;
@@ -132,6 +132,7 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 2 : 1)
     uint64_t *kfull = bars, *vfull = bars + 2, *empty = bars + 4, *qfull = bars + 6, *qempty = bars + 8, *sfull = bars + 10,
              *pfull = bars + 12, *ofull = bars + 14, *qready = bars + 16, *done = bars + 20;
     auto *meta = reinterpret_cast<volatile tile_meta *>(smem + S::at_meta);
+    // of eight units: a unit's are read until its close, when the queries may be four units ahead
     auto *scales = reinterpret_cast<float *>(smem + S::at_scale);
     auto *scan = reinterpret_cast<int *>(smem + S::at_scan);
     volatile int *abort = scan + 32;
@@ -170,7 +171,7 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 2 : 1)
     for (unsigned b = 0; b < a.n_seq; b += blockDim.x) {
         const unsigned i = b + threadIdx.x;
         unsigned row = 0, lo = 0, hi = 0;
-        if (i < a.n_seq) span_of(a, L, i, row, lo, hi);
+        if (i < a.n_seq) span_of(a, i, row, lo, hi);
         int total;
         const int upto = block_scan(lo < hi ? (int)((hi - lo + KEYS - 1) / KEYS) : 0, scan, &total);
         if (i < a.n_seq) {
@@ -236,7 +237,7 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 2 : 1)
                     was = s;
                     lo = first_key[s];
                     hi = end_key[s] & 0x7fffffffu;
-                    tab = a.tables + (size_t)(a.listed ? L.row[s] : s) * a.max_pages;
+                    tab = a.tables + (size_t)(a.rows ? a.rows[s] : (unsigned)s) * a.max_pages;
                     newest = a.k_new && !(end_key[s] >> 31) ? hi - 1 : 0xffffffffu;
                 }
 #pragma unroll
@@ -428,8 +429,8 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 2 : 1)
                         *reinterpret_cast<uint4 *>(qs + (ch >> 3) * NT * 128 + (r * 8 + h) * 128 + (((ch & 7) ^ h) << 4)) =
                             make_uint4(w[r][0], w[r][1], w[r][2], w[r][3]);
                     if (ch == 0) {
-                        scales[(u & 3) * 2 * GP + h] = a.scale2 / f;
-                        scales[((u & 3) * 2 + 1) * GP + h] = a.sinks && h < heads ? a.sinks[h0 + h] * LOG2E : -INFINITY;
+                        scales[(u & 7) * 2 * GP + h] = a.scale2 / f;
+                        scales[((u & 7) * 2 + 1) * GP + h] = a.sinks && h < heads ? a.sinks[h0 + h] * LOG2E : -INFINITY;
                     }
                 }
                 fence_async();
@@ -470,7 +471,7 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 2 : 1)
                     for (int h = 0; h < GP; ++h) {
                         O[h] = l[h] = 0.f;
                         m[h] = -INFINITY;
-                        sc[h] = scales[(u & 3) * 2 * GP + h];
+                        sc[h] = scales[(u & 7) * 2 * GP + h];
                     }
                     pending = false;
                 }
@@ -542,7 +543,7 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 2 : 1)
                         for (int h = 0; h < GP; ++h) {
                             if (h >= heads) break;
                             float sum = l[h], f = 1.f;
-                            const float sk = scales[((u & 3) * 2 + 1) * GP + h];
+                            const float sk = scales[((u & 7) * 2 + 1) * GP + h];
                             if (sk != -INFINITY) {
                                 const float top = fmaxf(m[h], sk);
                                 f = m[h] == -INFINITY ? 0.f : ex2(m[h] - top);
@@ -575,13 +576,13 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 2 : 1)
 }
 
 template <int D, bool BF>
-cudaError_t launch(moearc_ctx *c, attn_args &a, const seq_list &L) {
+cudaError_t launch(moearc_ctx *c, attn_args &a) {
     static std::atomic<bool> done[MOEARC_MAX_DEVICES];
     const cudaError_t e = once_per_device(done, [] { return set_smem(k_attn_tc<D, BF>, tc_smem<D>::total((int)KV_LIST)); });
     if (e != cudaSuccess) return e;
     const int grid = attn_tc_grid(D, c->sm_count);
     const cudaError_t e2 =
-        launch_pdl(k_attn_tc<D, BF>, dim3((unsigned)grid), dim3(THREADS), (size_t)tc_smem<D>::total((int)a.n_seq), c->stream, a, L);
+        launch_pdl(k_attn_tc<D, BF>, dim3((unsigned)grid), dim3(THREADS), (size_t)tc_smem<D>::total((int)a.n_seq), c->stream, a);
     return e2 != cudaSuccess ? e2 : attn_join_launch<GP>(c, grid, a);
 }
 
@@ -597,12 +598,12 @@ bool attn_tc_serves(const moearc_x_kv_cache &kv, unsigned layer) {
            (unsigned long long)kv.n_pages * kv.page_tokens < (1ull << 31);  // tokens are numbered in 32 bits
 }
 
-cudaError_t attn_tc_launch(moearc_ctx *c, const moearc_x_kv_cache &kv, attn_args a, const seq_list &L) {
+cudaError_t attn_tc_launch(moearc_ctx *c, const moearc_x_kv_cache &kv, attn_args a) {
     a.subs = (a.group + GP - 1) / GP;
     a.hg = 1;
     a.nhg = (int)kv.n_kv_heads * a.subs;
-    if (kv.head_dim == 64) return kv.kv_type == T_BF16 ? launch<64, true>(c, a, L) : launch<64, false>(c, a, L);
-    return kv.kv_type == T_BF16 ? launch<128, true>(c, a, L) : launch<128, false>(c, a, L);
+    if (kv.head_dim == 64) return kv.kv_type == T_BF16 ? launch<64, true>(c, a) : launch<64, false>(c, a);
+    return kv.kv_type == T_BF16 ? launch<128, true>(c, a) : launch<128, false>(c, a);
 }
 
 }  // namespace moearc
