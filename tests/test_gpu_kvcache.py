@@ -374,3 +374,163 @@ def test_attention_without_rows_and_its_checks(ctx):
         p.c.attn_decode(0, b, b, 2, 4, 1.0, k_new=b, v_new=b, seqs=[1, 1])
     with pytest.raises(Exception):
         p.c.attn_decode(0, b, b, 2, 4, 1.0, k_new=b)
+
+
+# ---- together, as a serving loop uses them -------------------------------------------------------
+
+def step_inputs(rng, n, H, kvh, D):
+    return (rng.standard_normal((n, H, D), np.float32), rng.standard_normal((n, kvh, D), np.float32), rng.standard_normal((n, kvh, D), np.float32))
+
+
+@pytest.mark.parametrize("kv, H, kvh, D, pt", [(BF16, 16, 2, 64, 8), (F16, 8, 2, 128, 5), (F32, 6, 3, 40, 4)])
+def test_a_serving_loop(ctx, kv, H, kvh, D, pt):
+    """Rows are started, decoded over two layers, scored, forked from the better and dropped from the
+    worse, cut back and compacted; every step's attention, pools and tables follow the model."""
+    rng = np.random.default_rng(D)
+    p = Pair(ctx, layers=2, pages=120, pt=pt, kvh=kvh, D=D, kv=kv, rows=10, max_pages=14, n_heads=H, seed=D)
+    p.do("grow", [0, 1, 2], [13, 1, 2 * pt])  # prompts, whose keys the pools hold already
+    alive, V = [0, 1, 2], 500
+    for step in range(8):
+        p.do("grow", alive, [1] * len(alive))
+        n = len(alive)
+        for layer in range(2):
+            q, kn, vn = step_inputs(rng, n, H, kvh, D)
+            out = ctx.alloc_n(np.float32, n * H * D)
+            p.c.attn_decode(layer, out, ctx.upload_new(q), n, H, D ** -0.5, seqs=alive, k_new=ctx.upload_new(kn), v_new=ctx.upload_new(vn))
+            want, vmax, amax = attend(p.m, layer, q, D ** -0.5, alive, k_new=kn, v_new=vn)
+            got = ctx.download(out, np.float32, n * H * D).reshape(want.shape)
+            assert np.abs(got - want).max() <= attend_tolerance(vmax, amax, D, max(p.m.n_kv))
+        p.same()
+        logits = rng.standard_normal((n, V)).astype(np.float32) + got.reshape(n, -1)[:, :1]
+        ids, top = ctx.alloc_n(np.uint32, n * 2), ctx.alloc_n(np.float32, n * 2)
+        ctx.token_logprobs(ctx.upload_new(logits), F32, n, V, k=2, top_ids=ids, top_logprobs=top)
+        assert (ctx.download(ids, np.uint32, 2 * n).reshape(n, 2)[:, 0] == logits.argmax(1)).all()
+        order = np.argsort(-ctx.download(top, np.float32, 2 * n).reshape(n, 2)[:, 0])
+        best, worst = alive[order[0]], alive[order[-1]]
+        if len(alive) > 2:
+            p.do("free", [worst])
+            alive.remove(worst)
+        new = [r for r in range(10) if p.m.n_kv[r] == 0][:2]
+        p.do("fork", [best] * len(new), new, deep=step == 3)
+        alive += new
+        if step % 3 == 2:
+            p.do("free", [alive[0]], [max(1, p.m.n_kv[alive[0]] - pt - 1)])  # rejected tokens
+            p.do("compact")
+        p.same()
+
+
+def test_a_captured_step_follows_the_cache(ctx):
+    """Growing, attention and scores captured once: each replay takes the lengths and tables it finds."""
+    torch = pytest.importorskip("torch")
+    H, kvh, D, pt, n, V = 8, 2, 64, 4, 3, 300
+    rng = np.random.default_rng(3)
+    p = Pair(ctx, layers=1, pages=40, pt=pt, kvh=kvh, D=D, rows=4, max_pages=12, n_heads=H)
+    p.do("grow", [0, 1, 3], [5, 1, 9])
+    q, kn, vn = step_inputs(rng, n, H, kvh, D)
+    dq, dk, dv, out = ctx.upload_new(q), ctx.upload_new(kn), ctx.upload_new(vn), ctx.alloc_n(np.float32, n * H * D)
+    logits, ent = ctx.upload_new(rng.standard_normal((n, V), np.float32)), ctx.alloc_n(np.float32, n)
+
+    def step():
+        p.c.grow([0, 1, 3], [1, 1, 1])
+        p.c.attn_decode(0, out, dq, n, H, 0.125, seqs=[0, 1, 3], k_new=dk, v_new=dv)
+        ctx.token_logprobs(logits, F32, n, V, entropy=ent)
+
+    def check():
+        p.m.grow([0, 1, 3], [1, 1, 1])
+        want, vmax, amax = attend(p.m, 0, q, 0.125, [0, 1, 3], k_new=kn, v_new=vn)
+        got = ctx.download(out, np.float32, n * H * D).reshape(want.shape)
+        assert np.abs(got - want).max() <= attend_tolerance(vmax, amax, D, 50)
+        assert np.isfinite(ctx.download(ent, np.float32, n)).all()
+        p.same()
+
+    step()  # attributes are set on the first call, outside a capture
+    check()
+    stream = torch.cuda.ExternalStream(ctx.lib.moearc_x_stream(ctx.raw))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        step()
+    for _ in range(6):
+        with torch.cuda.stream(stream):
+            graph.replay()
+        ctx.sync()
+        check()
+    p.do("free", [1])
+    p.do("fork", [3], [1])
+    p.do("compact")
+    with torch.cuda.stream(stream):
+        graph.replay()
+    check()
+    del graph
+
+
+def test_two_contexts_at_once():
+    """Two caches on two streams, interleaved without waiting: neither sees the other."""
+    a, b = Context(), Context()
+    H, kvh, D, n = 16, 2, 128, 4
+    rng = np.random.default_rng(9)
+    sides = []
+    for c, kv in ((a, BF16), (b, F16)):
+        p = Pair(c, layers=1, pages=400, pt=16, kvh=kvh, D=D, kv=kv, rows=n, max_pages=90, n_heads=H, seed=kv)
+        p.do("grow", list(range(n)), [1200, 7, 300, 64])
+        q = rng.standard_normal((n, H, D)).astype(np.float32)
+        sides.append((p, q, c.upload_new(q), [c.alloc_n(np.float32, n * H * D) for _ in range(20)]))
+    for i in range(20):
+        for p, q, dq, outs in sides:
+            p.c.attn_decode(0, outs[i], dq, n, H, D ** -0.5)
+    for p, q, dq, outs in sides:
+        want, vmax, amax = attend(p.m, 0, q, D ** -0.5)
+        first = p.ctx.download(outs[0], np.float32, want.size)
+        assert np.abs(first.reshape(want.shape) - want).max() <= attend_tolerance(vmax, amax, D, 1200)
+        for o in outs[1:]:
+            assert np.array_equal(p.ctx.download(o, np.float32, want.size), first)
+    for c in (a, b):
+        c.close()
+
+
+@pytest.mark.parametrize("kv, H, kvh, D, pt", [(BF16, 16, 4, 128, 16), (F32, 8, 4, 128, 16)])
+def test_pools_past_32_bit_offsets(ctx, kv, H, kvh, D, pt):
+    """Pages beyond 4 GiB (and 2^31 elements) of a pool: attention, the new token's store and copies."""
+    size = 4 if kv == F32 else 2
+    page_bytes = pt * kvh * D * size
+    pages = (5 << 30) // page_bytes + 5
+    small = Paged(1, 8, pt, kvh, D, kv, 3, 6, seed=4)
+    far = [pages - 1 - i for i in range(4)] + list(range(4))  # where the model's pages lie
+    pools = [ctx.alloc(pages * page_bytes) for _ in range(2)]
+    for pool, host in zip(pools, (small.k, small.v)):
+        for i, f in enumerate(far):
+            ctx.upload(pool.view(f * page_bytes, page_bytes), host[0, i])
+    c = KvCache(ctx, n_layer=1, n_pages=pages, page_tokens=pt, n_kv_heads=kvh, head_dim=D, kv_type=kv, max_seq=3, max_pages=6,
+                n_heads=H, k_pages=[pools[0]], v_pages=[pools[1]])
+    small.tables[0][:3], small.n_kv[0] = [0, 4, 1], 3 * pt - 2
+    refs = np.zeros(pages, np.uint32)
+    refs[:4] = 1  # taken, so that the copies below go to pages that are far, then near
+    refs[far[0]] = refs[far[1]] = 1
+    tables = np.full((3, 6), NO_PAGE, np.uint32)
+    tables[0, :3] = [far[p] for p in small.tables[0][:3]]
+    ctx.upload(c.tables, tables)
+    ctx.upload(c.n_kv, np.array(small.n_kv, np.uint32))
+    ctx.upload(c.refs, refs)
+    rng = np.random.default_rng(1)
+    q, kn, vn = step_inputs(rng, 1, H, kvh, D)
+    out = ctx.alloc_n(np.float32, H * D)
+    c.attn_decode(0, out, ctx.upload_new(q), 1, H, D ** -0.5, k_new=ctx.upload_new(kn), v_new=ctx.upload_new(vn))
+    want, vmax, amax = attend(small, 0, q, D ** -0.5, k_new=kn, v_new=vn)
+    assert np.abs(ctx.download(out, np.float32, H * D).reshape(want.shape) - want).max() <= attend_tolerance(vmax, amax, D, 3 * pt)
+    for pool, host in zip(pools, (small.k, small.v)):
+        for i, f in enumerate(far):
+            assert np.array_equal(ctx.download(pool.view(f * page_bytes, page_bytes), host.dtype, host[0, i].size), host[0, i].ravel())
+    c.fork([0], [1], deep=True)
+    t = ctx.download(c.tables, np.uint32, 18).reshape(3, 6)
+    assert t[1, :3].tolist() == [4, 5, 6] and c.status() == 0
+    refs[:] = 1  # only far pages are free
+    refs[far[2]] = refs[far[3]] = 0
+    ctx.upload(c.refs, refs)
+    c.fork([0], [2])
+    t = ctx.download(c.tables, np.uint32, 18).reshape(3, 6)
+    assert t[2, :3].tolist() == [t[0, 0], t[0, 1], min(far[2], far[3])]
+    for a, b in zip(list(t[0, :3]) * 2, list(t[1, :3]) + list(t[2, :3])):
+        for pool in pools:
+            x, y = (ctx.download(pool.view(int(f) * page_bytes, page_bytes), np.uint32, page_bytes // 4) for f in (a, b))
+            assert np.array_equal(x, y)
+    for b in pools:
+        b.free()

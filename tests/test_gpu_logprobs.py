@@ -162,3 +162,19 @@ def test_checks(ctx):
     with pytest.raises(BadArgument):
         ctx.token_logprobs(b, 39, 1, 100, entropy=b)
     ctx.token_logprobs(b, F32, 0, 100, entropy=b)
+
+
+def test_rows_past_32_bit_offsets(ctx):
+    """The last row of logits starts beyond 2^32 elements."""
+    V, n = 200003, 22000
+    buf = ctx.alloc(n * V * 2)
+    x = np.random.default_rng(7).standard_normal(V).astype(np.float32)
+    bits = store(x, BF16)
+    ctx.upload(buf.view((n - 1) * V * 2, V * 2), bits)
+    ids, top, ent = ctx.alloc_n(np.uint32, n), ctx.alloc_n(np.float32, n), ctx.alloc_n(np.float32, n)
+    ctx.token_logprobs(buf, BF16, n, V, entropy=ent, k=1, top_ids=ids, top_logprobs=top)
+    y = as_f32(bits, BF16).astype(np.float64)
+    assert ctx.download(ids, np.uint32, n)[-1] == int(y.argmax())
+    lse = np.log(np.exp(y - y.max()).sum()) + y.max()
+    assert abs(ctx.download(top, np.float32, n)[-1] - (y.max() - lse)) <= 1e-4  # as in check(): V / 256 sums
+    buf.free()
