@@ -671,7 +671,7 @@ typedef struct {
     void *const *v_pages;      /* page_tokens x n_kv_heads x head_dim elements each */
     unsigned int n_layer;      /* <= MOEARC_X_KV_LAYERS */
     unsigned int n_pages;      /* <= 2^28 */
-    unsigned int page_tokens;  /* any size; max_pages * page_tokens < 2^31 */
+    unsigned int page_tokens;  /* any size; max_pages * page_tokens < 2^31, a page < 2^31 elements */
     unsigned int n_kv_heads, head_dim;  /* head_dim <= 1024 */
     unsigned int kv_type;      /* F32 0, F16 1, BF16 30 */
     unsigned int max_seq;      /* rows, <= 65536 */
@@ -683,8 +683,8 @@ typedef struct {
     void *work;                /* device, 16-byte aligned; holds nothing between calls */
     unsigned long work_bytes;  /* >= moearc_x_kv_work_bytes */
 } moearc_x_kv_cache;
-/* Bytes of `work` that the page calls and attention with up to n_heads query heads (0: page calls
- * only) need; 0 on an unsupported shape. */
+/* Bytes of `work` that the page calls and, with n_heads > 0, attention need; enough for any other
+ * multiple of n_kv_heads query heads too. 0 on an unsupported shape. */
 unsigned long moearc_x_kv_work_bytes(moearc_ctx *c, const moearc_x_kv_cache *kv, unsigned int n_heads);
 /* Every row empty, every page free, status 0. The pools are left as they are. */
 int moearc_x_kv_reset(moearc_ctx *c, const moearc_x_kv_cache *kv);
@@ -704,8 +704,8 @@ int moearc_x_kv_fork(moearc_ctx *c, const moearc_x_kv_cache *kv, const unsigned 
 int moearc_x_kv_free(moearc_ctx *c, const moearc_x_kv_cache *kv, const unsigned int *seqs, const unsigned int *keep,
                      unsigned int n);
 /* Moves the pages in use together: with n_live of them, the i-th live page at or past n_live moves, in
- * every pool, to the i-th free page below it. tables_out, refs_out (each may be the cache's own
- * array) get the tables and counts that go with the moved pages, *n_live (device word, may be
+ * every pool, to the i-th free page below it. tables_out, refs_out (both the cache's own
+ * arrays, or both others) get the tables and counts that go with the moved pages, *n_live (device word, may be
  * NULL) their number. The pages moved from keep their contents, so the old tables stay readable
  * until pages at or past n_live are handed out again. */
 int moearc_x_kv_compact(moearc_ctx *c, const moearc_x_kv_cache *kv, unsigned int *tables_out, unsigned int *refs_out,
@@ -722,7 +722,7 @@ int moearc_x_kv_status(moearc_ctx *c, const moearc_x_kv_cache *kv);
  * a row without tokens in range stores nothing. seqs: HOST list of distinct rows, or NULL for rows
  * 0 .. n_seq - 1; kv_begin: device [n_seq] or NULL (0); sinks: device [n_heads] or NULL. Queries,
  * and keys and values in range, are finite; what lies in pages outside the range may be anything.
- * Results do not depend on timing: the same call gives the same bits. Enqueues two kernels (three
+ * out overlaps no input. Results do not depend on timing: the same call gives the same bits. Enqueues two kernels (three
  * with seqs), no allocation; lengths and tables are read on the device, so a captured call follows them. */
 int moearc_x_attn_decode_batch(moearc_ctx *c, const moearc_x_kv_cache *kv, unsigned int layer, float *out, const float *q,
                                unsigned long q_stride, const float *k_new, const float *v_new, unsigned long new_stride,

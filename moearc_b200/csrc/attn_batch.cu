@@ -872,6 +872,9 @@ bool plan_of(attn_plan &p, bool mma, unsigned kv_type, int n_heads, int n_kv, in
 // The work buffer: the rows' list, a note a CTA, then the parts.
 size_t attn_bytes(int grid, int hg, int gp, int D) { return KV_LIST * 4 + (size_t)grid * 16 + (size_t)grid * 2 * hg * gp * (D + 2) * 4; }
 size_t attn_bytes(const attn_plan &p, int D) { return attn_bytes(p.grid, p.hg, p.gp, D); }
+// Most query heads that the CTAs of an SM work on at once, CTAs x hg x gp: 2 x 8 x 8 (tensor-core tiles
+// of 64 channels) or 1 x 16 x 8 (CUDA cores) up to 128 channels, 8 warps of 8 or of 4 heads above.
+int heads_of_sm(unsigned D) { return D <= 128 ? 128 : D <= 256 ? 64 : 32; }
 
 template <class Tile, int MINB>
 cudaError_t launch(moearc_ctx *c, const attn_plan &p, const attn_args &a) {
@@ -894,18 +897,11 @@ unsigned long moearc_x_kv_work_bytes(moearc_ctx *c, const moearc_x_kv_cache *kv,
     size_t need = kv_page_work_bytes(kv->n_pages);
     if (n_heads) {
         if (n_heads > 65535 || n_heads % kv->n_kv_heads) return 0;
-        // the cut goes by the batch (its prefix takes shared memory) and, for 16-bit caches, by the
-        // pools' alignment: the largest of them all
+        // the cut goes by the batch, the heads and the pools' alignment: the most that any takes
         const int D = (int)kv->head_dim;
         attn_plan p;
-        for (int n = 32; n <= (int)KV_LIST; n += 32) {
-            if (!plan_of(p, false, kv->kv_type, (int)n_heads, (int)kv->n_kv_heads, D, n, c->sm_count)) return 0;
-            need = std::max(need, attn_bytes(p, D));
-            if (kv->kv_type == T_F32 || !mma_dim(kv->head_dim)) continue;
-            if (!plan_of(p, true, kv->kv_type, (int)n_heads, (int)kv->n_kv_heads, D, n, c->sm_count)) return 0;
-            need = std::max(need, attn_bytes(p, D));
-        }
-        need = std::max(need, attn_bytes(attn_tc_grid(kv->head_dim, c->sm_count), 1, 8, D));
+        if (!plan_of(p, false, kv->kv_type, (int)n_heads, (int)kv->n_kv_heads, D, (int)KV_LIST, c->sm_count)) return 0;
+        need = std::max(need, KV_LIST * 4 + (size_t)c->sm_count * (2 * 16 + 2 * (size_t)heads_of_sm(kv->head_dim) * (D + 2) * 4));
     }
     return need;
 }

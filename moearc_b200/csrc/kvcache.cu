@@ -400,13 +400,11 @@ int finish(moearc_ctx *c, cudaError_t e) {
     return c->sync_each && cudaStreamSynchronize(c->stream) != cudaSuccess ? ERR : OK;
 }
 
-// kv_check, the work buffer's size and the page size's limit for the copy's 32-bit element index.
+// kv_check and the work buffer's size.
 int page_call_check(moearc_ctx *c, const moearc_x_kv_cache *kv) {
     const int rc = kv_check(c, kv);
     if (rc) return rc;
-    if (kv->work_bytes < kv_plan_bytes(kv->n_pages)) return ERR_ARG;
-    if ((unsigned long long)kv->page_tokens * kv->n_kv_heads * kv->head_dim >= (1ull << 31)) return ERR_ARG;
-    return OK;
+    return kv->work_bytes < kv_plan_bytes(kv->n_pages) ? ERR_ARG : OK;
 }
 
 }  // namespace
@@ -510,6 +508,7 @@ int moearc_x_kv_compact(moearc_ctx *c, const moearc_x_kv_cache *kv, unsigned int
     const int rc = page_call_check(c, kv);
     if (rc) return rc;
     if (!tables_out || !refs_out) return ERR;
+    if ((tables_out == kv->tables) != (refs_out == kv->refs)) return ERR_ARG;  // counts that do not go with the tables
     device_guard g(c->device);
     if (!g.ok) return ERR;
     const work_view w = work_of(kv->work, kv->n_pages);

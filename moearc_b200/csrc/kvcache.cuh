@@ -20,7 +20,8 @@ inline bool kv_shape_ok(const moearc_x_kv_cache &k) {
     return k.n_layer >= 1 && k.n_layer <= KV_LAYERS && k.n_pages >= 1 && k.n_pages <= (1u << 28) && k.page_tokens >= 1 &&
            k.n_kv_heads >= 1 && k.n_kv_heads <= 65535 && k.head_dim >= 1 && k.head_dim <= 1024 && kv_elem_bytes(k.kv_type) &&
            k.max_seq >= 1 && k.max_seq <= KV_MAX_SEQ && k.max_pages >= 1 && k.max_pages <= (1u << 24) &&
-           (unsigned long long)k.max_pages * k.page_tokens < (1ull << 31);
+           (unsigned long long)k.max_pages * k.page_tokens < (1ull << 31) &&
+           (unsigned long long)k.page_tokens * k.n_kv_heads < (1ull << 31) / k.head_dim;  // a page's elements, for 32-bit indexes
 }
 
 // 0 when every pointer is there and every number in range; else the code to return.

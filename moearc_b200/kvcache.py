@@ -44,7 +44,8 @@ def _at(a: array) -> int:
 
 
 class KvCache:
-    """Buffers that are not given are allocated and set up as the empty cache (``reset``); with any
+    """n_heads: query heads of the attention that will read it (0: page calls only; the workspace that is
+    made serves any number of them). Buffers that are not given are allocated and set up as the empty cache (``reset``); with any
     of tables, n_kv and refs given, all three are the caller's and taken as they are."""
 
     def __init__(self, ctx: Context, *, n_layer: int, n_pages: int, page_tokens: int, n_kv_heads: int, head_dim: int,
@@ -122,7 +123,7 @@ class KvCache:
     def compact(self, tables_out: DeviceBuffer | None = None, refs_out: DeviceBuffer | None = None,
                 n_live: DeviceBuffer | None = None) -> None:
         """Moves the pages in use below every free one; tables and counts in place, or into
-        tables_out and refs_out."""
+        tables_out and refs_out (both)."""
         t, r = tables_out or self.tables, refs_out or self.refs
         t.require("compacted page table", 4 * self.max_seq * self.max_pages)
         r.require("compacted reference count", 4 * self.n_pages)
@@ -143,8 +144,8 @@ class KvCache:
                     sinks: DeviceBuffer | None = None) -> None:
         """Attention of one new token for n_seq batch rows (moearc_x_attn_decode_batch). Strides are in
         floats; seqs names the cache rows (default 0 .. n_seq - 1)."""
-        if not 0 < n_heads <= self.n_heads:
-            raise BadArgument(f"{n_heads} query heads: the cache's workspace was made for {self.n_heads}")
+        if n_heads < 1 or not self.n_heads:
+            raise BadArgument(f"{n_heads} query heads (a cache made without n_heads has no workspace for attention)")
         if n_seq < 0 or layer < 0:
             raise BadArgument("a negative count")
         row, kv_row = n_heads * self.head_dim, self.n_kv_heads * self.head_dim

@@ -41,7 +41,8 @@ def ctx():
 
 BAD = [dict(n_layer=0), dict(n_layer=129), dict(n_pages=0), dict(n_pages=(1 << 28) + 1), dict(page_tokens=0), dict(n_kv_heads=0),
        dict(head_dim=0), dict(head_dim=1025), dict(kv_type=2), dict(kv_type=39), dict(max_seq=0), dict(max_seq=65537),
-       dict(max_pages=0), dict(max_pages=(1 << 24) + 1), dict(max_pages=1 << 20, page_tokens=1 << 11), dict(work=0x10008)]
+       dict(max_pages=0), dict(max_pages=(1 << 24) + 1), dict(max_pages=1 << 20, page_tokens=1 << 11),
+       dict(page_tokens=1 << 20, max_pages=1, n_kv_heads=64, head_dim=32), dict(work=0x10008)]
 
 
 @pytest.mark.parametrize("kw", BAD)
@@ -73,6 +74,8 @@ def test_a_missing_pool_or_context_is_refused(lib, ctx):
     assert lib.moearc_x_kv_reset(ctx, None) == -1
     assert lib.moearc_x_kv_work_bytes(None, k.ref, 8) == 0
     assert lib.moearc_x_kv_compact(ctx, k.ref, None, 0x10000, None) == -1
+    assert lib.moearc_x_kv_compact(ctx, k.ref, 0x20000, 0x10000, None) == -2  # tables elsewhere, counts in place
+    assert lib.moearc_x_kv_compact(ctx, k.ref, 0x10000, 0x20000, None) == -2
 
 
 def test_row_lists_are_checked(lib, ctx):
@@ -113,7 +116,7 @@ def test_attention_arguments_are_checked(lib, ctx, kw, rc):
 @pytest.mark.parametrize("kw, rc", [
     (dict(logits=None), -1), (dict(tokens=None), -1), (dict(lp=None), -1), (dict(k=2, ids=None), -1), (dict(k=2, top=None), -1),
     (dict(ty=39), -2), (dict(stride=99), -2), (dict(vocab=0), -2), (dict(k=33), -2), (dict(k=5, vocab=4), -2), (dict(scale=0.0), -2),
-    (dict(scale=-1.0), -2), (dict(scale=float("nan")), -2), (dict(scale=float("inf")), -2), (dict(logits=0x10002), -2), (dict(rows=0), 0)])
+    (dict(scale=-1.0), -2), (dict(scale=1e-31), -2), (dict(scale=2e30), -2), (dict(scale=float("nan")), -2), (dict(scale=float("inf")), -2), (dict(logits=0x10002), -2), (dict(rows=0), 0)])
 def test_logprob_arguments_are_checked(lib, ctx, kw, rc):
     v = dict(logits=0x10000, ty=0, stride=100, rows=4, vocab=100, scale=1.0, tokens=0x10000, lp=0x10000, ent=0x10000, k=0, ids=0x10000, top=0x10000)
     v.update(kw)
