@@ -382,7 +382,7 @@ __global__ void __launch_bounds__(TH, sizeof(T) == 4 ? 4 : 5) k_logprobs(const l
         first.whole[rank] = r;
     }
     if (size > 1) {
-        if (threadIdx.x < a.k) first.top[rank][threadIdx.x] = sh.best[threadIdx.x];
+        if (threadIdx.x < MAX_K && a.k) first.top[rank][threadIdx.x] = sh.best[threadIdx.x];
         cluster.sync();
         if (rank != 0) return;
     } else {
@@ -405,13 +405,22 @@ __global__ void __launch_bounds__(TH, sizeof(T) == 4 ? 4 : 5) k_logprobs(const l
     }
     if (a.k) {
         if (size > 1) {
-            // every CTA's keys side by side (the unused end of a list is 0), then the best of them
-            for (unsigned i = threadIdx.x; i < size * a.k; i += TH) sh.list[i] = sh.top[i / a.k][i % a.k];
-            unsigned n = size * a.k;
-            if ((n & 1) && threadIdx.x == 0) sh.list[n] = 0;
-            n += n & 1;
-            __syncthreads();
-            rank_list(sh.list, n, a.k, sh.best);
+            // a key's rank: its place in its own list, and in each other list the keys above it
+            for (unsigned i = threadIdx.x; i < size * a.k; i += TH) {
+                const unsigned c = i / a.k, e = i - c * a.k;
+                const u64 key = sh.top[c][e];
+                unsigned place = e;
+                for (unsigned o = 0; o < size; ++o) {
+                    if (o == c) continue;
+                    unsigned n = 0;  // lists fall, their unused ends are 0
+#pragma unroll
+                    for (unsigned w = MAX_K / 2; w > 0; w >>= 1)
+                        if (sh.top[o][n + w - 1] > key) n += w;
+                    if (sh.top[o][n] > key) ++n;
+                    place += n;
+                }
+                if (key && place < a.k) sh.best[place] = key;
+            }
             __syncthreads();
         }
         if (threadIdx.x < a.k) {
