@@ -31,7 +31,12 @@ using namespace moearc;
 
 namespace {
 
-constexpr int TH = 256, WARPS = TH / 32, MAX_K = MAX_TOPK, LIST = 512;
+constexpr int MAX_K = MAX_TOPK, LIST = 512;
+// Threads a CTA: 128 where there are more rows than SMs hold such CTAs (about 8 an SM) and they are
+// short, so that what follows a row's pass is hidden by more rows; else 256, for a row's own speed.
+// 3000 rows of 8000 f32: 44 us with 256, 29 with 128; 600 of 32000 bf16: 17 and 24; 2047 of 100003
+// bf16: 83 and 91.
+constexpr size_t SHORT_ROW = 100 << 10;
 constexpr float LOG2E = 1.4426950408889634f;
 
 typedef unsigned long long u64;
@@ -188,7 +193,9 @@ struct run {
     __device__ unsigned tail() const { return body() + nv * vec<T>::N; }
 };
 
+template <int TH>
 struct shared_lists {
+    static constexpr int WARPS = TH / 32;
     triple part[WARPS];
     float warp_bound[WARPS];
     __align__(16) float max_v[TH];
@@ -204,6 +211,7 @@ struct shared_lists {
 
 // The largest k of list[0, n) in order into top, 0 past the last; rank by counting. n is even (a
 // 0 fills up an odd one).
+template <int TH>
 __device__ void rank_list(const u64 *list, unsigned n, unsigned k, u64 *top) {
     const auto *two = reinterpret_cast<const ulonglong2 *>(list);
     for (unsigned i = threadIdx.x; i < n; i += TH) {
@@ -220,9 +228,9 @@ __device__ void rank_list(const u64 *list, unsigned n, unsigned k, u64 *top) {
 
 // The largest min(k, elements) keys of the CTA's run, in order, into top, 0 past the last; m: the
 // thread's maximum, scaled.
-template <typename T>
-__device__ void top_of_run(const run<T> &R, float m, float scale, unsigned k, shared_lists &sh, u64 *top) {
-    constexpr int V = vec<T>::N;
+template <int TH, typename T>
+__device__ void top_of_run(const run<T> &R, float m, float scale, unsigned k, shared_lists<TH> &sh, u64 *top) {
+    constexpr int V = vec<T>::N, WARPS = TH / 32;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     // a first bound: each warp has ceil(k / WARPS) lanes at or above its own, so k threads of the
     // CTA are at or above the least of them (as ordered bits, for the warp's maximum in one step)
@@ -304,7 +312,7 @@ __device__ void top_of_run(const run<T> &R, float m, float scale, unsigned k, sh
         if ((n & 1) && threadIdx.x == 0) sh.list[n] = 0;
         n += n & 1;
         __syncthreads();
-        rank_list(sh.list, n, k, top);
+        rank_list<TH>(sh.list, n, k, top);
         __syncthreads();
         if (!over) return;
         least = top[k - 1];  // k listed elements reach it: the next bound, above the last
@@ -312,10 +320,10 @@ __device__ void top_of_run(const run<T> &R, float m, float scale, unsigned k, sh
     }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(TH, sizeof(T) == 4 ? 4 : 5) k_logprobs(const lp_args a) {
-    constexpr int V = vec<T>::N;
-    __shared__ shared_lists sh;
+template <int TH, typename T>
+__global__ void __launch_bounds__(TH, (sizeof(T) == 4 ? 4 : 5) * 256 / TH) k_logprobs(const lp_args a) {
+    constexpr int V = vec<T>::N, WARPS = TH / 32;
+    __shared__ shared_lists<TH> sh;
     cg::cluster_group cluster = cg::this_cluster();
     const unsigned size = cluster.num_blocks(), rank = cluster.block_rank();
     const unsigned row = blockIdx.x / size;
@@ -375,7 +383,7 @@ __global__ void __launch_bounds__(TH, sizeof(T) == 4 ? 4 : 5) k_logprobs(const l
     if (a.k) top_of_run(R, mine, scale, a.k, sh, size > 1 ? sh.best : sh.top[0]);
     else __syncthreads();
     if (size > 1) cluster.barrier_wait();
-    shared_lists &first = size > 1 ? *cluster.map_shared_rank(&sh, 0) : sh;
+    shared_lists<TH> &first = size > 1 ? *cluster.map_shared_rank(&sh, 0) : sh;
     if (threadIdx.x == 0) {
         r = sh.part[0];
         for (int w = 1; w < WARPS; ++w) r = join(r, sh.part[w]);
@@ -432,11 +440,11 @@ __global__ void __launch_bounds__(TH, sizeof(T) == 4 ? 4 : 5) k_logprobs(const l
     }
 }
 
-template <typename T>
-cudaError_t launch(moearc_ctx *c, const lp_args &a, unsigned n_rows) {
+template <int TH, typename T>
+cudaError_t launch_with(moearc_ctx *c, const lp_args &a, unsigned n_rows) {
     static std::atomic<bool> done[MOEARC_MAX_DEVICES];
     cudaError_t e = once_per_device(done, [] {
-        return cudaFuncSetAttribute(k_logprobs<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        return cudaFuncSetAttribute(k_logprobs<TH, T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     });
     if (e != cudaSuccess) return e;
     // CTAs for twice the SMs, but at least 16 vectors a thread of each; clusters of 16 only where they
@@ -456,7 +464,12 @@ cudaError_t launch(moearc_ctx *c, const lp_args &a, unsigned n_rows) {
     at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, k_logprobs<T>, a);
+    return cudaLaunchKernelEx(&cfg, k_logprobs<TH, T>, a);
+}
+
+template <typename T>
+cudaError_t launch(moearc_ctx *c, const lp_args &a, unsigned n_rows) {
+    return n_rows > (unsigned)c->sm_count * 8 && (size_t)a.n_vocab * sizeof(T) <= SHORT_ROW ? launch_with<128, T>(c, a, n_rows) : launch_with<256, T>(c, a, n_rows);
 }
 
 }  // namespace

@@ -91,7 +91,7 @@ def test_sizes_and_types(ctx, n, V, ty):
     check(ctx, x, ty)
 
 
-@pytest.mark.parametrize("n, V", [(1, 200003), (3, 131072), (40, 50001), (700, 3001)])
+@pytest.mark.parametrize("n, V", [(1, 200003), (3, 131072), (40, 50001), (700, 3001), (1500, 2003)])
 def test_every_cluster_size(ctx, n, V):
     x = np.random.default_rng(n).standard_normal((n, V)).astype(np.float32) * 2
     check(ctx, x, F32, k=20)
