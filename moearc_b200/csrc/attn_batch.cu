@@ -26,8 +26,8 @@
 //   an f16 cache as two f16 terms (22 bits) of values scaled by a power of two.
 //   A tile's P V is summed from zero and added to the f32 accumulator by an ordinary add: the
 //   tensor core's own accumulation truncates, which a long context would show.
-// - f32 caches, and head sizes without a tensor-core form, take a CUDA-core kernel on the same
-//   line of tiles.
+// - f32 caches multiply on the tensor cores as well, in two tf32 terms a side (22 bits); head sizes
+//   without a tensor-core form take CUDA cores, all on the same line of tiles.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -64,7 +64,7 @@ __device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], unsigned p) {
 
 template <int D_, bool BF>
 struct mma_tile {
-    static constexpr int KEYS = 16, GP = 8, ELEM = 2, D = D_, WARPS = D_ > 128 ? 4 : 8;
+    static constexpr int KEYS = 16, GP = 8, ELEM = 2, D = D_, WARPS = D_ > 128 ? 6 : 8;
     // Rows of a stage: chunk c of row r lies at c ^ (r & 7) where a row is whole 128-byte lines,
     // else rows are padded by one chunk to an odd number of them, so that the eight rows of an
     // ldmatrix meet eight different bank groups.
@@ -79,7 +79,8 @@ struct mma_tile {
     uint32_t qa[D / 16][4], ql[BF ? D / 16 : 1][2];
     float o[D / 8][2], c[CHAIN > 1 ? D / 8 : 1][4], m, l, sc;
     int chained;
-    static __host__ __device__ int row_bytes(int) { return ROW * 2; }
+    static __host__ __device__ int stage_bytes(int) { return 2 * KEYS * ROW * 2; }
+    static __host__ __device__ bool padded(int d) { return d < D; }  // channels past head_dim are zeros in a stage
     static __host__ __device__ int extra_bytes(int) { return 0; }
     // byte offset of chunk c of row r
     static __device__ __forceinline__ int at(int r, int c) { return r * ROW * 2 + (SWZ ? (c ^ (r & 7)) : c) * 16; }
@@ -94,6 +95,7 @@ struct mma_tile {
             const uint8_t *p = src + (size_t)rr * a.token_bytes + ch * 16;
             const size_t step = a.token_bytes * RW;
             const unsigned d0 = s0 + at(rr, ch);
+            if (ch < a.D / 8)
 #pragma unroll
             for (int i = 0; i < KEYS / RW; ++i, p += step) {
                 const unsigned d = (d0 ^ (SWZ ? (i * RW & 7) << 4 : 0)) + i * RW * ROW * 2;
@@ -104,6 +106,7 @@ struct mma_tile {
 #pragma unroll
             for (int i = 0; i < KEYS * CH / 32; ++i) {
                 const int c = lane + 32 * i, r = c / CH, ch = c % CH;
+                if (ch >= a.D / 8) continue;
                 const uint8_t *p = src + (size_t)r * a.token_bytes + ch * 16;
                 const unsigned d = s0 + at(r, ch);
                 cp_async16(d, p);
@@ -118,6 +121,7 @@ struct mma_tile {
         for (int i = 0; i < KEYS * CH / 32; ++i) {
             const int c = lane + 32 * i, r = c / CH, ch = c % CH;
             const long long b = __shfl_sync(0xffffffffu, off, r);
+            if (ch >= a.D / 8) continue;
             const size_t src = (b < 0 ? 0 : (size_t)b) + ch * 16;
             const unsigned d = s0 + at(r, ch);
             cp_async16z(d, a.k + src, b >= 0);
@@ -129,14 +133,15 @@ struct mma_tile {
     __device__ __forceinline__ void init(const float *q, int heads, const attn_args &a, uint8_t *, int lane) {
         const int hr = lane >> 2, qd = lane & 3;
         const bool live = hr < heads;
-        const float *p = q + (size_t)(live ? hr : 0) * D;
+        const float *p = q + (size_t)(live ? hr : 0) * a.D;
+        auto x = [&](int d) { return live && d < a.D ? p[d] : 0.f; };
         float f = 1.f;
         if constexpr (!BF) {
             float mx = 0.f;
 #pragma unroll
             for (int kk = 0; kk < D / 16; ++kk)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) mx = fmaxf(mx, fabsf(p[16 * kk + 2 * qd + (e & 1) + (e >> 1) * 8]));
+                for (int e = 0; e < 4; ++e) mx = fmaxf(mx, fabsf(x(16 * kk + 2 * qd + (e & 1) + (e >> 1) * 8)));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
             // the largest magnitude to [2^12, 2^13)
@@ -147,8 +152,8 @@ struct mma_tile {
         for (int kk = 0; kk < D / 16; ++kk) {
             const int c0 = 16 * kk + 2 * qd, c1 = c0 + 8;
             uint32_t t2 = 0, u2 = 0;
-            terms<BF>(live ? p[c0] * f : 0.f, live ? p[c0 + 1] * f : 0.f, qa[kk][0], qa[kk][1], t2);
-            terms<BF>(live ? p[c1] * f : 0.f, live ? p[c1 + 1] * f : 0.f, qa[kk][2], qa[kk][3], u2);
+            terms<BF>(x(c0) * f, x(c0 + 1) * f, qa[kk][0], qa[kk][1], t2);
+            terms<BF>(x(c1) * f, x(c1 + 1) * f, qa[kk][2], qa[kk][3], u2);
             if constexpr (BF) {
                 ql[kk][0] = t2;
                 ql[kk][1] = u2;
@@ -183,8 +188,8 @@ struct mma_tile {
     }
 
     // Row r of the stage (keys, then values) from f32, and into its slot where that is given.
-    static __device__ __forceinline__ void round_row(const float *x, uint8_t *stage, int r, uint8_t *slot, const attn_args &, int lane) {
-        for (int d = lane; d < D; d += 32) {
+    static __device__ __forceinline__ void round_row(const float *x, uint8_t *stage, int r, uint8_t *slot, const attn_args &a, int lane) {
+        for (int d = lane; d < a.D; d += 32) {
             const uint16_t b = to16<BF>(x[d]);
             *reinterpret_cast<uint16_t *>(stage + at(r, d >> 3) + (d & 7) * 2) = b;
             if (slot) reinterpret_cast<uint16_t *>(slot)[d] = b;
@@ -270,14 +275,212 @@ struct mma_tile {
     }
     // f(head, d, o, m, l) for every value this lane holds; one(head, m, l) once a head.
     template <typename F, typename G>
-    __device__ __forceinline__ void each(int lane, const attn_args &, F &&f, G &&one) {
+    __device__ __forceinline__ void each(int lane, const attn_args &a, F &&f, G &&one) {
         const int hr = lane >> 2, qd = lane & 3;
         one(hr, m, l, qd == 0);
 #pragma unroll
         for (int i = 0; i < D / 8; ++i) {
+            if (8 * i >= a.D) break;  // head_dim is a multiple of 8
             f(hr, 8 * i + 2 * qd, o[i][0]);
             f(hr, 8 * i + 2 * qd + 1, o[i][1]);
         }
+    }
+};
+
+// ---- the tensor-core tile of f32 caches ---------------------------------------------------------
+//
+// head_dim up to D_, a multiple of 4. mma.sync m16n8k8 on tf32 terms: a key or value is its leading 11
+// bits and the rest (two MMAs, 22 bits), q and the weights are two rounded terms on rows 0-7 and 8-15
+// of the A operand. Which channel (or key) stands for which k of an MMA is free as long as both
+// operands agree: k = j and j + 4 are channels 2 j and 2 j + 1 of an eight, read as one 8-byte load,
+// and keys 2 j and 2 j + 1, as the scores come out. Rows are 8 (keys) and 4 (values) words off a
+// multiple of 32, so that these reads meet 32 banks.
+
+__device__ __forceinline__ uint32_t tf32(float x) {
+    uint32_t u;
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(u) : "f"(x));
+    return u;
+}
+__device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// The leading 11 bits, and what is left of x without them (the MMA drops what tf32 does not hold).
+__device__ __forceinline__ void halves(float x, uint32_t &hi, uint32_t &lo) {
+    hi = __float_as_uint(x) & 0xffffe000u;
+    lo = __float_as_uint(x - __uint_as_float(hi));
+}
+
+template <int D_>
+struct tf32_tile {
+    static constexpr int KEYS = 16, GP = 8, ELEM = 4, D = D_, WARPS = D_ > 128 ? 4 : 8;
+    static constexpr int KROW = (D + 31) / 32 * 32 + 8, VROW = (D + 31) / 32 * 32 + 4;  // words
+    static constexpr bool QREG = D <= 128;  // q's terms in registers, else in shared memory
+
+    uint32_t qa[QREG ? D / 8 : 1][4];
+    float o[D / 8][2], m, l;
+    static __host__ __device__ int stage_bytes(int) { return KEYS * (KROW + VROW) * 4; }
+    static __host__ __device__ bool padded(int d) { return d < D; }
+    static __host__ __device__ int extra_bytes(int) { return QREG ? 0 : D / 8 * 512; }
+    static __device__ __forceinline__ int key_row(int r) { return r * KROW * 4; }
+    static __device__ __forceinline__ int value_row(int r) { return (KEYS * KROW + r * VROW) * 4; }
+
+    __device__ __forceinline__ void init(const float *q, int heads, const attn_args &a, uint8_t *extra, int lane) {
+        const int hr = lane >> 2, qd = lane & 3;
+        const bool live = hr < heads;
+        const float *p = q + (size_t)(live ? hr : 0) * a.D;
+        if constexpr (!QREG) __syncwarp();
+#pragma unroll 4
+        for (int kk = 0; kk < D / 8; ++kk) {
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int d = 8 * kk + 2 * qd + e;
+                const float x = live && d < a.D ? p[d] : 0.f;
+                w[2 * e] = tf32(x);
+                w[2 * e + 1] = tf32(x - __uint_as_float(w[2 * e]));
+            }
+            if constexpr (QREG) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) qa[kk][e] = w[e];
+            } else {
+                reinterpret_cast<uint4 *>(extra)[kk * 32 + lane] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+        }
+        if constexpr (!QREG) __syncwarp();
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = 0.f;
+        m = -INFINITY;
+        l = 0.f;
+    }
+    // copy(row, chunk) for every 16-byte chunk of the tile's rows
+    template <typename F>
+    static __device__ __forceinline__ void chunks(const attn_args &a, int lane, F &&copy) {
+        constexpr int CH = D / 4;
+        if (a.D == D) {
+#pragma unroll
+            for (int i = 0; i < KEYS * CH / 32; ++i) copy((lane + 32 * i) / CH, (lane + 32 * i) % CH, true);
+        } else {
+#pragma unroll 4
+            for (int i = 0; i < KEYS * CH / 32; ++i) copy((lane + 32 * i) / CH, (lane + 32 * i) % CH, (lane + 32 * i) % CH < a.D / 4);
+        }
+    }
+    static __device__ __forceinline__ void load_run(uint8_t *stage, const uint8_t *src, long long to_v, const attn_args &a, int lane) {
+        const unsigned s0 = smem_u32(stage);
+        chunks(a, lane, [&](int r, int ch, bool on) {
+            const uint8_t *p = src + (size_t)r * a.token_bytes + ch * 16;
+            if (on) {
+                cp_async16(s0 + key_row(r) + ch * 16, p);
+                cp_async16(s0 + value_row(r) + ch * 16, p + to_v);
+            }
+        });
+    }
+    static __device__ __forceinline__ void load_rows(uint8_t *stage, long long off, const attn_args &a, int lane) {
+        const unsigned s0 = smem_u32(stage);
+        chunks(a, lane, [&](int r, int ch, bool on) {
+            const long long b = __shfl_sync(0xffffffffu, off, r);
+            const size_t src = (b < 0 ? 0 : (size_t)b) + ch * 16;
+            if (on) {
+                cp_async16z(s0 + key_row(r) + ch * 16, a.k + src, b >= 0);
+                cp_async16z(s0 + value_row(r) + ch * 16, a.v + src, b >= 0);
+            }
+        });
+    }
+    static __device__ __forceinline__ void round_row(const float *x, uint8_t *stage, int r, uint8_t *slot, const attn_args &a, int lane) {
+        auto *row = reinterpret_cast<float *>(stage + (r < KEYS ? key_row(r) : value_row(r - KEYS)));
+        for (int d = lane; d < a.D; d += 32) {
+            row[d] = x[d];
+            if (slot) reinterpret_cast<float *>(slot)[d] = x[d];
+        }
+    }
+    __device__ __forceinline__ void step(const uint8_t *stage, unsigned live, const attn_args &a, uint8_t *extra, int lane) {
+        const int g = lane >> 2, qd = lane & 3;
+        float c0[2][4] = {}, c1[2][4] = {};
+        const float *ks = reinterpret_cast<const float *>(stage + key_row(g)) + 2 * qd;
+#pragma unroll
+        for (int kk = 0; kk < D / 8; ++kk) {
+            uint32_t w[4];
+            if constexpr (QREG) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] = qa[kk][e];
+            } else {
+                const uint4 u = reinterpret_cast<const uint4 *>(extra)[kk * 32 + lane];
+                w[0] = u.x;
+                w[1] = u.y;
+                w[2] = u.z;
+                w[3] = u.w;
+            }
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                const float2 k = *reinterpret_cast<const float2 *>(ks + n * 8 * KROW + 8 * kk);
+                uint32_t h0, h1, l0, l1;
+                halves(k.x, h0, l0);
+                halves(k.y, h1, l1);
+                mma_tf32(c0[n], w, h0, h1);
+                mma_tf32(c1[n], w, l0, l1);
+            }
+        }
+        // scores (in powers of two) of head lane / 4 for keys 2 qd, 2 qd + 1, 8 + 2 qd, 9 + 2 qd
+        float s[4];
+        const unsigned in = live >> (2 * qd);
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const float x = (c0[n][e] + (c0[n][e + 2] + (c1[n][e] + c1[n][e + 2]))) * a.scale2;
+                s[2 * n + e] = in >> (8 * n + e) & 1 ? x : -INFINITY;
+            }
+        float mt = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+        if (__any_sync(0xffffffffu, mt > m + LAZY)) {
+            mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
+            mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 2));
+            const float mn = fmaxf(m, mt), corr = ex2(m - (mn == -INFINITY ? 0.f : mn));
+            l *= corr;
+            m = mn;
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i) {
+                o[i][0] *= corr;
+                o[i][1] *= corr;
+            }
+        }
+        const float base = m == -INFINITY ? 0.f : m;
+        uint32_t pa[2][4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float p = ex2(s[e] - base);
+            l += p;
+            pa[e >> 1][2 * (e & 1)] = tf32(p);
+            pa[e >> 1][2 * (e & 1) + 1] = tf32(p - __uint_as_float(pa[e >> 1][2 * (e & 1)]));
+        }
+        const float *vs = reinterpret_cast<const float *>(stage + value_row(2 * qd)) + g;
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+            float c[4] = {}, d[4] = {};
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                uint32_t h0, h1, l0, l1;
+                halves(vs[n * 8 * VROW + 8 * i], h0, l0);
+                halves(vs[(n * 8 + 1) * VROW + 8 * i], h1, l1);
+                mma_tf32(c, pa[n], h0, h1);
+                mma_tf32(d, pa[n], l0, l1);
+            }
+            o[i][0] += c[0] + (c[2] + (d[0] + d[2]));
+            o[i][1] += c[1] + (c[3] + (d[1] + d[3]));
+        }
+    }
+    __device__ __forceinline__ void close(int) {
+        l += __shfl_xor_sync(0xffffffffu, l, 1);
+        l += __shfl_xor_sync(0xffffffffu, l, 2);
+    }
+    template <typename F, typename G>
+    __device__ __forceinline__ void each(int lane, const attn_args &a, F &&f, G &&one) {
+        const int hr = lane >> 2, qd = lane & 3;
+        one(hr, m, l, qd == 0);
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                if (8 * i + 2 * qd + e < a.D) f(hr, 8 * i + 2 * qd + e, o[i][e]);
     }
 };
 
@@ -324,6 +527,8 @@ struct core_tile {
     // A row in shared memory: an odd number of 16-byte chunks, so that eight keys meet eight bank
     // groups; its tail past head_dim is zero.
     static __host__ __device__ int row_bytes(int D) { return (((D * (int)sizeof(T) + 15) / 16) | 1) * 16; }
+    static __host__ __device__ int stage_bytes(int D) { return 2 * KEYS * row_bytes(D); }
+    static __host__ __device__ bool padded(int D) { return D * (int)sizeof(T) % 16 != 0; }
     static __host__ __device__ int dpad(int D) { return (D + 3) & ~3; }
     // per warp beside the stages: q, the tile's weights, the heads' corrections
     static __host__ __device__ int extra_bytes(int D) { return (GP * dpad(D) + 2 * KEYS * GP + GP) * 4; }
@@ -547,7 +752,7 @@ __global__ void __launch_bounds__(Tile::WARPS * 32, MINB)
     constexpr int KEYS = Tile::KEYS, GP = Tile::GP;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     const int D = a.D, HG = a.hg, R = a.rsplit, hs = warp % HG, r = warp / HG;
-    const int pitch = Tile::row_bytes(D), stage_bytes = 2 * KEYS * pitch;
+    const int stage_bytes = Tile::stage_bytes(D);
     const smem_layout S = layout_of((int)a.n_seq, warps, ns, stage_bytes, Tile::extra_bytes(D), GP, warps - HG, D);
     int *sums = reinterpret_cast<int *>(smem), *pre = sums + 32;
     uint8_t *ring = smem + S.ring + warp * ns * stage_bytes;
@@ -557,8 +762,8 @@ __global__ void __launch_bounds__(Tile::WARPS * 32, MINB)
     auto warp_heads = [&](int w) { return reinterpret_cast<float *>(smem + S.warp + w * S.warp_bytes + MAX_NS * 12); };
     float *hm = warp_heads(warp), *hl = hm + GP, *ff = hl + GP;
     uint8_t *extra = reinterpret_cast<uint8_t *>(ff + GP);
-    // core rows' tails past head_dim hold zeros
-    if (D * (int)Tile::ELEM % 16)
+    // rows' tails past head_dim hold zeros: no copy writes there
+    if (Tile::padded(D))
         for (int i = threadIdx.x * 16; i < warps * ns * stage_bytes; i += blockDim.x * 16)
             *reinterpret_cast<uint4 *>(smem + S.ring + i) = make_uint4(0, 0, 0, 0);
     pdl_trigger();
@@ -797,10 +1002,13 @@ struct attn_plan {
     int gp, keys, subs, hg, rsplit, nhg, warps, ns, smem, grid;
 };
 
-// f32 rows of up to 128 channels whose kv heads serve four query heads at most take half the
+// Which tile serves a shape (the pools' rows 16-byte aligned): tensor cores for 16-bit caches of a
+// multiple of 8 channels and for f32 ones of a multiple of 4, from the size at which half of the
+// smallest tile is used on; CUDA cores for the rest.
+bool tensor_dim(unsigned D, unsigned kv_type) { return D > 32 && D <= 256 && D % (kv_type == T_F32 ? 4 : 8) == 0; }
+// Of the latter, up to 128 channels whose kv heads serve four query heads at most take half the
 // arithmetic with tiles of four heads.
 bool few_heads(unsigned D, int group) { return D <= 128 && group <= 4; }
-bool mma_dim(unsigned D) { return D == 64 || D == 80 || D == 96 || D == 128 || D == 256; }
 
 template <class Tile>
 bool cut(attn_plan &p, int warps, int ns, int minb, int n_heads, int n_kv, int D, int n_seq, int sms) {
@@ -816,7 +1024,7 @@ bool cut(attn_plan &p, int warps, int ns, int minb, int n_heads, int n_kv, int D
     p.nhg = V / p.hg;
     p.warps = p.hg * p.rsplit;
     p.ns = ns;
-    p.smem = layout_of(n_seq, p.warps, ns, 2 * Tile::KEYS * Tile::row_bytes(D), Tile::extra_bytes(D), p.gp, p.warps - p.hg, D).total;
+    p.smem = layout_of(n_seq, p.warps, ns, Tile::stage_bytes(D), Tile::extra_bytes(D), p.gp, p.warps - p.hg, D).total;
     if (p.smem > MAX_SMEM - 512) return false;
     p.grid = sms * std::max(1, std::min(minb, 233472 / (p.smem + 1536)));
     return true;
@@ -835,9 +1043,15 @@ bool cut_any(attn_plan &p, int minb, int n_heads, int n_kv, int D, int n_seq, in
 template <typename F>
 auto with_tile(bool mma, unsigned kv_type, unsigned D, int group, F &&f) {
 #define MMA_CASE(d, mb)                                                                       \
-    if (D == d)                                                                               \
+    if (D <= d)                                                                               \
         return kv_type == T_BF16 ? f((mma_tile<d, true> *)nullptr, std::integral_constant<int, mb>()) \
                                  : f((mma_tile<d, false> *)nullptr, std::integral_constant<int, mb>());
+    if (mma && kv_type == T_F32) {
+        if (D <= 64) return f((tf32_tile<64> *)nullptr, std::integral_constant<int, 1>());
+        if (D <= 80) return f((tf32_tile<80> *)nullptr, std::integral_constant<int, 1>());
+        if (D <= 128) return f((tf32_tile<128> *)nullptr, std::integral_constant<int, 1>());
+        return f((tf32_tile<256> *)nullptr, std::integral_constant<int, 1>());
+    }
     if (mma) {
         MMA_CASE(64, 2)
         MMA_CASE(80, 1)
@@ -926,7 +1140,7 @@ int moearc_x_attn_decode_batch(moearc_ctx *c, const moearc_x_kv_cache *kv, unsig
         return ERR_ARG;
     }
     const uintptr_t align = reinterpret_cast<uintptr_t>(kv->k_pages[layer]) | reinterpret_cast<uintptr_t>(kv->v_pages[layer]);
-    const bool mma = kv->kv_type != T_F32 && mma_dim(kv->head_dim) && (align & 15) == 0;
+    const bool mma = tensor_dim(kv->head_dim, kv->kv_type) && (align & 15) == 0;
     attn_plan p;
     if (!plan_of(p, mma, kv->kv_type, (int)n_heads, (int)kv->n_kv_heads, (int)D, (int)n_seq, c->sm_count)) return ERR_ARG;
     const bool tc = mma && attn_tc_serves(*kv, layer);
