@@ -289,8 +289,8 @@ struct mma_tile {
 
 // ---- the tensor-core tile of f32 caches ---------------------------------------------------------
 //
-// head_dim up to D_, a multiple of 4. mma.sync m16n8k8 on tf32 terms: a key or value is its leading 11
-// bits and the rest (two MMAs, 22 bits), q and the weights are two rounded terms on rows 0-7 and 8-15
+// head_dim up to D_, a multiple of 4. mma.sync m16n8k8 on tf32 terms: a key or value is its rounding to
+// 11 bits and the rest (two MMAs, 23 bits), q and the weights are two rounded terms on rows 0-7 and 8-15
 // of the A operand. Which channel (or key) stands for which k of an MMA is free as long as both
 // operands agree: k = j and j + 4 are channels 2 j and 2 j + 1 of an eight, read as one 8-byte load,
 // and keys 2 j and 2 j + 1, as the scores come out. Rows are 8 (keys) and 4 (values) words off a
@@ -305,9 +305,9 @@ __device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], 
     asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// The leading 11 bits, and what is left of x without them (the MMA drops what tf32 does not hold).
+// x rounded to 11 bits, and what is left: 12 bits at most, of which the MMA drops the last.
 __device__ __forceinline__ void halves(float x, uint32_t &hi, uint32_t &lo) {
-    hi = __float_as_uint(x) & 0xffffe000u;
+    hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
     lo = __float_as_uint(x - __uint_as_float(hi));
 }
 
