@@ -20,14 +20,15 @@
 //   warps share a head, taking alternate tiles. A warp streams its K and V tiles through a ring of
 //   cp.async stages of its own, which runs on across rows: no barrier in the loop, and the next
 //   row's keys are on their way before this row is finished.
-// - 16-bit caches multiply on the tensor cores (mma.sync m16n8k16; the M = 128 of tcgen05 would be
-//   filled to a sixteenth by 8 heads, and the kernel is bound by memory either way). q and the
-//   softmax weights stay f32 in effect: a bf16 cache takes them as three bf16 terms (24 bits),
-//   an f16 cache as two f16 terms (22 bits) of values scaled by a power of two.
+// - 16-bit caches of up to 128 channels, a multiple of 8 above 32, have a kernel of their own on
+//   tcgen05 (attn_tc.cu). Here, on the same line of tiles: 16-bit caches of up to 256 channels and
+//   f32 ones of up to 256 on mma.sync (one warp's tile is 16 keys, and a tile of 128 keys of such
+//   rows would leave no room for a second), every other size on CUDA cores.
+// - q and the softmax weights stay f32 in effect: a bf16 cache takes them as three bf16 terms (24
+//   bits), an f16 cache as two f16 terms (22 bits) of values scaled by a power of two, an f32 cache
+//   everything as two tf32 terms (22 to 23 bits).
 //   A tile's P V is summed from zero and added to the f32 accumulator by an ordinary add: the
 //   tensor core's own accumulation truncates, which a long context would show.
-// - f32 caches multiply on the tensor cores as well, in two tf32 terms a side (22 bits); head sizes
-//   without a tensor-core form take CUDA cores, all on the same line of tiles.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -42,7 +43,7 @@ size_t kv_page_work_bytes(unsigned n_pages);
 
 namespace {
 
-// ---- the tensor-core tile (16-bit caches) -----------------------------------------------------
+// ---- the tensor-core tile of 16-bit caches: head_dim up to 256, a multiple of 8 -----------------
 
 template <bool BF>
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -62,70 +63,47 @@ __device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], unsigned p) {
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(p) : "memory");
 }
 
-template <int D_, bool BF>
+template <bool BF>
 struct mma_tile {
-    static constexpr int KEYS = 16, GP = 8, ELEM = 2, D = D_, WARPS = D_ > 128 ? 6 : 8;
-    // Rows of a stage: chunk c of row r lies at c ^ (r & 7) where a row is whole 128-byte lines,
-    // else rows are padded by one chunk to an odd number of them, so that the eight rows of an
-    // ldmatrix meet eight different bank groups.
-    static constexpr bool SWZ = D % 64 == 0;
-    static constexpr int CH = D / 8, ROW = SWZ ? D : D + 8;
+    static constexpr int KEYS = 16, GP = 8, D = 256, WARPS = 6;
+    // Rows of a stage are D channels, those past head_dim zeros: chunk c of row r lies at c ^ (r & 7),
+    // so that the eight rows of an ldmatrix meet eight different bank groups.
+    static constexpr int CH = D / 8, ROW = D * 2;
     // f16 weights are scaled away from subnormals (and stay below 65504 with the 2^8 of LAZY)
     static constexpr float PSCALE = BF ? 1.f : 64.f;
-    // Tiles whose P V the tensor core sums before they are added to o (its sums truncate: a few
-    // are within f32's rounding, a long row's are not). Above 128 channels registers allow one.
-    static constexpr int CHAIN = D <= 128 ? 8 : 1;
 
     uint32_t qa[D / 16][4], ql[BF ? D / 16 : 1][2];
-    float o[D / 8][2], c[CHAIN > 1 ? D / 8 : 1][4], m, l, sc;
-    int chained;
-    static __host__ __device__ int stage_bytes(int) { return 2 * KEYS * ROW * 2; }
-    static __host__ __device__ bool padded(int d) { return d < D; }  // channels past head_dim are zeros in a stage
+    float o[D / 8][2], m, l, sc;
+    static __host__ __device__ int stage_bytes(int) { return 2 * KEYS * ROW; }
+    static __host__ __device__ bool padded(int d) { return d < D; }
     static __host__ __device__ int extra_bytes(int) { return 0; }
     // byte offset of chunk c of row r
-    static __device__ __forceinline__ int at(int r, int c) { return r * ROW * 2 + (SWZ ? (c ^ (r & 7)) : c) * 16; }
+    static __device__ __forceinline__ int at(int r, int c) { return r * ROW + (c ^ (r & 7)) * 16; }
 
     // A whole tile of consecutive slots: `src` is the first key's row in the K pool, `to_v` the way
-    // from the K pool to the V pool.
+    // from the K pool to the V pool. A lane copies one chunk of every row.
     static __device__ __forceinline__ void load_run(uint8_t *stage, const uint8_t *src, long long to_v, const attn_args &a, int lane) {
-        const unsigned s0 = smem_u32(stage);
-        if constexpr (32 % CH == 0) {  // a lane keeps its chunk and takes every 32 / CH-th row
-            constexpr int RW = 32 / CH;
-            const int rr = lane / CH, ch = lane % CH;
-            const uint8_t *p = src + (size_t)rr * a.token_bytes + ch * 16;
-            const size_t step = a.token_bytes * RW;
-            const unsigned d0 = s0 + at(rr, ch);
-            if (ch < a.D / 8)
+        const uint8_t *p = src + lane * 16;
+        const unsigned d0 = smem_u32(stage) + lane * 16;
+        if (lane * 8 < a.D)
 #pragma unroll
-            for (int i = 0; i < KEYS / RW; ++i, p += step) {
-                const unsigned d = (d0 ^ (SWZ ? (i * RW & 7) << 4 : 0)) + i * RW * ROW * 2;
+            for (int r = 0; r < KEYS; ++r, p += a.token_bytes) {
+                const unsigned d = (d0 ^ ((r & 7) << 4)) + r * ROW;
                 cp_async16(d, p);
-                cp_async16(d + KEYS * ROW * 2, p + to_v);
+                cp_async16(d + KEYS * ROW, p + to_v);
             }
-        } else {
-#pragma unroll
-            for (int i = 0; i < KEYS * CH / 32; ++i) {
-                const int c = lane + 32 * i, r = c / CH, ch = c % CH;
-                if (ch >= a.D / 8) continue;
-                const uint8_t *p = src + (size_t)r * a.token_bytes + ch * 16;
-                const unsigned d = s0 + at(r, ch);
-                cp_async16(d, p);
-                cp_async16(d + KEYS * ROW * 2, p + to_v);
-            }
-        }
     }
     // Any tile: lane r holds the byte offset of key r's row in a pool, or -1 for zeros.
     static __device__ __forceinline__ void load_rows(uint8_t *stage, long long off, const attn_args &a, int lane) {
-        const unsigned s0 = smem_u32(stage);
+        const unsigned d0 = smem_u32(stage) + lane * 16;
 #pragma unroll 4
-        for (int i = 0; i < KEYS * CH / 32; ++i) {
-            const int c = lane + 32 * i, r = c / CH, ch = c % CH;
+        for (int r = 0; r < KEYS; ++r) {
             const long long b = __shfl_sync(0xffffffffu, off, r);
-            if (ch >= a.D / 8) continue;
-            const size_t src = (b < 0 ? 0 : (size_t)b) + ch * 16;
-            const unsigned d = s0 + at(r, ch);
+            if (lane * 8 >= a.D) continue;
+            const size_t src = (b < 0 ? 0 : (size_t)b) + lane * 16;
+            const unsigned d = (d0 ^ ((r & 7) << 4)) + r * ROW;
             cp_async16z(d, a.k + src, b >= 0);
-            cp_async16z(d + KEYS * ROW * 2, a.v + src, b >= 0);
+            cp_async16z(d + KEYS * ROW, a.v + src, b >= 0);
         }
     }
     // Rows 0-7 of the A operand hold the first term of the (up to 8) heads, rows 8-15 the second;
@@ -160,30 +138,15 @@ struct mma_tile {
             }
         }
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i) {
-            o[i][0] = o[i][1] = 0.f;
-            if constexpr (CHAIN > 1) c[i][0] = c[i][1] = c[i][2] = c[i][3] = 0.f;
-        }
+        for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = 0.f;
         m = -INFINITY;
         l = 0.f;
-        chained = 0;
     }
-    // o takes the chained sums, both scaled.
-    __device__ __forceinline__ void flush(float f) {
-        if constexpr (CHAIN > 1) {
+    __device__ __forceinline__ void scale_o(float f) {
 #pragma unroll
-            for (int i = 0; i < D / 8; ++i) {
-                o[i][0] = (o[i][0] + (c[i][0] + c[i][2])) * f;
-                o[i][1] = (o[i][1] + (c[i][1] + c[i][3])) * f;
-                c[i][0] = c[i][1] = c[i][2] = c[i][3] = 0.f;
-            }
-            chained = 0;
-        } else {
-#pragma unroll
-            for (int i = 0; i < D / 8; ++i) {
-                o[i][0] *= f;
-                o[i][1] *= f;
-            }
+        for (int i = 0; i < D / 8; ++i) {
+            o[i][0] *= f;
+            o[i][1] *= f;
         }
     }
 
@@ -201,12 +164,12 @@ struct mma_tile {
         // this lane's rows of the ldmatrix operands: keys (non-transposed) and values (transposed).
         // Stages start on whole rows, so chunk c + 2 i of a swizzled row is chunk c's address xor 32 i.
         const unsigned kb = smem_u32(stage) + at(((mi >> 1) << 3) | (lane & 7), mi & 1);
-        const unsigned vb = smem_u32(stage) + KEYS * ROW * 2 + at(((mi & 1) << 3) | (lane & 7), mi >> 1);
+        const unsigned vb = smem_u32(stage) + KEYS * ROW + at(((mi & 1) << 3) | (lane & 7), mi >> 1);
         float c0[2][4] = {}, c1[2][4] = {};
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
             uint32_t b[4];
-            ldsm4(b, SWZ ? kb ^ (kk * 32) : kb + kk * 32);
+            ldsm4(b, kb ^ (kk * 32));
             mma<BF>(c0[0], qa[kk][0], qa[kk][1], qa[kk][2], qa[kk][3], b[0], b[1]);
             mma<BF>(c0[1], qa[kk][0], qa[kk][1], qa[kk][2], qa[kk][3], b[2], b[3]);
             if constexpr (BF) {
@@ -225,18 +188,13 @@ struct mma_tile {
                 s[2 * n + e] = in >> (8 * n + e) & 1 ? x : -INFINITY;
             }
         float mt = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
-        const bool up = __any_sync(0xffffffffu, mt > m + LAZY);
-        if (up || (CHAIN > 1 && chained == CHAIN)) {
-            float corr = 1.f;
-            if (up) {
-                mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
-                mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 2));
-                const float mn = fmaxf(m, mt);
-                corr = ex2(m - (mn == -INFINITY ? 0.f : mn));
-                l *= corr;
-                m = mn;
-            }
-            flush(corr);
+        if (__any_sync(0xffffffffu, mt > m + LAZY)) {
+            mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
+            mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 2));
+            const float mn = fmaxf(m, mt), corr = ex2(m - (mn == -INFINITY ? 0.f : mn));
+            l *= corr;
+            m = mn;
+            scale_o(corr);
         }
         const float base = m == -INFINITY ? 0.f : m;
         float p[4];
@@ -249,29 +207,23 @@ struct mma_tile {
 #pragma unroll
         for (int dn = 0; dn < D / 16; ++dn) {
             uint32_t b[4];
-            ldsm4t(b, SWZ ? vb ^ (dn * 32) : vb + dn * 32);
+            ldsm4t(b, vb ^ (dn * 32));
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                if constexpr (CHAIN > 1) {
-                    if constexpr (BF) mma<BF>(c[2 * dn + h], b0, 0u, b2, 0u, b[2 * h], b[2 * h + 1]);
-                    mma<BF>(c[2 * dn + h], a0, a1, a2, a3, b[2 * h], b[2 * h + 1]);
-                } else {
-                    float t[4] = {};
-                    if constexpr (BF) mma<BF>(t, b0, 0u, b2, 0u, b[2 * h], b[2 * h + 1]);
-                    mma<BF>(t, a0, a1, a2, a3, b[2 * h], b[2 * h + 1]);
-                    o[2 * dn + h][0] += t[0] + t[2];
-                    o[2 * dn + h][1] += t[1] + t[3];
-                }
+                float t[4] = {};
+                if constexpr (BF) mma<BF>(t, b0, 0u, b2, 0u, b[2 * h], b[2 * h + 1]);
+                mma<BF>(t, a0, a1, a2, a3, b[2 * h], b[2 * h + 1]);
+                o[2 * dn + h][0] += t[0] + t[2];
+                o[2 * dn + h][1] += t[1] + t[3];
             }
         }
-        ++chained;
     }
 
     // After the last tile: l summed over the head's lanes, o without its scale.
     __device__ __forceinline__ void close(int) {
         l += __shfl_xor_sync(0xffffffffu, l, 1);
         l += __shfl_xor_sync(0xffffffffu, l, 2);
-        flush(1.f / PSCALE);
+        scale_o(1.f / PSCALE);
     }
     // f(head, d, o, m, l) for every value this lane holds; one(head, m, l) once a head.
     template <typename F, typename G>
@@ -313,7 +265,7 @@ __device__ __forceinline__ void halves(float x, uint32_t &hi, uint32_t &lo) {
 
 template <int D_>
 struct tf32_tile {
-    static constexpr int KEYS = 16, GP = 8, ELEM = 4, D = D_, WARPS = D_ > 128 ? 4 : 8;
+    static constexpr int KEYS = 16, GP = 8, D = D_, WARPS = D_ > 128 ? 4 : 8;
     static constexpr int KROW = (D + 31) / 32 * 32 + 8, VROW = (D + 31) / 32 * 32 + 4;  // words
     static constexpr bool QREG = D <= 128;  // q's terms in registers, else in shared memory
 
@@ -520,7 +472,7 @@ __device__ __forceinline__ void round_to(float v, __nv_bfloat16 &d) { d = __floa
 
 template <typename T, int NQ, int GP_>
 struct core_tile {
-    static constexpr int KEYS = 8, GP = GP_, ELEM = sizeof(T), WARPS = NQ == 1 ? 16 : 8;
+    static constexpr int KEYS = 8, GP = GP_, WARPS = NQ == 1 ? 16 : 8;
     float2 acc[NQ][GP][2];
     float m[GP / 4], l[GP / 4];
 
@@ -745,8 +697,8 @@ __host__ __device__ inline smem_layout layout_of(int n_seq, int warps, int ns, i
     return s;
 }
 
-template <class Tile, int MINB>
-__global__ void __launch_bounds__(Tile::WARPS * 32, MINB)
+template <class Tile>
+__global__ void __launch_bounds__(Tile::WARPS * 32, 1)
     k_attn_batch(const __grid_constant__ attn_args a, int ns) {
     extern __shared__ __align__(1024) uint8_t smem[];
     constexpr int KEYS = Tile::KEYS, GP = Tile::GP;
@@ -998,20 +950,19 @@ cudaError_t with_list(const unsigned *rows, unsigned n, F &&f) {
 
 // How a shape is cut: virtual heads and warps per CTA, stages, shared memory and the grid.
 struct attn_plan {
-    bool mma;
     int gp, keys, subs, hg, rsplit, nhg, warps, ns, smem, grid;
 };
 
-// Which tile serves a shape (the pools' rows 16-byte aligned): tensor cores for 16-bit caches of a
-// multiple of 8 channels and for f32 ones of a multiple of 4, from the size at which half of the
-// smallest tile is used on; CUDA cores for the rest.
+// Whether the tensor cores serve a shape, where the pools' rows are 16-byte aligned: multiples of 8
+// channels of 16 bits and of 4 channels of f32, from the size at which half of the smallest tile is
+// used on. CUDA cores have the rest.
 bool tensor_dim(unsigned D, unsigned kv_type) { return D > 32 && D <= 256 && D % (kv_type == T_F32 ? 4 : 8) == 0; }
 // Of the latter, up to 128 channels whose kv heads serve four query heads at most take half the
 // arithmetic with tiles of four heads.
 bool few_heads(unsigned D, int group) { return D <= 128 && group <= 4; }
 
 template <class Tile>
-bool cut(attn_plan &p, int warps, int ns, int minb, int n_heads, int n_kv, int D, int n_seq, int sms) {
+bool cut(attn_plan &p, int warps, int ns, int n_heads, int n_kv, int D, int n_seq, int sms) {
     p.gp = Tile::GP;
     p.keys = Tile::KEYS;
     const int group = n_heads / n_kv;
@@ -1026,46 +977,37 @@ bool cut(attn_plan &p, int warps, int ns, int minb, int n_heads, int n_kv, int D
     p.ns = ns;
     p.smem = layout_of(n_seq, p.warps, ns, Tile::stage_bytes(D), Tile::extra_bytes(D), p.gp, p.warps - p.hg, D).total;
     if (p.smem > MAX_SMEM - 512) return false;
-    p.grid = sms * std::max(1, std::min(minb, 233472 / (p.smem + 1536)));
+    p.grid = sms;
     return true;
 }
 
 // Three stages where the tile's warps have them, else two, else fewer warps.
 template <class Tile>
-bool cut_any(attn_plan &p, int minb, int n_heads, int n_kv, int D, int n_seq, int sms) {
+bool cut_any(attn_plan &p, int n_heads, int n_kv, int D, int n_seq, int sms) {
     for (int warps = Tile::WARPS; warps >= 1; warps /= 2)
         for (int ns = 3; ns >= 2; --ns)
-            if (cut<Tile>(p, warps, ns, minb, n_heads, n_kv, D, n_seq, sms)) return true;
+            if (cut<Tile>(p, warps, ns, n_heads, n_kv, D, n_seq, sms)) return true;
     return false;
 }
 
-// f(Tile, MINB) for the tile that serves a shape.
+// f(a null pointer to the tile) for the tile that serves a shape.
 template <typename F>
 auto with_tile(bool mma, unsigned kv_type, unsigned D, int group, F &&f) {
-#define MMA_CASE(d, mb)                                                                       \
-    if (D <= d)                                                                               \
-        return kv_type == T_BF16 ? f((mma_tile<d, true> *)nullptr, std::integral_constant<int, mb>()) \
-                                 : f((mma_tile<d, false> *)nullptr, std::integral_constant<int, mb>());
     if (mma && kv_type == T_F32) {
-        if (D <= 64) return f((tf32_tile<64> *)nullptr, std::integral_constant<int, 1>());
-        if (D <= 80) return f((tf32_tile<80> *)nullptr, std::integral_constant<int, 1>());
-        if (D <= 128) return f((tf32_tile<128> *)nullptr, std::integral_constant<int, 1>());
-        return f((tf32_tile<256> *)nullptr, std::integral_constant<int, 1>());
+        if (D <= 64) return f((tf32_tile<64> *)nullptr);
+        if (D <= 80) return f((tf32_tile<80> *)nullptr);
+        if (D <= 128) return f((tf32_tile<128> *)nullptr);
+        return f((tf32_tile<256> *)nullptr);
     }
-    if (mma) {
-        MMA_CASE(64, 2)
-        MMA_CASE(80, 1)
-        MMA_CASE(96, 1)
-        MMA_CASE(128, 1)
-        MMA_CASE(256, 1)
-    }
-#undef MMA_CASE
+    if (mma)  // above 128 channels: attn_tc.cu has those below
+        return kv_type == T_BF16 ? f((mma_tile<true> *)nullptr)
+                                 : f((mma_tile<false> *)nullptr);
 #define CORE_CASE(T)                                                                                  \
-    if (few_heads(D, group)) return f((core_tile<T, 1, 4> *)nullptr, std::integral_constant<int, 1>()); \
-    if (D <= 128) return f((core_tile<T, 1, 8> *)nullptr, std::integral_constant<int, 1>());          \
-    if (D <= 256) return f((core_tile<T, 2, 8> *)nullptr, std::integral_constant<int, 1>());          \
-    if (D <= 512) return f((core_tile<T, 4, 4> *)nullptr, std::integral_constant<int, 1>());          \
-    return f((core_tile<T, 8, 4> *)nullptr, std::integral_constant<int, 1>());
+    if (few_heads(D, group)) return f((core_tile<T, 1, 4> *)nullptr); \
+    if (D <= 128) return f((core_tile<T, 1, 8> *)nullptr);          \
+    if (D <= 256) return f((core_tile<T, 2, 8> *)nullptr);          \
+    if (D <= 512) return f((core_tile<T, 4, 4> *)nullptr);          \
+    return f((core_tile<T, 8, 4> *)nullptr);
     if (kv_type == T_F32) {
         CORE_CASE(float)
     } else if (kv_type == T_F16) {
@@ -1076,28 +1018,27 @@ auto with_tile(bool mma, unsigned kv_type, unsigned D, int group, F &&f) {
 }
 
 bool plan_of(attn_plan &p, bool mma, unsigned kv_type, int n_heads, int n_kv, int D, int n_seq, int sms) {
-    p.mma = mma;
-    return with_tile(mma, kv_type, (unsigned)D, n_heads / n_kv, [&](auto *t, auto minb) {
+    return with_tile(mma, kv_type, (unsigned)D, n_heads / n_kv, [&](auto *t) {
         using Tile = std::remove_pointer_t<decltype(t)>;
-        return cut_any<Tile>(p, minb(), n_heads, n_kv, D, n_seq, sms);
+        return cut_any<Tile>(p, n_heads, n_kv, D, n_seq, sms);
     });
 }
 
 // The work buffer: the rows' list, a note a CTA, then the parts.
 size_t attn_bytes(int grid, int hg, int gp, int D) { return KV_LIST * 4 + (size_t)grid * 16 + (size_t)grid * 2 * hg * gp * (D + 2) * 4; }
 size_t attn_bytes(const attn_plan &p, int D) { return attn_bytes(p.grid, p.hg, p.gp, D); }
-// Most query heads that the CTAs of an SM work on at once, CTAs x hg x gp: 2 x 8 x 8 (tensor-core tiles
-// of 64 channels) or 1 x 16 x 8 (CUDA cores) up to 128 channels, 8 warps of 8 or of 4 heads above.
+// Most query heads that an SM's CTA works on at once, hg x gp: 16 x 8 (CUDA cores) up to 128 channels,
+// 8 warps of 8 or of 4 heads above; attn_tc.cu's two CTAs of one head group are fewer.
 int heads_of_sm(unsigned D) { return D <= 128 ? 128 : D <= 256 ? 64 : 32; }
 
-template <class Tile, int MINB>
+template <class Tile>
 cudaError_t launch(moearc_ctx *c, const attn_plan &p, const attn_args &a) {
     static std::atomic<bool> done[MOEARC_MAX_DEVICES];
     cudaError_t e = once_per_device(done, [] {
-        return set_smem(k_attn_batch<Tile, MINB>, MAX_SMEM - 512);
+        return set_smem(k_attn_batch<Tile>, MAX_SMEM - 512);
     });
     if (e == cudaSuccess)
-        e = launch_pdl(k_attn_batch<Tile, MINB>, dim3((unsigned)p.grid), dim3((unsigned)p.warps * 32), (size_t)p.smem, c->stream, a, p.ns);
+        e = launch_pdl(k_attn_batch<Tile>, dim3((unsigned)p.grid), dim3((unsigned)p.warps * 32), (size_t)p.smem, c->stream, a, p.ns);
     if (e == cudaSuccess) e = attn_join_launch<Tile::GP>(c, p.grid, a);
     return e;
 }
@@ -1143,7 +1084,9 @@ int moearc_x_attn_decode_batch(moearc_ctx *c, const moearc_x_kv_cache *kv, unsig
     const bool mma = tensor_dim(kv->head_dim, kv->kv_type) && (align & 15) == 0;
     attn_plan p;
     if (!plan_of(p, mma, kv->kv_type, (int)n_heads, (int)kv->n_kv_heads, (int)D, (int)n_seq, c->sm_count)) return ERR_ARG;
-    const bool tc = mma && attn_tc_serves(*kv, layer);
+    const bool tc = mma && kv->kv_type != T_F32 && D <= 128;
+    // tokens are numbered in 32 bits there; more of them than that would not fit the memory
+    if (tc && (unsigned long long)kv->n_pages * kv->page_tokens >= (1ull << 31)) return ERR_ARG;
     const int tc_grid = attn_tc_grid(kv->head_dim, c->sm_count);
     if (kv->work_bytes < (tc ? attn_bytes(tc_grid, 1, 8, (int)D) : attn_bytes(p, (int)D))) return ERR_ARG;
     const unsigned cap = kv->max_pages * kv->page_tokens;
@@ -1195,8 +1138,8 @@ int moearc_x_attn_decode_batch(moearc_ctx *c, const moearc_x_kv_cache *kv, unsig
             constexpr int N = (int)(sizeof(L.row) / sizeof(unsigned));
             return launch_pdl(k_attn_rows<N>, dim3(1), dim3(KV_LIST), 0, c->stream, L, n_seq, static_cast<unsigned *>(kv->work));
         });
-    if (e == cudaSuccess) e = tc ? attn_tc_launch(c, *kv, a) : with_tile(mma, kv->kv_type, kv->head_dim, a.group, [&](auto *t, auto minb) {
-        return launch<std::remove_pointer_t<decltype(t)>, decltype(minb)::value>(c, p, a);
+    if (e == cudaSuccess) e = tc ? attn_tc_launch(c, *kv, a) : with_tile(mma, kv->kv_type, kv->head_dim, a.group, [&](auto *t) {
+        return launch<std::remove_pointer_t<decltype(t)>>(c, p, a);
     });
     if (e != cudaSuccess) cudaGetLastError();  // the failed launch's error, not left for an unrelated later check
     const int rc2 = ls.finish();

@@ -249,8 +249,8 @@ static cudaError_t attn_join_launch(moearc_ctx *c, int grid, const attn_args &a)
                       dim3(JOIN_THREADS), (size_t)GP * grid * 4, c->stream, a);
 }
 
-// The tcgen05 kernel (attn_tc.cu): whether it serves a shape, its grid, and its launch.
-bool attn_tc_serves(const moearc_x_kv_cache &kv, unsigned layer);
+// The tcgen05 kernel (attn_tc.cu), for 16-bit caches of head_dim 40 to 128, a multiple of 8, with fewer
+// than 2^31 tokens: its grid, and its launch.
 int attn_tc_grid(unsigned head_dim, int sms);
 cudaError_t attn_tc_launch(moearc_ctx *c, const moearc_x_kv_cache &kv, attn_args a);
 

@@ -1,6 +1,6 @@
 // attn_tc.cu — decode attention of a ragged batch over the paged cache on the fifth-generation
-// tensor cores: 16-bit caches of head_dim 64 or 128 (attn_batch.cu serves the rest; the formula, the
-// equal runs and the join are the same).
+// tensor cores: 16-bit caches of up to 128 channels, a multiple of 8 above 32 (attn_batch.cu serves
+// the rest; the formula, the equal runs and the join are the same).
 //
 // A unit is a batch row and a kv head (with up to eight of its query heads); its keys are cut into
 // tiles of 128, and each CTA takes an equal run of all units' tiles. Per tile:
@@ -15,8 +15,8 @@
 //
 // Two tiles are in flight or in use. They are loaded by 16-byte asynchronous copies, two warps a
 // stage: any page size, and as many bytes under way as the stages hold. (TMA boxes of 128-byte rows
-// brought 3.5 TB/s where these bring 5.5, one head of a token being 128 or 256 bytes in a row of
-// thousands.) Roles, each a warp or more that meet at mbarriers: loads; MMA issue; four warps of
+// brought 3.5 TB/s and untiled bulk copies of a row 4, where these bring 6.2: one head of a token is
+// 128 or 256 bytes in a row of thousands.) Roles, each a warp or more that meet at mbarriers: loads; MMA issue; four warps of
 // softmax; two warps that split the next unit's queries into terms ahead of its first tile. Keys are
 // given back for loading as soon as S is computed, values once O is. Every wait has a limit
 // (tc.cuh): one that runs out raises MOEARC_X_KV_WAIT and ends the kernel.
@@ -120,11 +120,13 @@ __device__ __forceinline__ bool soft_any(bool x) {
     return r != 0;
 }
 
-template <int D, bool BF>
-__global__ void __launch_bounds__(THREADS, D == 64 ? 2 : 1)
+// DP: the channels that tiles have room for, 64 or 128; head_dim is that (FULL) or less.
+template <int DP, bool FULL, bool BF>
+__global__ void __launch_bounds__(THREADS, DP == 64 ? 2 : 1)
     k_attn_tc(const __grid_constant__ attn_args a) {
-    using S = tc_smem<D>;
-    constexpr int CH = D / 8, TERMS = BF ? 3 : 2;
+    using S = tc_smem<DP>;
+    const int D = FULL ? DP : a.D;
+    constexpr int CH = DP / 8, TERMS = BF ? 3 : 2;
     constexpr float PSCALE = BF ? 1.f : 64.f;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = smem_raw + (((tc::sa(smem_raw) + 1023u) & ~1023u) - tc::sa(smem_raw));
@@ -143,6 +145,10 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 2 : 1)
     int *status = reinterpret_cast<int *>(a.status);
     constexpr int WAIT = (int)MOEARC_X_KV_WAIT;
 
+    // channels past head_dim are zeros in the keys and in q, and never written again
+    if (D < DP)
+        for (int i = threadIdx.x * 16; i < S::at_p; i += THREADS * 16) *reinterpret_cast<uint4 *>(smem + i) = make_uint4(0, 0, 0, 0);
+    fence_async();
     if (warp == 4) tc::tmem_alloc(tslot, 128);
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
@@ -253,6 +259,7 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 2 : 1)
             };
             if (st < n_tiles) look_up(g0 + st);
             const int ch = t % CH, r0 = t / CH;
+            const bool used = ch * 8 < D;
             uint8_t *stage = smem + st * S::STAGE;
             const unsigned d0 = smem_u32(stage) + (ch >> 3) * KEYS * 128;
             constexpr int RW = LOADERS / CH, BATCH = 8;  // rows a step; steps whose rows are looked at together
@@ -265,7 +272,7 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 2 : 1)
 #pragma unroll
                     for (int e = 0; e < BATCH; ++e) {
                         const int q = r + e * RW;
-                        cp_async16p(dst + q * 128 + (((ch & 7) ^ (q & 7)) << 4), pool + (size_t)(unsigned)max(at[e], 0) * a.token_bytes, at[e] >= 0, at[e] > -2);
+                        cp_async16p(dst + q * 128 + (((ch & 7) ^ (q & 7)) << 4), pool + (size_t)(unsigned)max(at[e], 0) * a.token_bytes, at[e] >= 0, used && at[e] > -2);
                     }
                 }
                 cp_commit();
@@ -310,16 +317,17 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 2 : 1)
                     meta[st].vh = vh_i;
                 }
                 copy(a.v + head + ch * 16, d0 + S::MAT);
-                float kn[D / 64], vn[D / 64];
+                float kn[DP / 64], vn[DP / 64];
                 uint8_t *slot_k = nullptr, *slot_v = nullptr;
                 const bool fresh = at_new >= 0 && tok[at_new] < -1;
                 if (fresh) {
                     const size_t src = (size_t)row_i * a.new_stride + (size_t)kvh * D + t, dst = (size_t)(-2 - tok[at_new]) * a.token_bytes + head;
 #pragma unroll
-                    for (int e = 0; e < D / 64; ++e) {
-                        kn[e] = a.k_new[src + e * 64];
-                        vn[e] = a.v_new[src + e * 64];
-                    }
+                    for (int e = 0; e < DP / 64; ++e)
+                        if (t + e * 64 < D) {
+                            kn[e] = a.k_new[src + e * 64];
+                            vn[e] = a.v_new[src + e * 64];
+                        }
                     if (stores) {
                         slot_k = a.k + dst;
                         slot_v = a.v + dst;
@@ -329,13 +337,15 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 2 : 1)
                 cp_wait<1>();
                 if (fresh)
 #pragma unroll
-                    for (int e = 0; e < D / 64; ++e) put(0, at_new, t + e * 64, kn[e], slot_k);
+                    for (int e = 0; e < DP / 64; ++e)
+                        if (t + e * 64 < D) put(0, at_new, t + e * 64, kn[e], slot_k);
                 fence_async();  // what the copies wrote, before the tensor core reads it
                 tc::bar_arrive(kfull + st);
                 cp_wait<0>();
                 if (fresh)
 #pragma unroll
-                    for (int e = 0; e < D / 64; ++e) put(1, at_new, t + e * 64, vn[e], slot_v);
+                    for (int e = 0; e < DP / 64; ++e)
+                        if (t + e * 64 < D) put(1, at_new, t + e * 64, vn[e], slot_v);
                 fence_async();
                 tc::bar_arrive(vfull + st);
                 if (!__all_sync(0xffffffffu, ok)) break;
@@ -359,8 +369,9 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 2 : 1)
                 tc::fence_after_sync();
                 if (lane == 0) {
 #pragma unroll
-                    for (int kk = 0; kk < D / 16; ++kk)
-                        tc::mma_bf16(tmem + (i & 1) * 32, tc::desc_k_sw128(base + st * S::STAGE + (kk >> 2) * KEYS * 128 + (kk & 3) * 32),
+                    for (int kk = 0; kk < DP / 16; ++kk)
+                        if (16 * kk < D)
+                            tc::mma_bf16(tmem + (i & 1) * 32, tc::desc_k_sw128(base + st * S::STAGE + (kk >> 2) * KEYS * 128 + (kk & 3) * 32),
                                      tc::desc_k_sw128(base + S::at_q + (u & 1) * S::Q + (kk >> 2) * NT * 128 + (kk & 3) * 32), kind, kk > 0);
                     tc::mma_commit(sfull + (i & 1));
                     if (flags & LAST) tc::mma_commit(qempty + (u & 1));
@@ -385,7 +396,7 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 2 : 1)
                     const uint32_t v = base + st * S::STAGE + S::MAT, p = base + S::at_p + st * S::P;
 #pragma unroll
                     for (int kk = 0; kk < KEYS / 16; ++kk)
-                        tc::mma_bf16(tmem + 64 + st * 32, desc_v(v + kk * 2048, D == 128 ? KEYS * 128 : 0), desc_p(p + kk * 1024), kind, kk > 0);
+                        tc::mma_bf16(tmem + 64 + st * 32, desc_v(v + kk * 2048, DP == 128 ? KEYS * 128 : 0), desc_p(p + kk * 1024), kind, kk > 0);
                     tc::mma_commit(ofull + st);
                     tc::mma_commit(empty + st);
                 }
@@ -411,7 +422,7 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 2 : 1)
                     const int h = c / CH, ch = c % CH;
                     float x[8];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) x[e] = h < heads ? q[(size_t)h * D + ch * 8 + e] : 0.f;
+                    for (int e = 0; e < 8; ++e) x[e] = h < heads && ch * 8 < D ? q[(size_t)h * D + ch * 8 + e] : 0.f;
                     float f = 1.f;
                     if constexpr (!BF) {  // the head's largest magnitude to [2^12, 2^13)
                         float mx = 0.f;
@@ -575,35 +586,33 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 2 : 1)
     if (warp == 4) tc::tmem_dealloc(tmem, 128);
 }
 
-template <int D, bool BF>
-cudaError_t launch(moearc_ctx *c, attn_args &a) {
+template <int DP, bool FULL, bool BF>
+cudaError_t launch_tile(moearc_ctx *c, attn_args &a) {
     static std::atomic<bool> done[MOEARC_MAX_DEVICES];
-    const cudaError_t e = once_per_device(done, [] { return set_smem(k_attn_tc<D, BF>, tc_smem<D>::total((int)KV_LIST)); });
+    const cudaError_t e = once_per_device(done, [] { return set_smem(k_attn_tc<DP, FULL, BF>, tc_smem<DP>::total((int)KV_LIST)); });
     if (e != cudaSuccess) return e;
-    const int grid = attn_tc_grid(D, c->sm_count);
+    const int grid = attn_tc_grid(DP, c->sm_count);
     const cudaError_t e2 =
-        launch_pdl(k_attn_tc<D, BF>, dim3((unsigned)grid), dim3(THREADS), (size_t)tc_smem<D>::total((int)a.n_seq), c->stream, a);
+        launch_pdl(k_attn_tc<DP, FULL, BF>, dim3((unsigned)grid), dim3(THREADS), (size_t)tc_smem<DP>::total((int)a.n_seq), c->stream, a);
     return e2 != cudaSuccess ? e2 : attn_join_launch<GP>(c, grid, a);
+}
+template <bool BF>
+cudaError_t launch(moearc_ctx *c, attn_args &a) {
+    if (a.D <= 64) return a.D == 64 ? launch_tile<64, true, BF>(c, a) : launch_tile<64, false, BF>(c, a);
+    return a.D == 128 ? launch_tile<128, true, BF>(c, a) : launch_tile<128, false, BF>(c, a);
 }
 
 }  // namespace
 
 namespace moearc {
 
-int attn_tc_grid(unsigned head_dim, int sms) { return head_dim == 64 ? 2 * sms : sms; }
-
-bool attn_tc_serves(const moearc_x_kv_cache &kv, unsigned layer) {
-    const uintptr_t align = reinterpret_cast<uintptr_t>(kv.k_pages[layer]) | reinterpret_cast<uintptr_t>(kv.v_pages[layer]);
-    return kv.kv_type != T_F32 && (kv.head_dim == 64 || kv.head_dim == 128) && (align & 15) == 0 &&
-           (unsigned long long)kv.n_pages * kv.page_tokens < (1ull << 31);  // tokens are numbered in 32 bits
-}
+int attn_tc_grid(unsigned head_dim, int sms) { return head_dim <= 64 ? 2 * sms : sms; }
 
 cudaError_t attn_tc_launch(moearc_ctx *c, const moearc_x_kv_cache &kv, attn_args a) {
     a.subs = (a.group + GP - 1) / GP;
     a.hg = 1;
     a.nhg = (int)kv.n_kv_heads * a.subs;
-    if (kv.head_dim == 64) return kv.kv_type == T_BF16 ? launch<64, true>(c, a) : launch<64, false>(c, a);
-    return kv.kv_type == T_BF16 ? launch<128, true>(c, a) : launch<128, false>(c, a);
+    return kv.kv_type == T_BF16 ? launch<true>(c, a) : launch<false>(c, a);
 }
 
 }  // namespace moearc

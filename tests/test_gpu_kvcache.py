@@ -301,6 +301,16 @@ def test_attention_of_one_long_row(ctx):
     batch(ctx, [9001], 4, 2, 80, F32, 64, seed=2)
 
 
+@pytest.mark.parametrize("D", [40, 48, 56, 72, 80, 88, 96, 104, 112, 120, 136, 248])
+@pytest.mark.parametrize("kv", [BF16, F16])
+def test_attention_between_the_usual_head_sizes(ctx, D, kv):
+    """16-bit heads of every multiple of 8 around the tensor-core tiles' sizes: rows of several tiles,
+    pages that end inside one, windows, and a pool that is NaN everywhere outside the live keys."""
+    lens, begin = [700, 0, 129, 128, 5, 390, 1], [3, 0, 0, 127, 5, 257, 0]
+    batch(ctx, lens, 15, 3, D, kv, 7, seed=D, sinks=True, new=D % 16 == 0, pad=D % 3)
+    batch(ctx, lens, 20, 2, D, kv, 24, seed=D, begin=begin, fill=np.nan)
+
+
 def test_attention_windows(ctx):
     lens = [100, 40, 3, 7, 90, 12]
     batch(ctx, lens, 8, 2, 64, BF16, 16, begin=[70, 0, 2, 7, 89, 30], sinks=True, new=True)  # row 3 has nothing left, row 5's start is past its end

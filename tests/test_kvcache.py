@@ -113,6 +113,11 @@ def test_attention_arguments_are_checked(lib, ctx, kw, rc):
     assert attn(lib, ctx, Described(), **kw) == rc
 
 
+def test_more_tokens_than_the_tensor_core_kernel_numbers_are_refused(lib, ctx):
+    assert attn(lib, ctx, Described(n_pages=1 << 28, page_tokens=8)) == -2
+    assert attn(lib, ctx, Described(n_pages=1 << 28, page_tokens=8, kv_type=0), n=0) == 0
+
+
 @pytest.mark.parametrize("kw, rc", [
     (dict(logits=None), -1), (dict(tokens=None), -1), (dict(lp=None), -1), (dict(k=2, ids=None), -1), (dict(k=2, top=None), -1),
     (dict(ty=39), -2), (dict(stride=99), -2), (dict(vocab=0), -2), (dict(k=33), -2), (dict(k=5, vocab=4), -2), (dict(scale=0.0), -2),
