@@ -658,7 +658,8 @@ int moearc_x_attn_decode_static(moearc_ctx *c, float *out, const float *q, const
  * (a fork onto a row that holds tokens). MOEARC_X_KV_WAIT is none of these: a kernel's wait for its
  * own copies ran out, and what it computed is invalid. New pages are the free pages of lowest id, in list order.
  * All calls are enqueued on the context's stream; the same cache must not be changed from two
- * streams at once, and calls that may overlap need a work buffer each. */
+ * streams at once, and calls that may overlap need a work buffer each. Addresses that are not whole
+ * numbers of their elements are refused (-2), here and in moearc_x_token_logprobs. */
 #define MOEARC_X_NO_PAGE 0xFFFFFFFFu
 #define MOEARC_X_KV_LIST 1024u
 #define MOEARC_X_KV_LAYERS 128u

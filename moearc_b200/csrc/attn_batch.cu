@@ -1068,6 +1068,9 @@ int moearc_x_attn_decode_batch(moearc_ctx *c, const moearc_x_kv_cache *kv, unsig
     const int rc = kv_check(c, kv);
     if (rc) return rc;
     if (!out || !q || (!k_new) != (!v_new)) return ERR;
+    for (const void *p : {static_cast<const void *>(out), static_cast<const void *>(q), static_cast<const void *>(k_new),
+                          static_cast<const void *>(v_new), static_cast<const void *>(kv_begin), static_cast<const void *>(sinks)})
+        if (!aligned(p, 4)) return ERR_ARG;
     if (layer >= kv->n_layer || n_heads == 0 || n_heads > 65535 || n_heads % kv->n_kv_heads || n_seq > KV_LIST) return ERR_ARG;
     if (n_seq == 0) return OK;
     const size_t D = kv->head_dim;

@@ -508,6 +508,7 @@ int moearc_x_kv_compact(moearc_ctx *c, const moearc_x_kv_cache *kv, unsigned int
     const int rc = page_call_check(c, kv);
     if (rc) return rc;
     if (!tables_out || !refs_out) return ERR;
+    if (!aligned(tables_out, 4) || !aligned(refs_out, 4) || !aligned(n_live, 4)) return ERR_ARG;
     if ((tables_out == kv->tables) != (refs_out == kv->refs)) return ERR_ARG;  // counts that do not go with the tables
     device_guard g(c->device);
     if (!g.ok) return ERR;

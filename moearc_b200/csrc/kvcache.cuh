@@ -24,12 +24,19 @@ inline bool kv_shape_ok(const moearc_x_kv_cache &k) {
            (unsigned long long)k.page_tokens * k.n_kv_heads < (1ull << 31) / k.head_dim;  // a page's elements, for 32-bit indexes
 }
 
+// Whether an address is a whole number of `each` bytes (2 or 4); NULL is.
+inline bool aligned(const void *p, unsigned each) { return (reinterpret_cast<uintptr_t>(p) & (each - 1)) == 0; }
+
 // 0 when every pointer is there and every number in range; else the code to return.
 inline int kv_check(const moearc_ctx *c, const moearc_x_kv_cache *k) {
     if (!c || !k || !k->k_pages || !k->v_pages || !k->tables || !k->n_kv || !k->refs || !k->status || !k->work) return ERR;
     if (!kv_shape_ok(*k)) return ERR_ARG;
     for (unsigned l = 0; l < k->n_layer; ++l)
         if (!k->k_pages[l] || !k->v_pages[l]) return ERR;
+    const unsigned each = kv_elem_bytes(k->kv_type);
+    for (unsigned l = 0; l < k->n_layer; ++l)
+        if (!aligned(k->k_pages[l], each) || !aligned(k->v_pages[l], each)) return ERR_ARG;
+    if (!aligned(k->tables, 4) || !aligned(k->n_kv, 4) || !aligned(k->refs, 4) || !aligned(k->status, 4)) return ERR_ARG;
     if (reinterpret_cast<uintptr_t>(k->work) & 15) return ERR_ARG;
     return OK;
 }

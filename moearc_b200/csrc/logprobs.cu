@@ -484,7 +484,8 @@ int moearc_x_token_logprobs(moearc_ctx *c, const void *logits, unsigned int type
     if (!kv_elem_bytes(type)) return ERR_ARG;
     if (n_vocab == 0 || n_vocab > (1u << 30) || row_stride < n_vocab || k > MAX_TOPK || k > n_vocab || n_rows > (1u << 26)) return ERR_ARG;
     if (!(scale >= 1e-30f && scale <= 1e30f)) return ERR_ARG;
-    if (reinterpret_cast<uintptr_t>(logits) % kv_elem_bytes(type)) return ERR_ARG;
+    if (!aligned(logits, kv_elem_bytes(type)) || !aligned(tokens, 4) || !aligned(logprob, 4) || !aligned(entropy, 4)) return ERR_ARG;
+    if (k && (!aligned(top_ids, 4) || !aligned(top_logprobs, 4))) return ERR_ARG;
     if (n_rows == 0) return OK;
     const lp_args a{logits, tokens, row_stride, n_vocab, k, scale, logprob, entropy, top_logprobs, top_ids};
     device_guard g(c->device);

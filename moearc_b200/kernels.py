@@ -327,6 +327,8 @@ class Context:
         """Log probabilities of `tokens` (u32 [n_rows]) under rows of logits (F32, F16 or BF16), each row's
         entropy and its k likeliest tokens (moearc_x_token_logprobs); outputs that are None are left out."""
         stride = n_vocab if row_stride is None else row_stride
+        if min(n_rows, n_vocab, stride, k) < 0:
+            raise BadArgument("a negative count or stride")
         if ty in KV_ELEM_BYTES and n_rows:
             logits.require("logits", KV_ELEM_BYTES[ty] * ((n_rows - 1) * stride + n_vocab))
         for b, what, each in ((tokens, "tokens", 1), (logprob, "log probability output", 1), (entropy, "entropy output", 1),

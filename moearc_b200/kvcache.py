@@ -146,8 +146,8 @@ class KvCache:
         floats; seqs names the cache rows (default 0 .. n_seq - 1)."""
         if n_heads < 1 or not self.n_heads:
             raise BadArgument(f"{n_heads} query heads (a cache made without n_heads has no workspace for attention)")
-        if n_seq < 0 or layer < 0:
-            raise BadArgument("a negative count")
+        if min(n_seq, layer, q_stride or 0, new_stride or 0) < 0:
+            raise BadArgument("a negative count or stride")
         row, kv_row = n_heads * self.head_dim, self.n_kv_heads * self.head_dim
         qs = row if q_stride is None else q_stride
         ns = kv_row if new_stride is None else new_stride

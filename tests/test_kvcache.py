@@ -4,7 +4,7 @@ import ctypes as C
 
 import pytest
 
-from moearc_b200 import BadArgument, _lib, kvcache
+from moearc_b200 import BadArgument, Context, _lib, kvcache
 from paged_model import BF16, FULL, LONG, TAKEN, Paged
 
 U3 = C.c_uint * 3
@@ -58,6 +58,23 @@ def test_a_bad_description_is_refused(lib, ctx, kw):
         assert lib.moearc_x_kv_work_bytes(ctx, k.ref, 8) == 0
 
 
+@pytest.mark.parametrize("name", ["tables", "n_kv", "refs", "status", "pool"])
+def test_an_address_between_elements_is_refused(lib, ctx, name):
+    for kv_type, off in ((30, 1), (0, 2)):
+        k = Described(kv_type=kv_type, **({} if name == "pool" else {name: 0x10002}))
+        if name == "pool":
+            k.one[1] = 0x10000 + off
+        assert lib.moearc_x_kv_reset(ctx, k.ref) == -2
+        assert lib.moearc_x_kv_free(ctx, k.ref, U3(0, 1, 2), None, 3) == -2
+        assert attn(lib, ctx, k) == -2
+
+
+def test_outputs_of_a_compaction_between_elements_are_refused(lib, ctx):
+    k = Described()
+    for t, r, n in ((0x20002, 0x30000, None), (0x20000, 0x30001, None), (0x20000, 0x30000, 0x10002)):
+        assert lib.moearc_x_kv_compact(ctx, k.ref, t, r, n) == -2
+
+
 @pytest.mark.parametrize("name", ["tables", "n_kv", "refs", "status", "work"])
 def test_a_missing_buffer_is_refused(lib, ctx, name):
     k = Described(**{name: None})
@@ -108,7 +125,8 @@ def attn(lib, ctx, k, **kw):
     (dict(out=None), -1), (dict(q=None), -1), (dict(kn=0x10000), -1), (dict(vn=0x10000), -1), (dict(layer=2), -2), (dict(heads=0), -2),
     (dict(heads=6), -2), (dict(qs=511), -2), (dict(kn=0x10000, vn=0x10000, ns=255), -2), (dict(n=9), -2), (dict(n=1025), -2),
     (dict(seqs=U3(0, 1, 1), n=3), -2), (dict(seqs=U3(0, 1, 8), n=3), -2), (dict(scale=float("nan")), -2), (dict(scale=float("inf")), -2),
-    (dict(n=0), 0)])
+    (dict(n=0), 0)] + [({name: 0x10002, **({"kn": 0x10000, "vn": 0x10000, name: 0x10002} if name in ("kn", "vn") else {})}, -2)
+                       for name in ("out", "q", "kn", "vn", "begin", "sinks")])
 def test_attention_arguments_are_checked(lib, ctx, kw, rc):
     assert attn(lib, ctx, Described(), **kw) == rc
 
@@ -121,11 +139,28 @@ def test_more_tokens_than_the_tensor_core_kernel_numbers_are_refused(lib, ctx):
 @pytest.mark.parametrize("kw, rc", [
     (dict(logits=None), -1), (dict(tokens=None), -1), (dict(lp=None), -1), (dict(k=2, ids=None), -1), (dict(k=2, top=None), -1),
     (dict(ty=39), -2), (dict(stride=99), -2), (dict(vocab=0), -2), (dict(k=33), -2), (dict(k=5, vocab=4), -2), (dict(scale=0.0), -2),
-    (dict(scale=-1.0), -2), (dict(scale=1e-31), -2), (dict(scale=2e30), -2), (dict(scale=float("nan")), -2), (dict(scale=float("inf")), -2), (dict(logits=0x10002), -2), (dict(rows=0), 0)])
+    (dict(scale=-1.0), -2), (dict(scale=1e-31), -2), (dict(scale=2e30), -2), (dict(scale=float("nan")), -2), (dict(scale=float("inf")), -2), (dict(logits=0x10002), -2), (dict(rows=0), 0)] +
+    [({name: 0x10002, "k": 2}, -2) for name in ("tokens", "lp", "ent", "ids", "top")] + [(dict(logits=0x10001, ty=30), -2)])
 def test_logprob_arguments_are_checked(lib, ctx, kw, rc):
     v = dict(logits=0x10000, ty=0, stride=100, rows=4, vocab=100, scale=1.0, tokens=0x10000, lp=0x10000, ent=0x10000, k=0, ids=0x10000, top=0x10000)
     v.update(kw)
     assert lib.moearc_x_token_logprobs(ctx, *v.values()) == rc
+
+
+def test_negative_counts_and_strides_are_refused():
+    """Before they would wrap to unsigned ones."""
+    c = object.__new__(kvcache.KvCache)
+    c.n_heads, c.head_dim, c.n_kv_heads = 8, 64, 4
+    for kw in (dict(n_seq=-1), dict(layer=-1), dict(q_stride=-512), dict(new_stride=-256)):
+        a = dict(layer=0, n_seq=2, q_stride=None, new_stride=None)
+        a.update(kw)
+        with pytest.raises(BadArgument):
+            c.attn_decode(a["layer"], None, None, a["n_seq"], 8, 1.0, q_stride=a["q_stride"], new_stride=a["new_stride"])
+    for kw in (dict(n_rows=-1), dict(n_vocab=-1), dict(row_stride=-100), dict(k=-1)):
+        a = dict(n_rows=2, n_vocab=100, row_stride=None, k=0)
+        a.update(kw)
+        with pytest.raises(BadArgument):
+            Context.token_logprobs(None, None, 0, a["n_rows"], a["n_vocab"], row_stride=a["row_stride"], k=a["k"])
 
 
 def test_python_lists_are_checked():
