@@ -671,7 +671,7 @@ typedef struct {
     void *const *k_pages;      /* HOST arrays of n_layer device pointers; a pool's pages hold */
     void *const *v_pages;      /* page_tokens x n_kv_heads x head_dim elements each */
     unsigned int n_layer;      /* <= MOEARC_X_KV_LAYERS */
-    unsigned int n_pages;      /* <= 2^28; a 16-bit cache of head_dim <= 128: n_pages * page_tokens < 2^31 */
+    unsigned int n_pages;      /* <= 2^28; a 16-bit cache of head_dim <= 256: n_pages * page_tokens < 2^31 */
     unsigned int page_tokens;  /* any size; max_pages * page_tokens < 2^31, a page < 2^31 elements */
     unsigned int n_kv_heads, head_dim;  /* head_dim <= 1024 */
     unsigned int kv_type;      /* F32 0, F16 1, BF16 30 */

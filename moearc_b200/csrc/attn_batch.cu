@@ -20,13 +20,11 @@
 //   warps share a head, taking alternate tiles. A warp streams its K and V tiles through a ring of
 //   cp.async stages of its own, which runs on across rows: no barrier in the loop, and the next
 //   row's keys are on their way before this row is finished.
-// - 16-bit caches of up to 128 channels, a multiple of 8 above 32, have a kernel of their own on
-//   tcgen05 (attn_tc.cu). Here, on the same line of tiles: 16-bit caches of up to 256 channels and
-//   f32 ones of up to 256 on mma.sync (one warp's tile is 16 keys, and a tile of 128 keys of such
-//   rows would leave no room for a second), every other size on CUDA cores.
-// - q and the softmax weights stay f32 in effect: a bf16 cache takes them as three bf16 terms (24
-//   bits), an f16 cache as two f16 terms (22 bits) of values scaled by a power of two, an f32 cache
-//   everything as two tf32 terms (22 to 23 bits).
+// - 16-bit caches of 40 to 256 channels, a multiple of 8, have a kernel of their own on tcgen05
+//   (attn_tc.cu). Here, on the same line of tiles: f32 caches of 36 to 256 channels, a multiple of 4,
+//   on mma.sync with tf32 terms (tcgen05's tf32 would want keys and values split in two in shared
+//   memory, twice the bytes there); every other size, and pools off a 16-byte boundary, on CUDA cores.
+// - q, the softmax weights and f32 keys and values are two tf32 terms each there (22 to 23 bits).
 //   A tile's P V is summed from zero and added to the f32 accumulator by an ordinary add: the
 //   tensor core's own accumulation truncates, which a long context would show.
 #include <algorithm>
@@ -43,202 +41,6 @@ size_t kv_page_work_bytes(unsigned n_pages);
 
 namespace {
 
-// ---- the tensor-core tile of 16-bit caches: head_dim up to 256, a multiple of 8 -----------------
-
-template <bool BF>
-__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    if constexpr (BF)
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-    else
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], unsigned p) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(p) : "memory");
-}
-__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], unsigned p) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(p) : "memory");
-}
-
-template <bool BF>
-struct mma_tile {
-    static constexpr int KEYS = 16, GP = 8, D = 256, WARPS = 6;
-    // Rows of a stage are D channels, those past head_dim zeros: chunk c of row r lies at c ^ (r & 7),
-    // so that the eight rows of an ldmatrix meet eight different bank groups.
-    static constexpr int CH = D / 8, ROW = D * 2;
-    // f16 weights are scaled away from subnormals (and stay below 65504 with the 2^8 of LAZY)
-    static constexpr float PSCALE = BF ? 1.f : 64.f;
-
-    uint32_t qa[D / 16][4], ql[BF ? D / 16 : 1][2];
-    float o[D / 8][2], m, l, sc;
-    static __host__ __device__ int stage_bytes(int) { return 2 * KEYS * ROW; }
-    static __host__ __device__ bool padded(int d) { return d < D; }
-    static __host__ __device__ int extra_bytes(int) { return 0; }
-    // byte offset of chunk c of row r
-    static __device__ __forceinline__ int at(int r, int c) { return r * ROW + (c ^ (r & 7)) * 16; }
-
-    // A whole tile of consecutive slots: `src` is the first key's row in the K pool, `to_v` the way
-    // from the K pool to the V pool. A lane copies one chunk of every row.
-    static __device__ __forceinline__ void load_run(uint8_t *stage, const uint8_t *src, long long to_v, const attn_args &a, int lane) {
-        const uint8_t *p = src + lane * 16;
-        const unsigned d0 = smem_u32(stage) + lane * 16;
-        if (lane * 8 < a.D)
-#pragma unroll
-            for (int r = 0; r < KEYS; ++r, p += a.token_bytes) {
-                const unsigned d = (d0 ^ ((r & 7) << 4)) + r * ROW;
-                cp_async16(d, p);
-                cp_async16(d + KEYS * ROW, p + to_v);
-            }
-    }
-    // Any tile: lane r holds the byte offset of key r's row in a pool, or -1 for zeros.
-    static __device__ __forceinline__ void load_rows(uint8_t *stage, long long off, const attn_args &a, int lane) {
-        const unsigned d0 = smem_u32(stage) + lane * 16;
-#pragma unroll 4
-        for (int r = 0; r < KEYS; ++r) {
-            const long long b = __shfl_sync(0xffffffffu, off, r);
-            if (lane * 8 >= a.D) continue;
-            const size_t src = (b < 0 ? 0 : (size_t)b) + lane * 16;
-            const unsigned d = (d0 ^ ((r & 7) << 4)) + r * ROW;
-            cp_async16z(d, a.k + src, b >= 0);
-            cp_async16z(d + KEYS * ROW, a.v + src, b >= 0);
-        }
-    }
-    // Rows 0-7 of the A operand hold the first term of the (up to 8) heads, rows 8-15 the second;
-    // the third, where there is one, is a second A operand with its rows 8-15 zero.
-    __device__ __forceinline__ void init(const float *q, int heads, const attn_args &a, uint8_t *, int lane) {
-        const int hr = lane >> 2, qd = lane & 3;
-        const bool live = hr < heads;
-        const float *p = q + (size_t)(live ? hr : 0) * a.D;
-        auto x = [&](int d) { return live && d < a.D ? p[d] : 0.f; };
-        float f = 1.f;
-        if constexpr (!BF) {
-            float mx = 0.f;
-#pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) mx = fmaxf(mx, fabsf(x(16 * kk + 2 * qd + (e & 1) + (e >> 1) * 8)));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            // the largest magnitude to [2^12, 2^13)
-            if (mx > 0.f) f = exp2f((float)min(100, 12 - ilogbf(mx)));
-        }
-        sc = a.scale2 / f;
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-            const int c0 = 16 * kk + 2 * qd, c1 = c0 + 8;
-            uint32_t t2 = 0, u2 = 0;
-            terms<BF>(x(c0) * f, x(c0 + 1) * f, qa[kk][0], qa[kk][1], t2);
-            terms<BF>(x(c1) * f, x(c1 + 1) * f, qa[kk][2], qa[kk][3], u2);
-            if constexpr (BF) {
-                ql[kk][0] = t2;
-                ql[kk][1] = u2;
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = 0.f;
-        m = -INFINITY;
-        l = 0.f;
-    }
-    __device__ __forceinline__ void scale_o(float f) {
-#pragma unroll
-        for (int i = 0; i < D / 8; ++i) {
-            o[i][0] *= f;
-            o[i][1] *= f;
-        }
-    }
-
-    // Row r of the stage (keys, then values) from f32, and into its slot where that is given.
-    static __device__ __forceinline__ void round_row(const float *x, uint8_t *stage, int r, uint8_t *slot, const attn_args &a, int lane) {
-        for (int d = lane; d < a.D; d += 32) {
-            const uint16_t b = to16<BF>(x[d]);
-            *reinterpret_cast<uint16_t *>(stage + at(r, d >> 3) + (d & 7) * 2) = b;
-            if (slot) reinterpret_cast<uint16_t *>(slot)[d] = b;
-        }
-    }
-
-    __device__ __forceinline__ void step(const uint8_t *stage, unsigned live, const attn_args &, uint8_t *, int lane) {
-        const int qd = lane & 3, mi = lane >> 3;
-        // this lane's rows of the ldmatrix operands: keys (non-transposed) and values (transposed).
-        // Stages start on whole rows, so chunk c + 2 i of a swizzled row is chunk c's address xor 32 i.
-        const unsigned kb = smem_u32(stage) + at(((mi >> 1) << 3) | (lane & 7), mi & 1);
-        const unsigned vb = smem_u32(stage) + KEYS * ROW + at(((mi & 1) << 3) | (lane & 7), mi >> 1);
-        float c0[2][4] = {}, c1[2][4] = {};
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-            uint32_t b[4];
-            ldsm4(b, kb ^ (kk * 32));
-            mma<BF>(c0[0], qa[kk][0], qa[kk][1], qa[kk][2], qa[kk][3], b[0], b[1]);
-            mma<BF>(c0[1], qa[kk][0], qa[kk][1], qa[kk][2], qa[kk][3], b[2], b[3]);
-            if constexpr (BF) {
-                mma<BF>(c1[0], ql[kk][0], 0u, ql[kk][1], 0u, b[0], b[1]);
-                mma<BF>(c1[1], ql[kk][0], 0u, ql[kk][1], 0u, b[2], b[3]);
-            }
-        }
-        // scores (in powers of two) of head lane / 4 for keys 2 qd, 2 qd + 1, 8 + 2 qd, 9 + 2 qd
-        float s[4];
-        const unsigned in = live >> (2 * qd);
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const float x = (c0[n][e] + (BF ? c0[n][e + 2] + c1[n][e] : c0[n][e + 2])) * sc;
-                s[2 * n + e] = in >> (8 * n + e) & 1 ? x : -INFINITY;
-            }
-        float mt = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
-        if (__any_sync(0xffffffffu, mt > m + LAZY)) {
-            mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
-            mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 2));
-            const float mn = fmaxf(m, mt), corr = ex2(m - (mn == -INFINITY ? 0.f : mn));
-            l *= corr;
-            m = mn;
-            scale_o(corr);
-        }
-        const float base = m == -INFINITY ? 0.f : m;
-        float p[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) p[e] = ex2(s[e] - base);
-        l += (p[0] + p[1]) + (p[2] + p[3]);
-        uint32_t a0, a1, a2, a3, b0 = 0, b2 = 0;
-        terms<BF>(p[0] * PSCALE, p[1] * PSCALE, a0, a1, b0);
-        terms<BF>(p[2] * PSCALE, p[3] * PSCALE, a2, a3, b2);
-#pragma unroll
-        for (int dn = 0; dn < D / 16; ++dn) {
-            uint32_t b[4];
-            ldsm4t(b, vb ^ (dn * 32));
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                float t[4] = {};
-                if constexpr (BF) mma<BF>(t, b0, 0u, b2, 0u, b[2 * h], b[2 * h + 1]);
-                mma<BF>(t, a0, a1, a2, a3, b[2 * h], b[2 * h + 1]);
-                o[2 * dn + h][0] += t[0] + t[2];
-                o[2 * dn + h][1] += t[1] + t[3];
-            }
-        }
-    }
-
-    // After the last tile: l summed over the head's lanes, o without its scale.
-    __device__ __forceinline__ void close(int) {
-        l += __shfl_xor_sync(0xffffffffu, l, 1);
-        l += __shfl_xor_sync(0xffffffffu, l, 2);
-        scale_o(1.f / PSCALE);
-    }
-    // f(head, d, o, m, l) for every value this lane holds; one(head, m, l) once a head.
-    template <typename F, typename G>
-    __device__ __forceinline__ void each(int lane, const attn_args &a, F &&f, G &&one) {
-        const int hr = lane >> 2, qd = lane & 3;
-        one(hr, m, l, qd == 0);
-#pragma unroll
-        for (int i = 0; i < D / 8; ++i) {
-            if (8 * i >= a.D) break;  // head_dim is a multiple of 8
-            f(hr, 8 * i + 2 * qd, o[i][0]);
-            f(hr, 8 * i + 2 * qd + 1, o[i][1]);
-        }
-    }
-};
-
 // ---- the tensor-core tile of f32 caches ---------------------------------------------------------
 //
 // head_dim up to D_, a multiple of 4. mma.sync m16n8k8 on tf32 terms: a key or value is its rounding to
@@ -247,6 +49,11 @@ struct mma_tile {
 // operands agree: k = j and j + 4 are channels 2 j and 2 j + 1 of an eight, read as one 8-byte load,
 // and keys 2 j and 2 j + 1, as the scores come out. Rows are 8 (keys) and 4 (values) words off a
 // multiple of 32, so that these reads meet 32 banks.
+//
+// 30 rows of up to 6000 tokens: 8 kv heads of 64 with 8 query heads each 123 us (319 on CUDA cores),
+// 4 heads of 128 with 8 each 160 (320), 1 of 256 with 16 235 (two passes over the keys), where the
+// bytes alone take 74, 74 and 37. Bound by the instructions around the MMAs (two a side, each operand
+// taken apart by integer work as it leaves shared memory) and, at one CTA an SM, by their latency.
 
 __device__ __forceinline__ uint32_t tf32(float x) {
     uint32_t u;
@@ -948,11 +755,6 @@ cudaError_t with_list(const unsigned *rows, unsigned n, F &&f) {
 
 // ---- host side --------------------------------------------------------------------------------
 
-// How a shape is cut: virtual heads and warps per CTA, stages, shared memory and the grid.
-struct attn_plan {
-    int gp, keys, subs, hg, rsplit, nhg, warps, ns, smem, grid;
-};
-
 // Whether the tensor cores serve a shape, where the pools' rows are 16-byte aligned: multiples of 8
 // channels of 16 bits and of 4 channels of f32, from the size at which half of the smallest tile is
 // used on. CUDA cores have the rest.
@@ -993,15 +795,12 @@ bool cut_any(attn_plan &p, int n_heads, int n_kv, int D, int n_seq, int sms) {
 // f(a null pointer to the tile) for the tile that serves a shape.
 template <typename F>
 auto with_tile(bool mma, unsigned kv_type, unsigned D, int group, F &&f) {
-    if (mma && kv_type == T_F32) {
+    if (mma) {  // f32: attn_tc.cu has the 16-bit ones
         if (D <= 64) return f((tf32_tile<64> *)nullptr);
         if (D <= 80) return f((tf32_tile<80> *)nullptr);
         if (D <= 128) return f((tf32_tile<128> *)nullptr);
         return f((tf32_tile<256> *)nullptr);
     }
-    if (mma)  // above 128 channels: attn_tc.cu has those below
-        return kv_type == T_BF16 ? f((mma_tile<true> *)nullptr)
-                                 : f((mma_tile<false> *)nullptr);
 #define CORE_CASE(T)                                                                                  \
     if (few_heads(D, group)) return f((core_tile<T, 1, 4> *)nullptr); \
     if (D <= 128) return f((core_tile<T, 1, 8> *)nullptr);          \
@@ -1025,8 +824,9 @@ bool plan_of(attn_plan &p, bool mma, unsigned kv_type, int n_heads, int n_kv, in
 }
 
 // The work buffer: the rows' list, a note a CTA, then the parts.
-size_t attn_bytes(int grid, int hg, int gp, int D) { return KV_LIST * 4 + (size_t)grid * 16 + (size_t)grid * 2 * hg * gp * (D + 2) * 4; }
-size_t attn_bytes(const attn_plan &p, int D) { return attn_bytes(p.grid, p.hg, p.gp, D); }
+size_t attn_bytes(const attn_plan &p, int D) {
+    return KV_LIST * 4 + (size_t)p.grid * 16 + (size_t)p.grid * 2 * p.hg * p.gp * (D + 2) * 4;
+}
 // Most query heads that an SM's CTA works on at once, hg x gp: 16 x 8 (CUDA cores) up to 128 channels,
 // 8 warps of 8 or of 4 heads above; attn_tc.cu's two CTAs of one head group are fewer.
 int heads_of_sm(unsigned D) { return D <= 128 ? 128 : D <= 256 ? 64 : 32; }
@@ -1084,14 +884,13 @@ int moearc_x_attn_decode_batch(moearc_ctx *c, const moearc_x_kv_cache *kv, unsig
         return ERR_ARG;
     }
     const uintptr_t align = reinterpret_cast<uintptr_t>(kv->k_pages[layer]) | reinterpret_cast<uintptr_t>(kv->v_pages[layer]);
-    const bool mma = tensor_dim(kv->head_dim, kv->kv_type) && (align & 15) == 0;
-    attn_plan p;
-    if (!plan_of(p, mma, kv->kv_type, (int)n_heads, (int)kv->n_kv_heads, (int)D, (int)n_seq, c->sm_count)) return ERR_ARG;
-    const bool tc = mma && kv->kv_type != T_F32 && D <= 128;
+    const bool mma = tensor_dim(kv->head_dim, kv->kv_type) && (align & 15) == 0, tc = mma && kv->kv_type != T_F32;
     // tokens are numbered in 32 bits there; more of them than that would not fit the memory
     if (tc && (unsigned long long)kv->n_pages * kv->page_tokens >= (1ull << 31)) return ERR_ARG;
-    const int tc_grid = attn_tc_grid(kv->head_dim, c->sm_count);
-    if (kv->work_bytes < (tc ? attn_bytes(tc_grid, 1, 8, (int)D) : attn_bytes(p, (int)D))) return ERR_ARG;
+    attn_plan p = {};
+    if (tc) attn_tc_plan(p, (int)n_heads, (int)kv->n_kv_heads, (int)D, c->sm_count);
+    else if (!plan_of(p, mma, kv->kv_type, (int)n_heads, (int)kv->n_kv_heads, (int)D, (int)n_seq, c->sm_count)) return ERR_ARG;
+    if (kv->work_bytes < attn_bytes(p, (int)D)) return ERR_ARG;
     const unsigned cap = kv->max_pages * kv->page_tokens;
     if ((unsigned long long)n_seq * (cap / (unsigned)(p.keys * p.rsplit) + 2) * p.nhg * p.hg >= (1ull << 31)) return ERR_ARG;
 
@@ -1131,7 +930,7 @@ int moearc_x_attn_decode_batch(moearc_ctx *c, const moearc_x_kv_cache *kv, unsig
     a.status = kv->status;
     a.rows = seqs ? static_cast<unsigned *>(kv->work) : nullptr;
     a.notes = reinterpret_cast<int4 *>(static_cast<uint8_t *>(kv->work) + KV_LIST * 4);
-    a.part = reinterpret_cast<float *>(a.notes + (tc ? tc_grid : p.grid));
+    a.part = reinterpret_cast<float *>(a.notes + p.grid);
     device_guard g(c->device);
     if (!g.ok) return ERR;
     launch_scope ls(c, "attn_decode_batch", n_seq, n_heads);
@@ -1141,7 +940,7 @@ int moearc_x_attn_decode_batch(moearc_ctx *c, const moearc_x_kv_cache *kv, unsig
             constexpr int N = (int)(sizeof(L.row) / sizeof(unsigned));
             return launch_pdl(k_attn_rows<N>, dim3(1), dim3(KV_LIST), 0, c->stream, L, n_seq, static_cast<unsigned *>(kv->work));
         });
-    if (e == cudaSuccess) e = tc ? attn_tc_launch(c, *kv, a) : with_tile(mma, kv->kv_type, kv->head_dim, a.group, [&](auto *t) {
+    if (e == cudaSuccess) e = tc ? attn_tc_launch(c, p, kv->kv_type, a) : with_tile(mma, kv->kv_type, kv->head_dim, a.group, [&](auto *t) {
         return launch<std::remove_pointer_t<decltype(t)>>(c, p, a);
     });
     if (e != cudaSuccess) cudaGetLastError();  // the failed launch's error, not left for an unrelated later check

@@ -249,9 +249,14 @@ static cudaError_t attn_join_launch(moearc_ctx *c, int grid, const attn_args &a)
                       dim3(JOIN_THREADS), (size_t)GP * grid * 4, c->stream, a);
 }
 
-// The tcgen05 kernel (attn_tc.cu), for 16-bit caches of head_dim 40 to 128, a multiple of 8, with fewer
-// than 2^31 tokens: its grid, and its launch.
-int attn_tc_grid(unsigned head_dim, int sms);
-cudaError_t attn_tc_launch(moearc_ctx *c, const moearc_x_kv_cache &kv, attn_args a);
+// How a shape is cut: virtual heads and warps per CTA, stages, shared memory and the grid.
+struct attn_plan {
+    int gp, keys, subs, hg, rsplit, nhg, warps, ns, smem, grid;
+};
+
+// The tcgen05 kernel (attn_tc.cu), for 16-bit caches of head_dim 40 to 256, a multiple of 8, with fewer
+// than 2^31 tokens: its cut, and its launch.
+void attn_tc_plan(attn_plan &p, int n_heads, int n_kv, int D, int sms);
+cudaError_t attn_tc_launch(moearc_ctx *c, const attn_plan &p, unsigned kv_type, const attn_args &a);
 
 }  // namespace moearc

@@ -1,5 +1,5 @@
 // attn_tc.cu — decode attention of a ragged batch over the paged cache on the fifth-generation
-// tensor cores: 16-bit caches of up to 128 channels, a multiple of 8 above 32 (attn_batch.cu serves
+// tensor cores: 16-bit caches of up to 256 channels, a multiple of 8 above 32 (attn_batch.cu serves
 // the rest; the formula, the equal runs and the join are the same).
 //
 // A unit is a batch row and a kv head (with up to eight of its query heads); its keys are cut into
@@ -9,11 +9,18 @@
 //   p = 2^(S - m), thread = key  eight heads a thread, from tensor memory
 //   O [channels x 32] = V' P     V as it was loaded (channel-major) as the A operand, P from the threads
 //
+// Measured: 3 rows of up to 100001 tokens, 8 heads of 128, f16, 1.08 GB: 171 us, 6.3 TB/s of a measured 6.56
+// (164 us); 64 rows of up to 4096, 4 heads of 128, bf16, 362 MB: 71 us (55), of which about 12 are the start
+// (lengths, tables, the first tile's way through the roles) and the join; 120 rows of 128 tokens, 8 heads
+// of 64: 19 us (5). The tensor pipe is 9% busy: HBM bounds long rows, the chain from load to weights to
+// output short ones. On mma.sync the first two took 193 and 93 us.
+//
 // The 32 columns are the 16-bit terms of eight heads: three for bf16 (24 bits of q and of p), two
 // for f16. The tensor core sums a tile (8 MMAs) and the threads, now one a channel, add the columns
 // of a head to f32 registers, since its sums truncate and a long row's would show it.
 //
-// Two tiles are in flight or in use. They are loaded by 16-byte asynchronous copies, two warps a
+// Two tiles are in flight or in use (one of 256 channels, its keys loaded again while its weights are
+// worked out: 16 heads over 1 of 256 channels, 30 rows of up to 6000, 50 us, 94 on mma.sync). They are loaded by 16-byte asynchronous copies, two warps a
 // stage: any page size, and as many bytes under way as the stages hold. (TMA boxes of 128-byte rows
 // brought 3.5 TB/s and untiled bulk copies of a row 4, where these bring 6.2: one head of a token is
 // 128 or 256 bytes in a row of thousands.) Roles, each a warp or more that meet at mbarriers: loads; MMA issue; four warps of
@@ -29,9 +36,9 @@ using namespace moearc;
 
 namespace {
 
-constexpr int KEYS = 128, GP = 8, NT = 32, NS = 2;
-// Warps: softmax 0-3, MMA of S 4, loads of even tiles 5-6 and of odd ones 7-8, queries 9-10, MMA of O 11.
-constexpr int THREADS = 384, LOADERS = 64;
+constexpr int KEYS = 128, GP = 8, NT = 32;
+// Warps: softmax 0-3, MMA of S 4, loads 5-8 (two a stage, or all four for the one), queries 9-10, MMA of O 11.
+constexpr int THREADS = 384, LOAD_THREADS = 128;
 constexpr int FIRST = 1, LAST = 2, WHOLE = 4, SECOND = 8;
 
 struct tile_meta {
@@ -41,11 +48,15 @@ struct tile_meta {
 
 template <int D>
 struct tc_smem {
+    // Stages of K and V: two, or one where two do not fit (a tile of 256 channels is 128 KB; its keys'
+    // half is loaded again while the weights are worked out). S, the weights, O and q are in two places either way.
+    static constexpr int NS = D <= 128 ? 2 : 1, LOADERS = LOAD_THREADS / NS;
+    static constexpr int TMEM = D <= 128 ? 128 : 256;  // columns: two of S, then two of O for each 128 channels
     static constexpr int MAT = KEYS * D * 2;       // a tile's keys (or values)
     static constexpr int Q = NT * D * 2, P = KEYS * NT * 2;
     static constexpr int STAGE = 2 * MAT;
     static constexpr int at_q = NS * STAGE, at_p = at_q + 2 * Q, at_bar = at_p + 2 * P;
-    static constexpr int at_meta = at_bar + 24 * 8, at_scale = at_meta + NS * (int)sizeof(tile_meta), at_red = at_scale + 8 * 2 * GP * 4;
+    static constexpr int at_meta = at_bar + 24 * 8, at_scale = at_meta + 2 * (int)sizeof(tile_meta), at_red = at_scale + 8 * 2 * GP * 4;
     static constexpr int at_max = at_red + 2 * 4 * GP * 4, at_tok = at_max + 2 * 4 * GP * 4;
     static constexpr int at_scan = at_tok + NS * KEYS * 4, at_pre = at_scan + 128 + 16;
     // the tile prefix, then each row's first key and end (bit 31: the end was cut to the table); 1024:
@@ -104,10 +115,11 @@ __device__ __forceinline__ float reduce8(const float (&v)[8], int lane, Op op) {
     c = op(c, __shfl_xor_sync(0xffffffffu, c, 2));
     return op(c, __shfl_xor_sync(0xffffffffu, c, 1));
 }
-// Barrier of the four softmax warps, and with it whether any thread's `x` holds.
+// Barriers of a stage's load warps, then of the four softmax warps, and with it whether any thread's `x` holds.
+template <int N>
 __device__ __forceinline__ void load_sync(int st) {
-    if (st) asm volatile("barrier.cta.sync 3, 64;" ::: "memory");
-    else asm volatile("barrier.cta.sync 2, 64;" ::: "memory");
+    if (st) asm volatile("barrier.cta.sync 3, %0;" ::"n"(N) : "memory");
+    else asm volatile("barrier.cta.sync 2, %0;" ::"n"(N) : "memory");
 }
 __device__ __forceinline__ void soft_sync() { asm volatile("barrier.cta.sync 1, 128;" ::: "memory"); }
 __device__ __forceinline__ bool soft_any(bool x) {
@@ -120,13 +132,13 @@ __device__ __forceinline__ bool soft_any(bool x) {
     return r != 0;
 }
 
-// DP: the channels that tiles have room for, 64 or 128; head_dim is that (FULL) or less.
+// DP: the channels that tiles have room for, 64, 128 or 256; head_dim is that (FULL) or less.
 template <int DP, bool FULL, bool BF>
 __global__ void __launch_bounds__(THREADS, DP == 64 ? 2 : 1)
     k_attn_tc(const __grid_constant__ attn_args a) {
     using S = tc_smem<DP>;
     const int D = FULL ? DP : a.D;
-    constexpr int CH = DP / 8, TERMS = BF ? 3 : 2;
+    constexpr int CH = DP / 8, TERMS = BF ? 3 : 2, NS = S::NS, LOADERS = S::LOADERS, MH = DP <= 128 ? 1 : DP / 128;
     constexpr float PSCALE = BF ? 1.f : 64.f;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = smem_raw + (((tc::sa(smem_raw) + 1023u) & ~1023u) - tc::sa(smem_raw));
@@ -149,7 +161,7 @@ __global__ void __launch_bounds__(THREADS, DP == 64 ? 2 : 1)
     if (D < DP)
         for (int i = threadIdx.x * 16; i < S::at_p; i += THREADS * 16) *reinterpret_cast<uint4 *>(smem + i) = make_uint4(0, 0, 0, 0);
     fence_async();
-    if (warp == 4) tc::tmem_alloc(tslot, 128);
+    if (warp == 4) tc::tmem_alloc(tslot, S::TMEM);
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
             tc::bar_init(kfull + i, LOADERS);
@@ -227,13 +239,14 @@ __global__ void __launch_bounds__(THREADS, DP == 64 ? 2 : 1)
         const int n_tiles = g1 - g0;
 
         if (warp >= 5 && warp < 9) {
-            // ---- loads: this group's tiles, every other one --------------------------------------
-            const int st = (warp - 5) >> 1, t = threadIdx.x - 160 - st * LOADERS;
+            // ---- loads: this group's tiles, every NS-th ------------------------------------------
+            const int st = NS == 2 ? (warp - 5) >> 1 : 0, t = threadIdx.x - 160 - st * LOADERS;
             auto *tok = reinterpret_cast<int *>(smem + S::at_tok) + st * KEYS;
             int s = s0, vh = vh0, u0 = unit_start(s, vh), u1 = u0 + pre[s + 1] - pre[s], was = -1;
-            unsigned lo = 0, hi = 0, newest = 0, page[2], slot[2];
+            constexpr int R = KEYS / LOADERS;  // keys a thread looks up
+            unsigned lo = 0, hi = 0, newest = 0, page[R], slot[R];
             const unsigned *tab = nullptr;
-            auto look_up = [&](int g) {  // keys t and 64 + t of tile g, one of the group's tiles early
+            auto look_up = [&](int g) {  // keys t, LOADERS + t ... of tile g, one of the group's tiles early
                 while (g >= u1) {
                     next_unit(s, vh);
                     u0 = u1;
@@ -247,8 +260,8 @@ __global__ void __launch_bounds__(THREADS, DP == 64 ? 2 : 1)
                     newest = a.k_new && !(end_key[s] >> 31) ? hi - 1 : 0xffffffffu;
                 }
 #pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    const unsigned j = lo + (unsigned)(g - u0) * KEYS + r * 64 + t;
+                for (int r = 0; r < R; ++r) {
+                    const unsigned j = lo + (unsigned)(g - u0) * KEYS + r * LOADERS + t;
                     page[r] = NO_PAGE;
                     if (j < hi) {
                         unsigned e;
@@ -287,7 +300,8 @@ __global__ void __launch_bounds__(THREADS, DP == 64 ? 2 : 1)
             for (; i < n_tiles; i += NS) {
                 const int g = g0 + i;
                 // the keys' place is free once S is computed, the values' once O is
-                bool ok = i < NS || tc::bar_wait(sfull + st, ((i >> 1) - 1) & 1, abort, status, WAIT);
+                const int was_in = i - NS;  // the stage's last tile
+                bool ok = i < NS || tc::bar_wait(sfull + (was_in & 1), (was_in >> 1) & 1, abort, status, WAIT);
                 if (!__all_sync(0xffffffffu, ok)) break;
                 const unsigned j0 = lo + (unsigned)(g - u0) * KEYS;
                 const int kvh = vh / a.subs, at_new = newest >= j0 && newest - j0 < KEYS ? (int)(newest - j0) : -1;
@@ -295,38 +309,39 @@ __global__ void __launch_bounds__(THREADS, DP == 64 ? 2 : 1)
                                   (u0 >= g0 && u1 <= g1 ? WHOLE : 0) | (u0 > g0 ? SECOND : 0);
                 const bool stores = vh == kvh * a.subs;
                 const int row_i = s, vh_i = vh;
-                unsigned m[2];
+                unsigned m[R];
 #pragma unroll
-                for (int r = 0; r < 2; ++r) {
+                for (int r = 0; r < R; ++r) {
                     const bool in = page[r] < a.n_pages;
                     const int id = in ? (int)(page[r] * a.pt + slot[r]) : -1;
                     m[r] = __ballot_sync(0xffffffffu, in);
-                    tok[r * 64 + t] = in && r * 64 + t == at_new ? -2 - id : id;
+                    tok[r * LOADERS + t] = in && r * LOADERS + t == at_new ? -2 - id : id;
                 }
-                load_sync(st);
+                load_sync<LOADERS>(st);
                 const size_t head = (size_t)kvh * a.head_bytes;
                 copy(a.k + head + ch * 16, d0);
-                ok = i < NS || tc::bar_wait(empty + st, ((i >> 1) - 1) & 1, abort, status, WAIT);
-                if (lane == 0) {
-                    meta[st].live[(warp - 5) & 1] = m[0];
-                    meta[st].live[2 + ((warp - 5) & 1)] = m[1];
-                }
+                ok = i < NS || tc::bar_wait(empty + (was_in & 1), (was_in >> 1) & 1, abort, status, WAIT);
+                auto &note = meta[i & 1];
+                if (lane == 0)
+#pragma unroll
+                    for (int r = 0; r < R; ++r) note.live[(r * LOADERS + t) >> 5] = m[r];
                 if (t == 0) {
-                    meta[st].flags = flags;
-                    meta[st].row = row_i;
-                    meta[st].vh = vh_i;
+                    note.flags = flags;
+                    note.row = row_i;
+                    note.vh = vh_i;
                 }
                 copy(a.v + head + ch * 16, d0 + S::MAT);
-                float kn[DP / 64], vn[DP / 64];
+                constexpr int EACH = DP / LOADERS;
+                float kn[EACH], vn[EACH];
                 uint8_t *slot_k = nullptr, *slot_v = nullptr;
                 const bool fresh = at_new >= 0 && tok[at_new] < -1;
                 if (fresh) {
                     const size_t src = (size_t)row_i * a.new_stride + (size_t)kvh * D + t, dst = (size_t)(-2 - tok[at_new]) * a.token_bytes + head;
 #pragma unroll
-                    for (int e = 0; e < DP / 64; ++e)
-                        if (t + e * 64 < D) {
-                            kn[e] = a.k_new[src + e * 64];
-                            vn[e] = a.v_new[src + e * 64];
+                    for (int e = 0; e < EACH; ++e)
+                        if (t + e * LOADERS < D) {
+                            kn[e] = a.k_new[src + e * LOADERS];
+                            vn[e] = a.v_new[src + e * LOADERS];
                         }
                     if (stores) {
                         slot_k = a.k + dst;
@@ -337,21 +352,21 @@ __global__ void __launch_bounds__(THREADS, DP == 64 ? 2 : 1)
                 cp_wait<1>();
                 if (fresh)
 #pragma unroll
-                    for (int e = 0; e < DP / 64; ++e)
-                        if (t + e * 64 < D) put(0, at_new, t + e * 64, kn[e], slot_k);
+                    for (int e = 0; e < EACH; ++e)
+                        if (t + e * LOADERS < D) put(0, at_new, t + e * LOADERS, kn[e], slot_k);
                 fence_async();  // what the copies wrote, before the tensor core reads it
                 tc::bar_arrive(kfull + st);
                 cp_wait<0>();
                 if (fresh)
 #pragma unroll
-                    for (int e = 0; e < DP / 64; ++e)
-                        if (t + e * 64 < D) put(1, at_new, t + e * 64, vn[e], slot_v);
+                    for (int e = 0; e < EACH; ++e)
+                        if (t + e * LOADERS < D) put(1, at_new, t + e * LOADERS, vn[e], slot_v);
                 fence_async();
                 tc::bar_arrive(vfull + st);
                 if (!__all_sync(0xffffffffu, ok)) break;
             }
             // the MMA's last arrival, before the CTA ends
-            if (i >= NS && *abort == 0) tc::bar_drain(empty + st, ((i >> 1) - 1) & 1);
+            if (i >= NS && *abort == 0) tc::bar_drain(empty + ((i - NS) & 1), ((i - NS) >> 1) & 1);
         } else if (warp == 4) {
             // ---- S = K Q' ------------------------------------------------------------------------
             // (apart from O = V' P: with one warp for both, a tile's O would wait for the next tile's keys)
@@ -359,10 +374,10 @@ __global__ void __launch_bounds__(THREADS, DP == 64 ? 2 : 1)
             const uint32_t base = tc::sa(smem);
             int u = 0;
             for (int i = 0; i < n_tiles; ++i) {
-                const int st = i & 1;
-                bool ok = tc::bar_wait(kfull + st, (i >> 1) & 1, abort, status, WAIT);
-                if (ok && i >= 2) ok = tc::bar_wait(pfull + st, ((i >> 1) - 1) & 1, abort, status, WAIT);  // tile i - 2's S has been read
-                const int flags = meta[st].flags;
+                const int st = i % NS;
+                bool ok = tc::bar_wait(kfull + st, (i / NS) & 1, abort, status, WAIT);
+                if (ok && i >= 2) ok = tc::bar_wait(pfull + (i & 1), ((i >> 1) - 1) & 1, abort, status, WAIT);  // tile i - 2's S has been read
+                const int flags = meta[i & 1].flags;
                 if (ok && (flags & FIRST)) ok = tc::bar_wait(qfull + (u & 1), (u >> 1) & 1, abort, status, WAIT);
                 if (!__all_sync(0xffffffffu, ok)) break;
                 __syncwarp();
@@ -387,18 +402,21 @@ __global__ void __launch_bounds__(THREADS, DP == 64 ? 2 : 1)
             constexpr uint32_t kind = (BF ? tc::idesc_bf16_f32(128, NT) : tc::idesc_f16_f32(128, NT)) | 1u << 15 | 1u << 16;
             const uint32_t base = tc::sa(smem);
             for (int i = 0; i < n_tiles; ++i) {
-                const int st = i & 1;
-                bool ok = tc::bar_wait(vfull + st, (i >> 1) & 1, abort, status, WAIT);
-                if (ok) ok = tc::bar_wait(pfull + st, (i >> 1) & 1, abort, status, WAIT);
+                const int st = i % NS, at = i & 1;
+                bool ok = tc::bar_wait(vfull + st, (i / NS) & 1, abort, status, WAIT);
+                if (ok) ok = tc::bar_wait(pfull + at, (i >> 1) & 1, abort, status, WAIT);
                 if (!__all_sync(0xffffffffu, ok)) break;
                 tc::fence_after_sync();
                 if (lane == 0) {
-                    const uint32_t v = base + st * S::STAGE + S::MAT, p = base + S::at_p + st * S::P;
+                    const uint32_t v = base + st * S::STAGE + S::MAT, p = base + S::at_p + at * S::P;
 #pragma unroll
-                    for (int kk = 0; kk < KEYS / 16; ++kk)
-                        tc::mma_bf16(tmem + 64 + st * 32, desc_v(v + kk * 2048, DP == 128 ? KEYS * 128 : 0), desc_p(p + kk * 1024), kind, kk > 0);
-                    tc::mma_commit(ofull + st);
-                    tc::mma_commit(empty + st);
+                    for (int h = 0; h < MH; ++h)  // 128 channels each
+#pragma unroll
+                        for (int kk = 0; kk < KEYS / 16; ++kk)
+                            tc::mma_bf16(tmem + 64 + (h * 2 + at) * 32, desc_v(v + h * 2 * KEYS * 128 + kk * 2048, DP >= 128 ? KEYS * 128 : 0),
+                                         desc_p(p + kk * 1024), kind, kk > 0);
+                    tc::mma_commit(ofull + at);
+                    tc::mma_commit(empty + at);
                 }
                 __syncwarp();
             }
@@ -455,7 +473,7 @@ __global__ void __launch_bounds__(THREADS, DP == 64 ? 2 : 1)
         } else {
             // ---- softmax: thread = key of S, then channel of O ----------------------------------
             const int t = threadIdx.x;
-            float O[GP], l[GP], m[GP], sc[GP];
+            float O[MH][GP], l[GP], m[GP], sc[GP];
             int u = 0;
             bool ok = true;
             auto *red = reinterpret_cast<float *>(smem + S::at_red);
@@ -464,23 +482,27 @@ __global__ void __launch_bounds__(THREADS, DP == 64 ? 2 : 1)
             auto flush = [&](int i) {  // O takes tile i's sums
                 if (!__all_sync(0xffffffffu, tc::bar_wait(ofull + (i & 1), (i >> 1) & 1, abort, status, WAIT))) return false;
                 tc::fence_after_sync();
-                float c[32];
-                tmem_ld32(tmem + 64 + (i & 1) * 32 + lanes, c);
 #pragma unroll
-                for (int h = 0; h < GP; ++h) O[h] += BF ? c[h] + (c[8 + h] + c[16 + h]) : c[h] + c[8 + h];
+                for (int b = 0; b < MH; ++b) {
+                    float c[32];
+                    tmem_ld32(tmem + 64 + (b * 2 + (i & 1)) * 32 + lanes, c);
+#pragma unroll
+                    for (int h = 0; h < GP; ++h) O[b][h] += BF ? c[h] + (c[8 + h] + c[16 + h]) : c[h] + c[8 + h];
+                }
                 return true;
             };
             bool pending = false;
             for (int i = 0; i < n_tiles; ++i) {
                 const int st = i & 1;
-                ok = ok && tc::bar_wait(kfull + st, (i >> 1) & 1, abort, status, WAIT) && tc::bar_wait(sfull + st, (i >> 1) & 1, abort, status, WAIT);
+                ok = ok && tc::bar_wait(kfull + i % NS, (i / NS) & 1, abort, status, WAIT) && tc::bar_wait(sfull + st, (i >> 1) & 1, abort, status, WAIT);
                 const int flags = meta[st].flags;
                 if (ok && (flags & FIRST)) ok = tc::bar_wait(qready + (u & 3), (u >> 2) & 1, abort, status, WAIT);
                 if (soft_any(!ok)) break;  // the four warps leave together: they meet at barriers
                 if (flags & FIRST) {
 #pragma unroll
                     for (int h = 0; h < GP; ++h) {
-                        O[h] = l[h] = 0.f;
+                        for (int b = 0; b < MH; ++b) O[b][h] = 0.f;
+                        l[h] = 0.f;
                         m[h] = -INFINITY;
                         sc[h] = scales[(u & 7) * 2 * GP + h];
                     }
@@ -514,7 +536,7 @@ __global__ void __launch_bounds__(THREADS, DP == 64 ? 2 : 1)
                         const float mn = fmaxf(fmaxf(fmaxf(m[h], x[0]), fmaxf(x[GP], x[2 * GP])), x[3 * GP]);
                         const float corr = ex2(m[h] - (mn == -INFINITY ? 0.f : mn));
                         l[h] *= corr;
-                        O[h] *= corr;
+                        for (int b = 0; b < MH; ++b) O[b][h] *= corr;
                         m[h] = mn;
                     }
                 }
@@ -546,7 +568,7 @@ __global__ void __launch_bounds__(THREADS, DP == 64 ? 2 : 1)
 #pragma unroll
                     for (int h = 0; h < GP; ++h) {
                         l[h] = (x[h] + x[GP + h]) + (x[2 * GP + h] + x[3 * GP + h]);
-                        O[h] *= 1.f / PSCALE;
+                        for (int b = 0; b < MH; ++b) O[b][h] *= 1.f / PSCALE;
                     }
                     if (flags & WHOLE) {
                         float *out = a.out + ((size_t)row * a.n_heads + h0) * D;
@@ -560,13 +582,18 @@ __global__ void __launch_bounds__(THREADS, DP == 64 ? 2 : 1)
                                 f = m[h] == -INFINITY ? 0.f : ex2(m[h] - top);
                                 sum = sum * f + ex2(sk - top);
                             }
-                            if (t < D) out[h * D + t] = sum == 0.f ? 0.f : O[h] * (f / sum);
+                            f = sum == 0.f ? 0.f : f / sum;
+#pragma unroll
+                            for (int b = 0; b < MH; ++b)
+                                if (b * 128 + t < D) out[h * D + b * 128 + t] = O[b][h] * f;
                         }
                     } else {
                         float *part = a.part + ((size_t)blockIdx.x * 2 + (flags & SECOND ? 1 : 0)) * GP * (D + 2);
 #pragma unroll
                         for (int h = 0; h < GP; ++h) {
-                            if (t < D) part[h * D + t] = O[h];
+#pragma unroll
+                            for (int b = 0; b < MH; ++b)
+                                if (b * 128 + t < D) part[h * D + b * 128 + t] = O[b][h];
                             if (t == h) {
                                 part[GP * D + 2 * h] = m[h];
                                 part[GP * D + 2 * h + 1] = l[h];
@@ -583,36 +610,39 @@ __global__ void __launch_bounds__(THREADS, DP == 64 ? 2 : 1)
     tc::fence_before_sync();
     __syncthreads();
     tc::fence_after_sync();
-    if (warp == 4) tc::tmem_dealloc(tmem, 128);
+    if (warp == 4) tc::tmem_dealloc(tmem, S::TMEM);
 }
 
 template <int DP, bool FULL, bool BF>
-cudaError_t launch_tile(moearc_ctx *c, attn_args &a) {
+cudaError_t launch_tile(moearc_ctx *c, int grid, const attn_args &a) {
     static std::atomic<bool> done[MOEARC_MAX_DEVICES];
-    const cudaError_t e = once_per_device(done, [] { return set_smem(k_attn_tc<DP, FULL, BF>, tc_smem<DP>::total((int)KV_LIST)); });
-    if (e != cudaSuccess) return e;
-    const int grid = attn_tc_grid(DP, c->sm_count);
-    const cudaError_t e2 =
-        launch_pdl(k_attn_tc<DP, FULL, BF>, dim3((unsigned)grid), dim3(THREADS), (size_t)tc_smem<DP>::total((int)a.n_seq), c->stream, a);
-    return e2 != cudaSuccess ? e2 : attn_join_launch<GP>(c, grid, a);
+    cudaError_t e = once_per_device(done, [] { return set_smem(k_attn_tc<DP, FULL, BF>, tc_smem<DP>::total((int)KV_LIST)); });
+    if (e == cudaSuccess)
+        e = launch_pdl(k_attn_tc<DP, FULL, BF>, dim3((unsigned)grid), dim3(THREADS), (size_t)tc_smem<DP>::total((int)a.n_seq), c->stream, a);
+    return e != cudaSuccess ? e : attn_join_launch<GP>(c, grid, a);
 }
 template <bool BF>
-cudaError_t launch(moearc_ctx *c, attn_args &a) {
-    if (a.D <= 64) return a.D == 64 ? launch_tile<64, true, BF>(c, a) : launch_tile<64, false, BF>(c, a);
-    return a.D == 128 ? launch_tile<128, true, BF>(c, a) : launch_tile<128, false, BF>(c, a);
+cudaError_t launch(moearc_ctx *c, int grid, const attn_args &a) {
+    if (a.D <= 64) return a.D == 64 ? launch_tile<64, true, BF>(c, grid, a) : launch_tile<64, false, BF>(c, grid, a);
+    if (a.D <= 128) return a.D == 128 ? launch_tile<128, true, BF>(c, grid, a) : launch_tile<128, false, BF>(c, grid, a);
+    return a.D == 256 ? launch_tile<256, true, BF>(c, grid, a) : launch_tile<256, false, BF>(c, grid, a);
 }
 
 }  // namespace
 
 namespace moearc {
 
-int attn_tc_grid(unsigned head_dim, int sms) { return head_dim <= 64 ? 2 * sms : sms; }
+void attn_tc_plan(attn_plan &p, int n_heads, int n_kv, int D, int sms) {
+    p.gp = GP;
+    p.keys = KEYS;
+    p.subs = (n_heads / n_kv + GP - 1) / GP;
+    p.hg = p.rsplit = 1;
+    p.nhg = n_kv * p.subs;
+    p.grid = D <= 64 ? 2 * sms : sms;
+}
 
-cudaError_t attn_tc_launch(moearc_ctx *c, const moearc_x_kv_cache &kv, attn_args a) {
-    a.subs = (a.group + GP - 1) / GP;
-    a.hg = 1;
-    a.nhg = (int)kv.n_kv_heads * a.subs;
-    return kv.kv_type == T_BF16 ? launch<true>(c, a) : launch<false>(c, a);
+cudaError_t attn_tc_launch(moearc_ctx *c, const attn_plan &p, unsigned kv_type, const attn_args &a) {
+    return kv_type == T_BF16 ? launch<true>(c, p.grid, a) : launch<false>(c, p.grid, a);
 }
 
 }  // namespace moearc
