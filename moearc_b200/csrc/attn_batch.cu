@@ -51,7 +51,7 @@ namespace {
 // multiple of 32, so that these reads meet 32 banks.
 //
 // 30 rows of up to 6000 tokens: 8 kv heads of 64 with 8 query heads each 123 us (319 on CUDA cores),
-// 4 heads of 128 with 8 each 160 (320), 1 of 256 with 16 235 (two passes over the keys), where the
+// 4 heads of 128 with 8 each 160 (320), 1 of 256 with 16 139 (two passes over the keys), where the
 // bytes alone take 74, 74 and 37. Bound by the instructions around the MMAs (two a side, each operand
 // taken apart by integer work as it leaves shared memory) and, at one CTA an SM, by their latency.
 
@@ -72,7 +72,9 @@ __device__ __forceinline__ void halves(float x, uint32_t &hi, uint32_t &lo) {
 
 template <int D_>
 struct tf32_tile {
-    static constexpr int KEYS = 16, GP = 8, D = D_, WARPS = D_ > 128 ? 4 : 8;
+    // 16 keys a tile; of 256 channels 8, so that four warps' tiles fit where two did (30 rows of up to
+    // 6000: 139 us, 235 with 16; at 64 and 80 channels 8 keys in twice the warps lose: 134 and 123)
+    static constexpr int KEYS = D_ > 128 ? 8 : 16, NB = KEYS / 8, GP = 8, D = D_, WARPS = D_ > 128 ? 4 : 8;
     static constexpr int KROW = (D + 31) / 32 * 32 + 8, VROW = (D + 31) / 32 * 32 + 4;  // words
     static constexpr bool QREG = D <= 128;  // q's terms in registers, else in shared memory
 
@@ -154,7 +156,7 @@ struct tf32_tile {
     }
     __device__ __forceinline__ void step(const uint8_t *stage, unsigned live, const attn_args &a, uint8_t *extra, int lane) {
         const int g = lane >> 2, qd = lane & 3;
-        float c0[2][4] = {}, c1[2][4] = {};
+        float c0[2][4] = {}, c1[2][4] = {};  // of each eight keys, or of one and every other eight channels
         const float *ks = reinterpret_cast<const float *>(stage + key_row(g)) + 2 * qd;
 #pragma unroll
         for (int kk = 0; kk < D / 8; ++kk) {
@@ -170,26 +172,33 @@ struct tf32_tile {
                 w[3] = u.w;
             }
 #pragma unroll
-            for (int n = 0; n < 2; ++n) {
+            for (int n = 0; n < NB; ++n) {
                 const float2 k = *reinterpret_cast<const float2 *>(ks + n * 8 * KROW + 8 * kk);
                 uint32_t h0, h1, l0, l1;
                 halves(k.x, h0, l0);
                 halves(k.y, h1, l1);
-                mma_tf32(c0[n], w, h0, h1);
-                mma_tf32(c1[n], w, l0, l1);
+                mma_tf32(c0[NB == 2 ? n : kk & 1], w, h0, h1);
+                mma_tf32(c1[NB == 2 ? n : kk & 1], w, l0, l1);
             }
         }
-        // scores (in powers of two) of head lane / 4 for keys 2 qd, 2 qd + 1, 8 + 2 qd, 9 + 2 qd
-        float s[4];
+        // scores (in powers of two) of head lane / 4 for keys 2 qd, 2 qd + 1 (and 8 + 2 qd, 9 + 2 qd)
+        float s[2 * NB], mt = -INFINITY;
         const unsigned in = live >> (2 * qd);
+        if constexpr (NB == 1) {
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+            for (int e = 0; e < 4; ++e) {
+                c0[0][e] += c0[1][e];
+                c1[0][e] += c1[1][e];
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const float x = (c0[n][e] + (c0[n][e + 2] + (c1[n][e] + c1[n][e + 2]))) * a.scale2;
                 s[2 * n + e] = in >> (8 * n + e) & 1 ? x : -INFINITY;
+                mt = fmaxf(mt, s[2 * n + e]);
             }
-        float mt = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
         if (__any_sync(0xffffffffu, mt > m + LAZY)) {
             mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
             mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 2));
@@ -203,9 +212,9 @@ struct tf32_tile {
             }
         }
         const float base = m == -INFINITY ? 0.f : m;
-        uint32_t pa[2][4];
+        uint32_t pa[NB][4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < 2 * NB; ++e) {
             const float p = ex2(s[e] - base);
             l += p;
             pa[e >> 1][2 * (e & 1)] = tf32(p);
@@ -216,7 +225,7 @@ struct tf32_tile {
         for (int i = 0; i < D / 8; ++i) {
             float c[4] = {}, d[4] = {};
 #pragma unroll
-            for (int n = 0; n < 2; ++n) {
+            for (int n = 0; n < NB; ++n) {
                 uint32_t h0, h1, l0, l1;
                 halves(vs[n * 8 * VROW + 8 * i], h0, l0);
                 halves(vs[(n * 8 + 1) * VROW + 8 * i], h1, l1);

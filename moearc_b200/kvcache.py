@@ -31,7 +31,13 @@ FULL, LONG, TAKEN, WAIT = 1, 2, 4, 8
 
 def _list(v) -> array:
     try:
-        a = v if isinstance(v, array) and v.typecode == "I" else array("I", v)
+        if isinstance(v, array) and v.typecode == "I":
+            a = v
+        elif isinstance(v, list):  # 256 rows: 3.0 us, 4.2 through the iterator
+            a = array("I")
+            a.fromlist(v)
+        else:
+            a = array("I", v)
     except (OverflowError, TypeError) as e:
         raise BadArgument(f"a row list of whole numbers is wanted: {e}") from None
     if len(a) > MAX_LIST:
