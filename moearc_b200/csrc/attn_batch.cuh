@@ -26,7 +26,6 @@ struct attn_args {
     const unsigned *rows;  // the batch rows' cache rows, or null: row i is i
     int n_heads, group, D, subs;  // subs: virtual heads a kv head (its query heads by GP)
     int hg, rsplit, nhg;          // virtual heads a CTA, warps a head, head groups
-    int min_tiles;
     float scale2;  // scale x log2(e): scores are kept in powers of two
     float *part;   // [CTA][2][hg][GP][D + 2]
     int4 *notes;   // [CTA] what is to join: batch row, first virtual head, parts (0: nothing), the first part's record
