@@ -19,7 +19,10 @@
 //   warps together read whole rows of a page; where a model has fewer heads than warps, several
 //   warps share a head, taking alternate tiles. A warp streams its K and V tiles through a ring of
 //   cp.async stages of its own, which runs on across rows: no barrier in the loop, and the next
-//   row's keys are on their way before this row is finished.
+//   row's keys are on their way before this row is finished. The tensor-core tiles' copies are issued by
+//   other warps (one for two), which hand stages over and back at mbarriers with a limit to every wait:
+//   the addresses of a tile's copies were a third of a computing warp's instructions (21 rows of up to
+//   2999, 20/5 heads of 80, f32: 52.6 -> 45.6 us). The CUDA cores' tile has 16 warps that hide them.
 // - 16-bit caches of 40 to 256 channels, a multiple of 8, have a kernel of their own on tcgen05
 //   (attn_tc.cu). Here, on the same line of tiles: f32 caches of 36 to 256 channels, a multiple of 4,
 //   on mma.sync with tf32 terms (tcgen05's tf32 would want keys and values split in two in shared
@@ -32,6 +35,7 @@
 #include <type_traits>
 
 #include "attn_batch.cuh"
+#include "tc.cuh"
 
 using namespace moearc;
 
@@ -50,8 +54,8 @@ namespace {
 // and keys 2 j and 2 j + 1, as the scores come out. Rows are 8 (keys) and 4 (values) words off a
 // multiple of 32, so that these reads meet 32 banks.
 //
-// 30 rows of up to 6000 tokens: 8 kv heads of 64 with 8 query heads each 123 us (319 on CUDA cores),
-// 4 heads of 128 with 8 each 160 (320), 1 of 256 with 16 139 (two passes over the keys), where the
+// 30 rows of up to 6000 tokens: 8 kv heads of 64 with 8 query heads each 114 us (319 on CUDA cores),
+// 4 heads of 128 with 8 each 149 (320), 1 of 256 with 16 140 (two passes over the keys), where the
 // bytes alone take 74, 74 and 37. Bound by the instructions around the MMAs (two a side, each operand
 // taken apart by integer work as it leaves shared memory) and, at one CTA an SM, by their latency.
 
@@ -75,6 +79,7 @@ struct tf32_tile {
     // 16 keys a tile; of 256 channels 8, so that four warps' tiles fit where two did (30 rows of up to
     // 6000: 139 us, 235 with 16; at 64 and 80 channels 8 keys in twice the warps lose: 134 and 123)
     static constexpr int KEYS = D_ > 128 ? 8 : 16, NB = KEYS / 8, GP = 8, D = D_, WARPS = D_ > 128 ? 4 : 8;
+    static constexpr bool SPLIT = true;
     static constexpr int KROW = (D + 31) / 32 * 32 + 8, VROW = (D + 31) / 32 * 32 + 4;  // words
     static constexpr bool QREG = D <= 128;  // q's terms in registers, else in shared memory
 
@@ -259,7 +264,7 @@ struct tf32_tile {
 // Values: a lane owns groups of four channels (lane + 32 i) of all GP heads, the weights come from
 // shared memory, each twice over: channels are multiplied in pairs (fma.rn.f32x2), which halves the
 // instructions, and those are what bounds it: 64 query heads over 8 of 64, f32, 30 rows of up to 6000
-// tokens 319 us, 2.6 times the tensor cores' tile.
+// tokens 319 us, 2.8 times the tensor cores' tile.
 
 // d += a b, two values at once.
 __device__ __forceinline__ void fma2(float2 &d, float2 a, float2 b) {
@@ -290,6 +295,7 @@ __device__ __forceinline__ void round_to(float v, __nv_bfloat16 &d) { d = __floa
 template <typename T, int NQ, int GP_>
 struct core_tile {
     static constexpr int KEYS = 8, GP = GP_, WARPS = NQ == 1 ? 16 : 8;
+    static constexpr bool SPLIT = false;
     float2 acc[NQ][GP][2];
     float m[GP / 4], l[GP / 4];
 
@@ -500,7 +506,8 @@ struct core_tile {
 // Shared memory: scan words and the tile prefix, then per warp its stages (KEYS rows of K, KEYS of V), then per
 // warp the stages' live masks and the new token's place, the heads' sums and what the tile keeps (q), then the
 // accumulators that warps of one head add.
-constexpr int MAX_NS = 4;  // masks and places kept a warp
+constexpr int MAX_NS = 4;  // masks, places and barriers kept a warp
+constexpr int WARP_HEAD = MAX_NS * 28;
 struct smem_layout {
     int ring, warp, warp_bytes, merge, total;
 };
@@ -508,29 +515,41 @@ __host__ __device__ inline smem_layout layout_of(int n_seq, int warps, int ns, i
     smem_layout s;
     s.ring = (128 + (((n_seq + 31) & ~31) + 1) * 4 + 511) & ~511;  // rows of up to 512 bytes start on a multiple of their size
     s.warp = s.ring + warps * ns * stage;
-    s.warp_bytes = (MAX_NS * 12 + 3 * gp * 4 + extra + 15) & ~15;
+    s.warp_bytes = (WARP_HEAD + 3 * gp * 4 + extra + 15) & ~15;
     s.merge = s.warp + warps * s.warp_bytes;
     s.total = s.merge + merge_warps * gp * D * 4;
     return s;
 }
 
 template <class Tile>
-__global__ void __launch_bounds__(Tile::WARPS * 32, 1)
+__global__ void __launch_bounds__(Tile::WARPS * (Tile::SPLIT ? 48 : 32), 1)
     k_attn_batch(const __grid_constant__ attn_args a, int ns) {
     extern __shared__ __align__(1024) uint8_t smem[];
     constexpr int KEYS = Tile::KEYS, GP = Tile::GP;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    const int D = a.D, HG = a.hg, R = a.rsplit, hs = warp % HG, r = warp / HG;
+    constexpr bool SPLIT = Tile::SPLIT;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int D = a.D, HG = a.hg, R = a.rsplit, hs = warp % HG, r = warp / HG, warps = HG * R;
     const int stage_bytes = Tile::stage_bytes(D);
     const smem_layout S = layout_of((int)a.n_seq, warps, ns, stage_bytes, Tile::extra_bytes(D), GP, warps - HG, D);
     int *sums = reinterpret_cast<int *>(smem), *pre = sums + 32;
-    uint8_t *ring = smem + S.ring + warp * ns * stage_bytes;
-    uint8_t *mine = smem + S.warp + warp * S.warp_bytes;
-    auto *slots = reinterpret_cast<long long *>(mine);  // the new token's place in a pool, where its tile is
-    auto *masks = reinterpret_cast<unsigned *>(slots + MAX_NS);
-    auto warp_heads = [&](int w) { return reinterpret_cast<float *>(smem + S.warp + w * S.warp_bytes + MAX_NS * 12); };
+    volatile int *abort = sums + 31;  // past what the scan's warps use
+    // a computing warp's: the new token's place in a pool, where its tile is; SPLIT: its stages' barriers;
+    // the stages' live keys
+    auto ring_of = [&](int w) { return smem + S.ring + w * ns * stage_bytes; };
+    auto slots_of = [&](int w) { return reinterpret_cast<long long *>(smem + S.warp + w * S.warp_bytes); };
+    auto full_of = [&](int w) { return reinterpret_cast<uint64_t *>(slots_of(w) + MAX_NS); };
+    auto empty_of = [&](int w) { return full_of(w) + MAX_NS; };
+    auto masks_of = [&](int w) { return reinterpret_cast<unsigned *>(empty_of(w) + MAX_NS); };
+    auto warp_heads = [&](int w) { return reinterpret_cast<float *>(smem + S.warp + w * S.warp_bytes + WARP_HEAD); };
     float *hm = warp_heads(warp), *hl = hm + GP, *ff = hl + GP;
     uint8_t *extra = reinterpret_cast<uint8_t *>(ff + GP);
+    if (SPLIT && warp < warps && lane == 0) {
+        for (int i = 0; i < ns; ++i) {
+            tc::bar_init(full_of(warp) + i, 33);  // a lane's copies each, and the note
+            tc::bar_init(empty_of(warp) + i, 1);
+        }
+        tc::bar_init_fence();
+    }
     // rows' tails past head_dim hold zeros: no copy writes there
     if (Tile::padded(D))
         for (int i = threadIdx.x * 16; i < warps * ns * stage_bytes; i += blockDim.x * 16)
@@ -549,7 +568,10 @@ __global__ void __launch_bounds__(Tile::WARPS * 32, 1)
         if (i < a.n_seq) pre[i + 1] = run + upto;
         run += total;
     }
-    if (threadIdx.x == 0) pre[0] = 0;
+    if (threadIdx.x == 0) {
+        pre[0] = 0;
+        *abort = 0;
+    }
     __syncthreads();
     const int line = run, T = line * a.nhg;  // below 2^31: the host has seen to it
     const int ctas = min((int)gridDim.x, max(1, T));
@@ -586,57 +608,98 @@ __global__ void __launch_bounds__(Tile::WARPS * 32, 1)
         } while (pre[s + 1] == pre[s]);
     };
 
-    // The loading side runs ns - 1 tiles ahead of the computing side, across rows.
+    // The loading side runs ns - 1 tiles ahead of the computing side, across rows: the same warp, or
+    // (SPLIT) a warp of its own for every two computing ones.
+    constexpr int SERVED = SPLIT ? 2 : 1;
+    const int apart = SPLIT ? (int)(blockDim.x >> 5) - warps : 0, first_w = SPLIT ? warp - warps : warp;
     int lg = g0, lend, ls = s0, lh = h0g, lstage = 0;
-    unsigned lrow, llo, lhi, lslot = 0, lpage = NO_PAGE, lnew;
+    unsigned lrow, llo, lhi, lnew, lslot[SERVED] = {}, lpage[SERVED], lj[SERVED] = {};
     const unsigned *ltab;
-    size_t lhead;
     auto enter = [&]() {
         span_of(a, (unsigned)ls, lrow, llo, lhi);
         ltab = a.tables + (size_t)lrow * a.max_pages;
-        lhead = (size_t)((lh * HG + hs) / a.subs) * a.head_bytes;
         lend = lh * line + pre[ls + 1];
         lnew = a.k_new ? a.n_kv[lrow] - 1 : 0xffffffffu;
     };
     // the table entry of the next tile's key `lane`, asked for one tile early
     const long long to_v = a.v - a.k;
-    unsigned lj = 0;
     auto look_up = [&]() {
         const unsigned t = (unsigned)(lg - lh * line - pre[ls]);
-        lj = llo / KEYS * KEYS + (t * R + r) * KEYS + lane;
-        lpage = NO_PAGE;
-        if (lane < KEYS && lj >= llo && lj < lhi) {
-            unsigned e;
-            place_of(a, lj, e, lslot);
-            lpage = ltab[e];
+#pragma unroll
+        for (int q = 0; q < SERVED; ++q) {
+            lj[q] = llo / KEYS * KEYS + (t * R + (first_w + q * apart) / HG) * KEYS + lane;
+            lpage[q] = NO_PAGE;
+            if (lane < KEYS && lj[q] >= llo && lj[q] < lhi) {
+                unsigned e;
+                place_of(a, lj[q], e, lslot[q]);
+                lpage[q] = ltab[e];
+            }
+        }
+    };
+    auto copy_tile = [&](int q, int w) {
+        const bool in = lpage[q] < a.n_pages;
+        const size_t head = (size_t)((lh * HG + w % HG) / a.subs) * a.head_bytes;
+        const long long off = in ? (long long)(((size_t)lpage[q] * a.pt + lslot[q]) * a.token_bytes + head) : -1;
+        const unsigned mask = __ballot_sync(0xffffffffu, in);
+        uint8_t *stage = ring_of(w) + lstage * stage_bytes;
+        if (lane == 0) masks_of(w)[lstage] = mask;
+        if (in && lj[q] == lnew) slots_of(w)[lstage] = off;
+        if (a.one_page && mask == (1u << KEYS) - 1) Tile::load_run(stage, a.k + __shfl_sync(0xffffffffu, off, 0), to_v, a, lane);
+        else Tile::load_rows(stage, off, a, lane);
+    };
+    auto advance = [&]() {
+        lstage = lstage + 1 == ns ? 0 : lstage + 1;
+        if (++lg < g1) {
+            if (lg == lend) {
+                next_row(ls, lh);
+                enter();
+            }
+            look_up();
         }
     };
     auto issue = [&]() {
         if (lg < g1) {
-            const bool in = lpage < a.n_pages;
-            const long long off = in ? (long long)(((size_t)lpage * a.pt + lslot) * a.token_bytes + lhead) : -1;
-            const unsigned mask = __ballot_sync(0xffffffffu, in);
-            uint8_t *stage = ring + lstage * stage_bytes;
-            if (lane == 0) masks[lstage] = mask;
-            if (in && lj == lnew) slots[lstage] = off;
-            if (a.one_page && mask == (1u << KEYS) - 1) Tile::load_run(stage, a.k + __shfl_sync(0xffffffffu, off, 0), to_v, a, lane);
-            else Tile::load_rows(stage, off, a, lane);
-            lstage = lstage + 1 == ns ? 0 : lstage + 1;
-            if (++lg < g1) {
-                if (lg == lend) {
-                    next_row(ls, lh);
-                    enter();
-                }
-                look_up();
-            }
+            copy_tile(0, first_w);
+            advance();
         }
         cp_commit();
     };
-    enter();
-    look_up();
+    int *status = reinterpret_cast<int *>(a.status);
+    constexpr int WAIT = (int)MOEARC_X_KV_WAIT;
+    if (SPLIT && warp >= warps) {
+        enter();
+        look_up();
+        for (unsigned phase = 1; lg < g1; advance()) {  // the first round waits for nothing
+#pragma unroll
+            for (int q = 0; q < SERVED; ++q) {
+                const int w = first_w + q * apart;
+                if (w >= warps) break;
+                const bool ok = lg - g0 < ns || tc::bar_wait(empty_of(w) + lstage, phase, abort, status, WAIT);
+                if (!__all_sync(0xffffffffu, ok)) {
+                    cp_commit();
+                    cp_wait<0>();
+                    return;
+                }
+                copy_tile(q, w);
+                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(full_of(w) + lstage)) : "memory");
+                __syncwarp();
+                if (lane == 0) tc::bar_arrive(full_of(w) + lstage);
+            }
+            if (lstage == ns - 1) phase ^= 1;
+        }
+        cp_commit();
+        cp_wait<0>();
+        return;
+    }
+    if constexpr (!SPLIT) {
+        enter();
+        look_up();
+    }
 
+    auto compute_sync = [&]() { asm volatile("barrier.cta.sync 1, %0;" ::"r"(warps * 32) : "memory"); };
     Tile tile;
     int s = s0, h = h0g, cstage = 0, ahead = ns - 1;
+    unsigned cphase = 0;
     for (int g = g0; g < g1; next_row(s, h)) {
         const int u0 = h * line + pre[s], u1 = h * line + pre[s + 1], first = g, end = min(u1, g1);
         unsigned row, lo, hi;
@@ -646,16 +709,21 @@ __global__ void __launch_bounds__(Tile::WARPS * 32, 1)
         const unsigned newest = a.k_new ? a.n_kv[row] - 1 : 0xffffffffu;
         tile.init(a.q + (size_t)s * a.q_stride + (size_t)h0 * D, heads, a, extra, lane);
         for (; g < end; ++g) {
-            for (; ahead >= 0; --ahead) issue();  // one a tile, ns before the first
-            ahead = 0;
-            if (ns == 3) cp_wait<2>();
-            else cp_wait<1>();
-            __syncwarp();
-            uint8_t *stage = ring + cstage * stage_bytes;
-            const unsigned live = masks[cstage], j0 = lo / KEYS * KEYS + ((unsigned)(g - u0) * R + r) * KEYS;
+            bool ok = true;
+            if constexpr (SPLIT) {
+                ok = __all_sync(0xffffffffu, tc::bar_wait(full_of(warp) + cstage, cphase, abort, status, WAIT));
+            } else {
+                for (; ahead >= 0; --ahead) issue();  // one a tile, ns before the first
+                ahead = 0;
+                if (ns == 3) cp_wait<2>();
+                else cp_wait<1>();
+                __syncwarp();
+            }
+            uint8_t *stage = ring_of(warp) + cstage * stage_bytes;
+            const unsigned live = ok ? masks_of(warp)[cstage] : 0, j0 = lo / KEYS * KEYS + ((unsigned)(g - u0) * R + r) * KEYS;
             if (newest >= j0 && newest - j0 < KEYS && (live >> (newest - j0) & 1)) {
                 const unsigned at = newest - j0;
-                const size_t dst = (size_t)slots[cstage];
+                const size_t dst = (size_t)slots_of(warp)[cstage];
                 const size_t src = (size_t)s * a.new_stride + (size_t)kvh * D;
                 Tile::round_row(a.k_new + src, stage, (int)at, sub == 0 ? a.k + dst : nullptr, a, lane);
                 Tile::round_row(a.v_new + src, stage, (int)(KEYS + at), sub == 0 ? a.v + dst : nullptr, a, lane);
@@ -663,7 +731,11 @@ __global__ void __launch_bounds__(Tile::WARPS * 32, 1)
             }
             if (live) tile.step(stage, live, a, extra, lane);
             __syncwarp();
-            cstage = cstage + 1 == ns ? 0 : cstage + 1;
+            if (SPLIT && lane == 0) tc::bar_arrive(empty_of(warp) + cstage);
+            if (++cstage == ns) {
+                cstage = 0;
+                cphase ^= 1;
+            }
         }
 
         // Close the row or its part: the head's warps are added into its first, which writes.
@@ -681,7 +753,7 @@ __global__ void __launch_bounds__(Tile::WARPS * 32, 1)
                 float *b = merge_of(r);
                 tile.each(lane, a, [&](int hd, int d, float &o) { b[hd * D + d] = o; }, [](int, float, float, bool) {});
             }
-            __syncthreads();
+            compute_sync();
             if (r == 0) {
                 if (lane < GP) {
                     float M = -INFINITY, sum = 0.f;
@@ -732,7 +804,7 @@ __global__ void __launch_bounds__(Tile::WARPS * 32, 1)
                 else if (hd < heads) out[(size_t)hd * D + d] = o * ff[hd];
             }, [](int, float, float, bool) {});
         }
-        if (R > 1) __syncthreads();  // the sums and accumulators are free for the next row
+        if (R > 1) compute_sync();  // the sums and accumulators are free for the next row
         else __syncwarp();
     }
 }
@@ -848,7 +920,7 @@ cudaError_t launch(moearc_ctx *c, const attn_plan &p, const attn_args &a) {
         return set_smem(k_attn_batch<Tile>, MAX_SMEM - 512);
     });
     if (e == cudaSuccess)
-        e = launch_pdl(k_attn_batch<Tile>, dim3((unsigned)p.grid), dim3((unsigned)p.warps * 32), (size_t)p.smem, c->stream, a, p.ns);
+        e = launch_pdl(k_attn_batch<Tile>, dim3((unsigned)p.grid), dim3((unsigned)(p.warps + (Tile::SPLIT ? (p.warps + 1) / 2 : 0)) * 32), (size_t)p.smem, c->stream, a, p.ns);
     if (e == cudaSuccess) e = attn_join_launch<Tile::GP>(c, p.grid, a);
     return e;
 }
