@@ -311,6 +311,16 @@ def test_attention_between_the_usual_head_sizes(ctx, D, kv):
     batch(ctx, lens, 20, 2, D, kv, 24, seed=D, begin=begin, fill=np.nan)
 
 
+@pytest.mark.parametrize("H, kvh, D", [(5, 5, 36), (8, 8, 64), (20, 5, 76), (14, 7, 80), (6, 2, 84), (24, 3, 128), (4, 1, 132), (16, 2, 252), (3, 3, 256)])
+def test_f32_attention_on_the_tensor_cores(ctx, H, kvh, D):
+    """f32 heads around the tiles' sizes: long and short rows together, one computing warp to eight with
+    their loading warps, pages that end inside a tile, windows, NaN outside the live keys, many rows."""
+    lens = [1300, 0, 129, 16, 5, 390, 1]
+    batch(ctx, lens, H, kvh, D, F32, 7, seed=D, sinks=True, new=True, pad=D % 3)
+    batch(ctx, lens, H, kvh, D, F32, 16, seed=D, begin=[3, 0, 0, 15, 5, 257, 0], fill=np.nan)
+    batch(ctx, [9] * 900, H, kvh, D, F32, 16, seed=D, new=True)
+
+
 def test_attention_windows(ctx):
     lens = [100, 40, 3, 7, 90, 12]
     batch(ctx, lens, 8, 2, 64, BF16, 16, begin=[70, 0, 2, 7, 89, 30], sinks=True, new=True)  # row 3 has nothing left, row 5's start is past its end
