@@ -249,7 +249,7 @@ def batch(ctx, lens, H, kvh, D, kv, pt, *, seed=0, begin=None, sinks=False, new=
     q, kn, vn = x[:, :H * D], x[:, H * D:(H + kvh) * D], x[:, (H + kvh) * D:(H + 2 * kvh) * D]
     sk = rng.standard_normal(H, np.float32) if sinks else None
     dx, out = ctx.upload_new(x), ctx.upload_new(np.full(n * H * D + 8, 7.5, np.float32))
-    scale = D ** -0.5 if scale is None else scale
+    usual, scale = scale is None, D ** -0.5 if scale is None else scale
     kw = dict(q_stride=width, new_stride=width, seqs=rows, kv_begin=None if begin is None else ctx.upload_new(np.array(begin, np.uint32)),
               sinks=None if sk is None else ctx.upload_new(sk))
     if new:
@@ -265,6 +265,8 @@ def batch(ctx, lens, H, kvh, D, kv, pt, *, seed=0, begin=None, sinks=False, new=
     rel = err and float(np.linalg.norm(got - want) / np.linalg.norm(want))
     print(f"attention {lens if len(lens) < 6 else len(lens)} {H}/{kvh} x {D} kv {kv}: max error {err:.2e} (bound {tol:.2e}), relative 2-norm {rel:.2e}")
     assert err <= tol
+    if usual:  # scores up to about 5, rounded (D + 8) times at random (5 sqrt(D + 8) EPS each, twice); exp and splits 2^-21
+        assert rel <= 2 * 5 * (D + 8) ** 0.5 * EPS + 2.0 ** -21
     for dev, host in ((p.c.k_pages, p.m.k), (p.c.v_pages, p.m.v)):  # the new tokens stored, nothing else written
         assert np.array_equal(ctx.download(dev[0], host.dtype, host[0].size), host[0].ravel())
     p.c.attn_decode(0, out, dx, n, H, scale, **kw)  # the same bits again
