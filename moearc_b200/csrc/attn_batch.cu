@@ -55,7 +55,7 @@ namespace {
 // multiple of 32, so that these reads meet 32 banks.
 //
 // 30 rows of up to 6000 tokens: 8 kv heads of 64 with 8 query heads each 114 us (319 on CUDA cores),
-// 4 heads of 128 with 8 each 149 (320), 1 of 256 with 16 140 (two passes over the keys), where the
+// 4 heads of 128 with 8 each 143 (320), 1 of 256 with 16 140 (two passes over the keys), where the
 // bytes alone take 74, 74 and 37. Bound by the instructions around the MMAs (two a side, each operand
 // taken apart by integer work as it leaves shared memory) and, at one CTA an SM, by their latency.
 
@@ -74,11 +74,9 @@ __device__ __forceinline__ void halves(float x, uint32_t &hi, uint32_t &lo) {
     lo = __float_as_uint(x - __uint_as_float(hi));
 }
 
-template <int D_>
+template <int D_, int KEYS_>
 struct tf32_tile {
-    // 16 keys a tile; of 256 channels 8, so that four warps' tiles fit where two did (30 rows of up to
-    // 6000: 139 us, 235 with 16; at 64 and 80 channels 8 keys in twice the warps lose: 134 and 123)
-    static constexpr int KEYS = D_ > 128 ? 8 : 16, NB = KEYS / 8, GP = 8, D = D_, WARPS = D_ > 128 ? 4 : 8;
+    static constexpr int KEYS = KEYS_, NB = KEYS / 8, GP = 8, D = D_, WARPS = D_ > 128 ? 4 : 8;
     static constexpr bool SPLIT = true;
     static constexpr int KROW = (D + 31) / 32 * 32 + 8, VROW = (D + 31) / 32 * 32 + 4;  // words
     static constexpr bool QREG = D <= 128;  // q's terms in registers, else in shared memory
@@ -878,10 +876,14 @@ bool cut_any(attn_plan &p, int n_heads, int n_kv, int D, int n_seq, int sms) {
 template <typename F>
 auto with_tile(bool mma, unsigned kv_type, unsigned D, int group, F &&f) {
     if (mma) {  // f32: attn_tc.cu has the 16-bit ones
-        if (D <= 64) return f((tf32_tile<64> *)nullptr);
-        if (D <= 80) return f((tf32_tile<80> *)nullptr);
-        if (D <= 128) return f((tf32_tile<128> *)nullptr);
-        return f((tf32_tile<256> *)nullptr);
+        // 16 keys a tile take fewer instructions a key, 8 let twice the warps' stages fit. So 8 above 128
+        // channels (16 query heads over 1 of 256, 30 rows of up to 6000: 140 us, 235 with 16), and above 80
+        // where each kv head is one unit (32 over 8 of 128: 247 and 275; 48 over 3, two units a kv head: 198
+        // and 167, its second unit's keys coming from L2); 16 below (64 over 8 of 64: 114, 134 with 8).
+        if (D <= 64) return f((tf32_tile<64, 16> *)nullptr);
+        if (D <= 80) return f((tf32_tile<80, 16> *)nullptr);
+        if (D <= 128) return group > 8 ? f((tf32_tile<128, 16> *)nullptr) : f((tf32_tile<128, 8> *)nullptr);
+        return f((tf32_tile<256, 8> *)nullptr);
     }
 #define CORE_CASE(T)                                                                                  \
     if (few_heads(D, group)) return f((core_tile<T, 1, 4> *)nullptr); \
