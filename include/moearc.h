@@ -722,7 +722,8 @@ int moearc_x_kv_status(moearc_ctx *c, const moearc_x_kv_cache *kv);
  * its slot (which no other row may hold: moearc_x_kv_grow sees to that) and attended as stored;
  * a row without tokens in range stores nothing. seqs: HOST list of distinct rows, or NULL for rows
  * 0 .. n_seq - 1; kv_begin: device [n_seq] or NULL (0); sinks: device [n_heads] or NULL. Queries,
- * and keys and values in range, are finite; what lies in pages outside the range may be anything.
+ * and keys and values in range, are finite, as are in f32 the scores and a row's sum of |v|; what lies
+ * in pages outside the range may be anything.
  * out overlaps no input. Results do not depend on timing: the same call gives the same bits. Enqueues two kernels (three
  * with seqs), no allocation; lengths and tables are read on the device, so a captured call follows them. */
 int moearc_x_attn_decode_batch(moearc_ctx *c, const moearc_x_kv_cache *kv, unsigned int layer, float *out, const float *q,

@@ -218,7 +218,7 @@ struct tf32_tile {
         uint32_t pa[NB][4];
 #pragma unroll
         for (int e = 0; e < 2 * NB; ++e) {
-            const float p = ex2(s[e] - base);
+            const float p = ex2(s[e] - base) * DOWN;
             l += p;
             pa[e >> 1][2 * (e & 1)] = tf32(p);
             pa[e >> 1][2 * (e & 1) + 1] = tf32(p - __uint_as_float(pa[e >> 1][2 * (e & 1)]));
@@ -448,7 +448,7 @@ struct core_tile {
         }
 #pragma unroll
         for (int h = 0; h < GP / 4; ++h) {
-            const float p = ex2(x[h] - (m[h] == -INFINITY ? 0.f : m[h]));
+            const float p = ex2(x[h] - (m[h] == -INFINITY ? 0.f : m[h])) * DOWN;
             l[h] += p;
             *reinterpret_cast<float2 *>(ps + 2 * (key * GP + cl * (GP / 4) + h)) = make_float2(p, p);
         }
@@ -784,7 +784,7 @@ __global__ void __launch_bounds__(Tile::WARPS * (Tile::SPLIT ? 48 : 32), 1)
                     if (a.sinks) {
                         const float sk = a.sinks[h0 + lane] * LOG2E, top = fmaxf(M, sk);
                         f = M == -INFINITY ? 0.f : ex2(M - top);
-                        sum = sum * f + (sk == -INFINITY ? 0.f : ex2(sk - top));
+                        sum = sum * f + (sk == -INFINITY ? 0.f : ex2(sk - top) * DOWN);
                     }
                     ff[lane] = sum == 0.f ? 0.f : f / sum;
                 }

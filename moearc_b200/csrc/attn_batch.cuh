@@ -9,9 +9,10 @@ namespace moearc {
 
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int MAX_SMEM = 227 * 1024;
-// A row's weights are taken against a reference that follows its maximum only once that is this much
-// above (in powers of two): most tiles then rescale nothing, and weights stay below 2^8.
-constexpr float LAZY = 8.f;
+// A row's weights are taken against a reference m that follows its maximum only once that is this much
+// above (in powers of two): most tiles then rescale nothing. A weight, in the sums and the records of
+// parts, is 2^(s - m - LAZY): one at most, so that no sum leaves the range before n times the largest value does.
+constexpr float LAZY = 8.f, DOWN = 1.f / 256;  // DOWN: 2^-LAZY
 
 struct attn_args {
     float *out;
@@ -181,7 +182,7 @@ static __global__ void __launch_bounds__(JOIN_THREADS, 4) k_attn_join(const __gr
         }
         sum = warp_sum(sum);
         if (lane == 0) {
-            sum += sk == -INFINITY ? 0.f : ex2(sk - M);
+            sum += sk == -INFINITY ? 0.f : ex2(sk - M) * DOWN;
             inv[hd] = sum == 0.f ? 0.f : 1.f / sum;
         }
     }

@@ -139,7 +139,7 @@ __global__ void __launch_bounds__(THREADS, DP == 64 ? 2 : 1)
     using S = tc_smem<DP>;
     const int D = FULL ? DP : a.D;
     constexpr int CH = DP / 8, TERMS = BF ? 3 : 2, NS = S::NS, LOADERS = S::LOADERS, MH = DP <= 128 ? 1 : DP / 128;
-    constexpr float PSCALE = BF ? 1.f : 64.f;
+    constexpr float PSCALE = BF ? 1.f : 16384.f;  // of the weights' terms
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = smem_raw + (((tc::sa(smem_raw) + 1023u) & ~1023u) - tc::sa(smem_raw));
     auto *bars = reinterpret_cast<uint64_t *>(smem + S::at_bar);
@@ -546,7 +546,7 @@ __global__ void __launch_bounds__(THREADS, DP == 64 ? 2 : 1)
                     const float p0 = ex2(s[h] - (m[h] == -INFINITY ? 0.f : m[h])), p1 = ex2(s[h + 1] - (m[h + 1] == -INFINITY ? 0.f : m[h + 1]));
                     l[h] += p0;
                     l[h + 1] += p1;
-                    terms<BF>(p0 * PSCALE, p1 * PSCALE, w[0][h / 2], w[1][h / 2], w[2][h / 2]);
+                    terms<BF>(p0 * (PSCALE * DOWN), p1 * (PSCALE * DOWN), w[0][h / 2], w[1][h / 2], w[2][h / 2]);
                 }
                 uint8_t *prow = smem + S::at_p + st * S::P + t * 64;
 #pragma unroll
@@ -567,7 +567,7 @@ __global__ void __launch_bounds__(THREADS, DP == 64 ? 2 : 1)
                     const float *x = red + (u & 1) * 4 * GP;
 #pragma unroll
                     for (int h = 0; h < GP; ++h) {
-                        l[h] = (x[h] + x[GP + h]) + (x[2 * GP + h] + x[3 * GP + h]);
+                        l[h] = ((x[h] + x[GP + h]) + (x[2 * GP + h] + x[3 * GP + h])) * DOWN;
                         for (int b = 0; b < MH; ++b) O[b][h] *= 1.f / PSCALE;
                     }
                     if (flags & WHOLE) {
@@ -580,7 +580,7 @@ __global__ void __launch_bounds__(THREADS, DP == 64 ? 2 : 1)
                             if (sk != -INFINITY) {
                                 const float top = fmaxf(m[h], sk);
                                 f = m[h] == -INFINITY ? 0.f : ex2(m[h] - top);
-                                sum = sum * f + ex2(sk - top);
+                                sum = sum * f + ex2(sk - top) * DOWN;
                             }
                             f = sum == 0.f ? 0.f : f / sum;
 #pragma unroll
