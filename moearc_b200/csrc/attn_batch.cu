@@ -202,7 +202,7 @@ struct tf32_tile {
                 s[2 * n + e] = in >> (8 * n + e) & 1 ? x : -INFINITY;
                 mt = fmaxf(mt, s[2 * n + e]);
             }
-        if (__any_sync(0xffffffffu, mt > m + LAZY)) {
+        if (__any_sync(0xffffffffu, mt - m > LAZY)) {
             mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
             mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 2));
             const float mn = fmaxf(m, mt), corr = ex2(m - (mn == -INFINITY ? 0.f : mn));
@@ -419,7 +419,7 @@ struct core_tile {
 #pragma unroll
         for (int h = 0; h < GP / 4; ++h) {
             x[h] = in ? x[h] * a.scale2 : -INFINITY;
-            up |= x[h] > m[h] + LAZY;
+            up |= x[h] - m[h] > LAZY;
         }
         if (__any_sync(0xffffffffu, up)) {
 #pragma unroll

@@ -15,8 +15,10 @@
 // of 64: 19 us (5). The tensor pipe is 9% busy: HBM bounds long rows, the chain from load to weights to
 // output short ones. On mma.sync the first two took 193 and 93 us.
 //
-// The 32 columns are the 16-bit terms of eight heads: three for bf16 (24 bits of q and of p), two
-// for f16. The tensor core sums a tile (8 MMAs) and the threads, now one a channel, add the columns
+// The 32 columns are the 16-bit terms of eight heads, three each of q and of p. f16's range is short: p's second
+// and third terms are 2^11 and 2^22 times as fine, so that a weight has 22 bits down to 2^-35 of its row's
+// largest (24 natural units of score) and the last of them at 2^-57; a row whose largest weights have
+// values of zero is made of the small ones. The tensor core sums a tile (8 MMAs) and the threads, now one a channel, add the columns
 // of a head to f32 registers, since its sums truncate and a long row's would show it.
 //
 // Two tiles are in flight or in use (one of 256 channels, its keys loaded again while its weights are
@@ -138,8 +140,8 @@ __global__ void __launch_bounds__(THREADS, DP == 64 ? 2 : 1)
     k_attn_tc(const __grid_constant__ attn_args a) {
     using S = tc_smem<DP>;
     const int D = FULL ? DP : a.D;
-    constexpr int CH = DP / 8, TERMS = BF ? 3 : 2, NS = S::NS, LOADERS = S::LOADERS, MH = DP <= 128 ? 1 : DP / 128;
-    constexpr float PSCALE = BF ? 1.f : 16384.f;  // of the weights' terms
+    constexpr int CH = DP / 8, TERMS = 3, NS = S::NS, LOADERS = S::LOADERS, MH = DP <= 128 ? 1 : DP / 128;
+    constexpr float PSCALE = BF ? 1.f : 32768.f;  // of the weights' terms
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = smem_raw + (((tc::sa(smem_raw) + 1023u) & ~1023u) - tc::sa(smem_raw));
     auto *bars = reinterpret_cast<uint64_t *>(smem + S::at_bar);
@@ -487,7 +489,8 @@ __global__ void __launch_bounds__(THREADS, DP == 64 ? 2 : 1)
                     float c[32];
                     tmem_ld32(tmem + 64 + (b * 2 + (i & 1)) * 32 + lanes, c);
 #pragma unroll
-                    for (int h = 0; h < GP; ++h) O[b][h] += BF ? c[h] + (c[8 + h] + c[16 + h]) : c[h] + c[8 + h];
+                    for (int h = 0; h < GP; ++h)
+                        O[b][h] += BF ? c[h] + (c[8 + h] + c[16 + h]) : fmaf(fmaf(c[16 + h], FINE, c[8 + h]), FINE, c[h]);
                 }
                 return true;
             };
@@ -517,11 +520,11 @@ __global__ void __launch_bounds__(THREADS, DP == 64 ? 2 : 1)
                     float c[32];
                     tmem_ld32(tmem + st * 32 + lanes, c);
 #pragma unroll
-                    for (int h = 0; h < GP; ++h) s[h] = live ? (BF ? c[h] + (c[8 + h] + c[16 + h]) : c[h] + c[8 + h]) * sc[h] : -INFINITY;
+                    for (int h = 0; h < GP; ++h) s[h] = live ? (c[h] + (c[8 + h] + c[16 + h])) * sc[h] : -INFINITY;
                 }
                 bool up = false;
 #pragma unroll
-                for (int h = 0; h < GP; ++h) up |= s[h] > m[h] + LAZY;
+                for (int h = 0; h < GP; ++h) up |= s[h] - m[h] > LAZY;
                 if (soft_any(up)) {
                     if (pending) {
                         ok = flush(i - 1) && ok;
@@ -540,18 +543,25 @@ __global__ void __launch_bounds__(THREADS, DP == 64 ? 2 : 1)
                         m[h] = mn;
                     }
                 }
-                uint32_t w[3][4];
 #pragma unroll
-                for (int h = 0; h < GP; h += 2) {
-                    const float p0 = ex2(s[h] - (m[h] == -INFINITY ? 0.f : m[h])), p1 = ex2(s[h + 1] - (m[h + 1] == -INFINITY ? 0.f : m[h + 1]));
-                    l[h] += p0;
-                    l[h + 1] += p1;
-                    terms<BF>(p0 * (PSCALE * DOWN), p1 * (PSCALE * DOWN), w[0][h / 2], w[1][h / 2], w[2][h / 2]);
+                for (int h = 0; h < GP; ++h) {
+                    const float p = ex2(s[h] - (m[h] == -INFINITY ? 0.f : m[h]));
+                    l[h] += p;
+                    s[h] = p * (PSCALE * DOWN);
                 }
                 uint8_t *prow = smem + S::at_p + st * S::P + t * 64;
 #pragma unroll
-                for (int r = 0; r < TERMS; ++r)
-                    *reinterpret_cast<uint4 *>(prow + ((r ^ (t >> 1 & 3)) << 4)) = make_uint4(w[r][0], w[r][1], w[r][2], w[r][3]);
+                for (int r = 0; r < TERMS; ++r) {  // a term of every head, then what it leaves
+                    uint32_t w[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        w[e] = pack<BF>(s[2 * e], s[2 * e + 1]);
+                        const float2 a = unpack<BF>(w[e]);
+                        s[2 * e] = rest<BF>(s[2 * e], a.x);
+                        s[2 * e + 1] = rest<BF>(s[2 * e + 1], a.y);
+                    }
+                    *reinterpret_cast<uint4 *>(prow + ((r ^ (t >> 1 & 3)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                }
                 fence_async();
                 tc::fence_before_sync();
                 tc::bar_arrive(pfull + st);

@@ -47,6 +47,29 @@ def queries(rows, H, D, first=8.0):
 SHAPES = [(8, 2, 64), (16, 2, 128), (6, 2, 80), (16, 1, 256), (4, 4, 20), (8, 1, 48)]
 
 
+@pytest.mark.parametrize("gap", [10, 15, 18, 20, 25, 30])
+@pytest.mark.parametrize("kv", [F16, BF16, F32])
+def test_weights_far_below_a_key_that_adds_nothing(ctx, kv, gap):
+    """One key `gap` above the others in score whose value is zero (an attention sink in the cache): the
+    output is the sum of the other weights alone, and keeps its own relative accuracy.
+
+    With X = gap + 6 the largest |score|: the scale's two roundings, the product's, the largest's and the
+    difference's are 5 X EPS of a weight (the high key's own product is exact); the others' scores, up to
+    5, are rounded (D + 8) times at random, twice; exponential and split 2^-21; the sums over n keys and
+    a join at random."""
+    for H, kvh, D in SHAPES:
+        for n, at in ((300, 0), (3000, 1700)):
+            def fill(k, v):
+                k[..., 0] = 0
+                k[:, at] = 0
+                k[:, at, :, 0] = gap / (8.0 * D ** -0.5)
+                v[:, at] = 0
+            got, want, _ = run(ctx, n, 2, H, kvh, D, kv, queries(2, H, D), fill)
+            rel = np.linalg.norm(got - want) / np.linalg.norm(want)
+            print(f"kv {kv} {H}/{kvh} x {D}, {n} keys, gap {gap}: relative 2-norm error {rel:.2e}")
+            assert rel <= (5 * (gap + 6) + 2 * 5 * (D + 8) ** 0.5 + 5 * (n / 8) ** 0.5) * EPS + 2.0 ** -21
+
+
 @pytest.mark.parametrize("kv", [BF16, F32])
 def test_values_of_large_magnitude(ctx, kv):
     """Values of 2^116 to 2^117 and scores that rise by seven powers of two half way along a row: no
