@@ -94,7 +94,8 @@ struct tf32_tile {
         const bool live = hr < heads;
         const float *p = q + (size_t)(live ? hr : 0) * a.D;
         if constexpr (!QREG) __syncwarp();
-#pragma unroll 4
+        // whole where q's terms are registers: an index known at run time puts the tile in local memory
+#pragma unroll(QREG ? D / 8 : 4)
         for (int kk = 0; kk < D / 8; ++kk) {
             uint32_t w[4];
 #pragma unroll
