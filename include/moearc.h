@@ -723,7 +723,10 @@ int moearc_x_kv_status(moearc_ctx *c, const moearc_x_kv_cache *kv);
  * a row without tokens in range stores nothing. seqs: HOST list of distinct rows, or NULL for rows
  * 0 .. n_seq - 1; kv_begin: device [n_seq] or NULL (0); sinks: device [n_heads] or NULL. Queries,
  * and keys and values in range, are finite, as are in f32 the scores and a row's sum of |v|; what lies
- * in pages outside the range may be anything.
+ * in pages outside the range may be anything. f32 arithmetic in effect, to within a few roundings: sums of products
+ * are f32, keys and values count with every bit, q and the softmax weights with 22 or more. (With an
+ * f16 cache: of a query's channels down to 2^-14 of its head's largest, of weights down to 2^-35 of their row's
+ * largest; smaller ones with fewer, to none at 2^-37 and 2^-57.)
  * out overlaps no input. Results do not depend on timing: the same call gives the same bits. Enqueues two kernels (three
  * with seqs), no allocation; lengths and tables are read on the device, so a captured call follows them. */
 int moearc_x_attn_decode_batch(moearc_ctx *c, const moearc_x_kv_cache *kv, unsigned int layer, float *out, const float *q,

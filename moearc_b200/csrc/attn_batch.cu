@@ -21,14 +21,14 @@
 //   cp.async stages of its own, which runs on across rows: no barrier in the loop, and the next
 //   row's keys are on their way before this row is finished. The tensor-core tiles' copies are issued by
 //   other warps (one for two), which hand stages over and back at mbarriers with a limit to every wait:
-//   the addresses of a tile's copies were a third of a computing warp's instructions (21 rows of up to
-//   2999, 20/5 heads of 80, f32: 52.6 -> 45.6 us). The CUDA cores' tile has 16 warps that hide them.
+//   the addresses of a tile's copies were a third of a computing warp's instructions. The CUDA cores' tile
+//   has 16 warps that hide them.
 // - 16-bit caches of 40 to 256 channels, a multiple of 8, have a kernel of their own on tcgen05
 //   (attn_tc.cu). Here, on the same line of tiles: f32 caches of 36 to 256 channels, a multiple of 4,
-//   on mma.sync with tf32 terms (tcgen05's tf32 would want keys and values split in two in shared
-//   memory, twice the bytes there); every other size, and pools off a 16-byte boundary, on CUDA cores.
-// - q, the softmax weights and f32 keys and values are two tf32 terms each there (22 to 23 bits).
-//   A tile's P V is summed from zero and added to the f32 accumulator by an ordinary add: the
+//   on mma.sync with tf32 terms (tcgen05's tf32 would want keys and values taken apart in shared
+//   memory, three times the bytes there); every other size, and pools off a 16-byte boundary, on CUDA cores.
+// - f32 keys and values keep all 24 bits there, as three tf32 terms; q and the softmax weights are two
+//   rounded ones (23 bits, a last place more than f32's own rounding of a product). A tile's P V is summed from zero and added to the f32 accumulator by an ordinary add: the
 //   tensor core's own accumulation truncates, which a long context would show.
 #include <algorithm>
 #include <cmath>
@@ -47,17 +47,18 @@ namespace {
 
 // ---- the tensor-core tile of f32 caches ---------------------------------------------------------
 //
-// head_dim up to D_, a multiple of 4. mma.sync m16n8k8 on tf32 terms: a key or value is its rounding to
-// 11 bits and the rest (two MMAs, 23 bits), q and the weights are two rounded terms on rows 0-7 and 8-15
-// of the A operand. Which channel (or key) stands for which k of an MMA is free as long as both
+// head_dim up to D_, a multiple of 4. mma.sync m16n8k8 on tf32 terms: a key or value is cut into 11, 11 and
+// 2 bits (three MMAs), q and the weights are two rounded terms on rows 0-7 and 8-15 of the A operand. Which channel (or key) stands for which k of an MMA is free as long as both
 // operands agree: k = j and j + 4 are channels 2 j and 2 j + 1 of an eight, read as one 8-byte load,
 // and keys 2 j and 2 j + 1, as the scores come out. Rows are 8 (keys) and 4 (values) words off a
 // multiple of 32, so that these reads meet 32 banks.
 //
-// 30 rows of up to 6000 tokens: 8 kv heads of 64 with 8 query heads each 114 us (319 on CUDA cores),
-// 4 heads of 128 with 8 each 143 (320), 1 of 256 with 16 140 (two passes over the keys), where the
-// bytes alone take 74, 74 and 37. Bound by the instructions around the MMAs (two a side, each operand
-// taken apart by integer work as it leaves shared memory) and, at one CTA an SM, by their latency.
+// 30 rows of up to 6000 tokens: 8 kv heads of 64 with 8 query heads each 107 us (318 on CUDA cores),
+// 4 heads of 128 with 8 each 125 (317), 1 of 256 with 16 159 (369; two passes over the keys), where the
+// bytes alone take 74, 74 and 37. Bound by the instructions around the MMAs (three a side, each operand
+// taken apart as it leaves shared memory) and, at one CTA an SM, by their latency. Keys and values in two terms
+// (23 bits: a row of one key did not return its value, and the largest finite values became
+// infinite) took 98, 110 and 140; the third as bf16 in MMAs of twice the k 105, 139 (its registers spill) and 177.
 
 __device__ __forceinline__ uint32_t tf32(float x) {
     uint32_t u;
@@ -68,10 +69,17 @@ __device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], 
     asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// x rounded to 11 bits, and what is left: 12 bits at most, of which the MMA drops the last.
-__device__ __forceinline__ void halves(float x, uint32_t &hi, uint32_t &lo) {
-    hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
-    lo = __float_as_uint(x - __uint_as_float(hi));
+// x rounded to 11 bits, the largest finite values to a finite one.
+__device__ __forceinline__ uint32_t tf32_finite(float x) {
+    return __float_as_uint(fminf(fmaxf(__uint_as_float(tf32(x)), __uint_as_float(0xff7fe000u)), __uint_as_float(0x7f7fe000u)));
+}
+// All 24 bits of x as tf32 terms of 11, 11 and 2 bits, cut rather than rounded: the largest finite values keep
+// finite terms.
+__device__ __forceinline__ void thirds(float x, uint32_t (&t)[3]) {
+    t[0] = __float_as_uint(x) & 0xffffe000u;
+    const float r = x - __uint_as_float(t[0]);
+    t[1] = __float_as_uint(r) & 0xffffe000u;
+    t[2] = __float_as_uint(r - __uint_as_float(t[1]));
 }
 
 template <int D_, int KEYS_>
@@ -102,7 +110,7 @@ struct tf32_tile {
             for (int e = 0; e < 2; ++e) {
                 const int d = 8 * kk + 2 * qd + e;
                 const float x = live && d < a.D ? p[d] : 0.f;
-                w[2 * e] = tf32(x);
+                w[2 * e] = tf32_finite(x);
                 w[2 * e + 1] = tf32(x - __uint_as_float(w[2 * e]));
             }
             if constexpr (QREG) {
@@ -178,11 +186,12 @@ struct tf32_tile {
 #pragma unroll
             for (int n = 0; n < NB; ++n) {
                 const float2 k = *reinterpret_cast<const float2 *>(ks + n * 8 * KROW + 8 * kk);
-                uint32_t h0, h1, l0, l1;
-                halves(k.x, h0, l0);
-                halves(k.y, h1, l1);
-                mma_tf32(c0[NB == 2 ? n : kk & 1], w, h0, h1);
-                mma_tf32(c1[NB == 2 ? n : kk & 1], w, l0, l1);
+                uint32_t x[3], y[3];
+                thirds(k.x, x);
+                thirds(k.y, y);
+                mma_tf32(c0[NB == 2 ? n : kk & 1], w, x[0], y[0]);
+                mma_tf32(c1[NB == 2 ? n : kk & 1], w, x[1], y[1]);
+                mma_tf32(c1[NB == 2 ? n : kk & 1], w, x[2], y[2]);
             }
         }
         // scores (in powers of two) of head lane / 4 for keys 2 qd, 2 qd + 1 (and 8 + 2 qd, 9 + 2 qd)
@@ -230,11 +239,12 @@ struct tf32_tile {
             float c[4] = {}, d[4] = {};
 #pragma unroll
             for (int n = 0; n < NB; ++n) {
-                uint32_t h0, h1, l0, l1;
-                halves(vs[n * 8 * VROW + 8 * i], h0, l0);
-                halves(vs[(n * 8 + 1) * VROW + 8 * i], h1, l1);
-                mma_tf32(c, pa[n], h0, h1);
-                mma_tf32(d, pa[n], l0, l1);
+                uint32_t x[3], y[3];
+                thirds(vs[n * 8 * VROW + 8 * i], x);
+                thirds(vs[(n * 8 + 1) * VROW + 8 * i], y);
+                mma_tf32(c, pa[n], x[0], y[0]);
+                mma_tf32(d, pa[n], x[1], y[1]);
+                mma_tf32(d, pa[n], x[2], y[2]);
             }
             o[i][0] += c[0] + (c[2] + (d[0] + d[2]));
             o[i][1] += c[1] + (c[3] + (d[1] + d[3]));
@@ -263,7 +273,7 @@ struct tf32_tile {
 // Values: a lane owns groups of four channels (lane + 32 i) of all GP heads, the weights come from
 // shared memory, each twice over: channels are multiplied in pairs (fma.rn.f32x2), which halves the
 // instructions, and those are what bounds it: 64 query heads over 8 of 64, f32, 30 rows of up to 6000
-// tokens 319 us, 2.8 times the tensor cores' tile.
+// tokens 318 us, three times the tensor cores' tile.
 
 // d += a b, two values at once.
 __device__ __forceinline__ void fma2(float2 &d, float2 a, float2 b) {
@@ -838,7 +848,9 @@ cudaError_t with_list(const unsigned *rows, unsigned n, F &&f) {
 
 // Whether the tensor cores serve a shape, where the pools' rows are 16-byte aligned: multiples of 8
 // channels of 16 bits and of 4 channels of f32, from the size at which half of the smallest tile is
-// used on. CUDA cores have the rest.
+// used on. CUDA cores have the rest. f32 heads without a group go the same way: they leave seven of eight rows of an
+// MMA empty and are level with CUDA cores or ahead of them (30 rows to 6000 and 200 to 500 tokens: 8 heads of 64 105
+// and 81 us, 156 and 120 on CUDA cores; 7 of 72 158 and 118, 154 and 122).
 bool tensor_dim(unsigned D, unsigned kv_type) { return D > 32 && D <= 256 && D % (kv_type == T_F32 ? 4 : 8) == 0; }
 // Of the latter, up to 128 channels whose kv heads serve four query heads at most take half the
 // arithmetic with tiles of four heads.
@@ -878,9 +890,9 @@ template <typename F>
 auto with_tile(bool mma, unsigned kv_type, unsigned D, int group, F &&f) {
     if (mma) {  // f32: attn_tc.cu has the 16-bit ones
         // 16 keys a tile take fewer instructions a key, 8 let twice the warps' stages fit. So 8 above 128
-        // channels (16 query heads over 1 of 256, 30 rows of up to 6000: 140 us, 235 with 16), and above 80
-        // where each kv head is one unit (32 over 8 of 128: 247 and 275; 48 over 3, two units a kv head: 198
-        // and 167, its second unit's keys coming from L2); 16 below (64 over 8 of 64: 114, 134 with 8).
+        // channels (16 query heads over 1 of 256, 30 rows of up to 6000: 159 us, 278 with 16), and above 80
+        // where each kv head is one unit (32 over 8 of 128: 217 and 260; 48 over 3, two units a kv head: 212
+        // and 188, its second unit's keys coming from L2); 16 below (64 over 8 of 64: 107, 155 with 8).
         if (D <= 64) return f((tf32_tile<64, 16> *)nullptr);
         if (D <= 80) return f((tf32_tile<80, 16> *)nullptr);
         if (D <= 128) return group > 8 ? f((tf32_tile<128, 16> *)nullptr) : f((tf32_tile<128, 8> *)nullptr);

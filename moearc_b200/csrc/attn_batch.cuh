@@ -101,10 +101,11 @@ __device__ __forceinline__ float2 unpack(uint32_t u) {
     else return __half22float2(*reinterpret_cast<const __half2 *>(&u));
 }
 // Two values as packed pairs of 16-bit terms: x = t0 + t1 + t2, each term the rounding of what
-// the ones before it leave.
+// the ones before it leave (the largest finite values' to a finite bf16).
 template <bool BF>
 __device__ __forceinline__ void terms(float x, float y, uint32_t &t0, uint32_t &t1, uint32_t &t2) {
-    t0 = pack<BF>(x, y);
+    const float most = __uint_as_float(0x7f7f0000u);
+    t0 = BF ? pack<BF>(fminf(fmaxf(x, -most), most), fminf(fmaxf(y, -most), most)) : pack<BF>(x, y);
     const float2 a = unpack<BF>(t0);
     t1 = pack<BF>(x - a.x, y - a.y);
     const float2 b = unpack<BF>(t1);

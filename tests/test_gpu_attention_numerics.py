@@ -86,3 +86,37 @@ def test_values_of_large_magnitude(ctx, kv):
         rel = np.abs(got - want).max() / np.abs(v).max()
         print(f"kv {kv} {H}/{kvh} x {D}: error over the largest value {rel:.2e}")
         assert rel <= 2 * (5 * (5 + 5) + 2 * (D + 8) + 600 / 8 + 64) * EPS + 2.0 ** -20
+
+
+def test_finite_ends_of_the_range_where_they_add_nothing(ctx):
+    """The largest finite values in live keys, in a channel where q is zero and behind a weight of zero, and in q
+    in a channel where the keys are (f16 caches: 2^10, as their terms of q are a head's fixed-point numbers)."""
+    for kv, most in ((F32, np.finfo(np.float32).max), (BF16, np.float32(2.0 ** 128 - 2.0 ** 120)), (F16, np.float32(65504.0))):
+        for H, kvh, D in SHAPES:
+            q = queries(2, H, D)
+            q[:, :, 1] = 0
+            q[:, :, 3] = 1024 if kv == F16 else np.finfo(np.float32).max
+            q[:, ::2, 3] *= -1
+
+            def fill(k, v):
+                k[:, ::3, :, 1] = most
+                k[:, 1::3, :, 1] = -most
+                k[:, 7, :, 0] = -3000.0
+                k[:, 7, :, 2:] = 0
+                k[:, :, :, 3] = 0
+                v[:, 7] = most
+                v[:, 7, :, ::2] = -most
+            got, want, _ = run(ctx, 200, 2, H, kvh, D, kv, q, fill)
+            assert np.isfinite(got).all(), (kv, H, kvh, D)
+            rel = np.linalg.norm(got - want) / np.linalg.norm(want)
+            # channel 0 adds 8 N(0, 1) D^-0.5 to the scores: up to 15 in all, five roundings of them
+            assert rel <= (5 * 15 + 2 * 5 * (D + 8) ** 0.5 + 25) * EPS + 2.0 ** -21
+
+
+@pytest.mark.parametrize("kv", [F32, F16, BF16])
+def test_a_row_of_one_key_is_its_value(ctx, kv):
+    """Its weight is one: the output is the stored value, every bit of it."""
+    for H, kvh, D in SHAPES + [(8, 8, 64), (32, 4, 128), (5, 5, 36), (24, 2, 96)]:
+        got, _, v = run(ctx, 1, 40, H, kvh, D, kv, queries(40, H, D), lambda k, v: None)
+        want = np.repeat(v[:, 0], H // kvh, axis=1).astype(np.float32)
+        assert np.array_equal(got, want), (kv, H, kvh, D)
