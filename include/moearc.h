@@ -741,9 +741,10 @@ int moearc_x_attn_decode_batch(moearc_ctx *c, const moearc_x_kv_cache *kv, unsig
  * logprob[i] = log softmax(x)[tokens[i]] (a token id not below n_vocab, as padding, gives 0);
  * entropy[i] = -sum softmax(x) log softmax(x); top_ids[i][0 .. k-1], top_logprobs[i][..] the k <= 32
  * largest, largest first, equal values by lowest id. tokens and logprob go together and may be
- * NULL, as may entropy; top_* only with k = 0. Logits of -inf are tokens with probability 0; a row
- * of them only has entropy 0 and log probabilities of -inf. A row with a NaN or +inf gives NaN, and
- * its alternatives rank a NaN with -inf. f32 arithmetic on any type; no allocation; one kernel. */
+ * NULL, as may entropy; top_* only with k = 0. An x of -inf (a logit of -inf, or a
+ * lowest finite one under a scale above 1) is a token with probability 0; a row of them only has entropy
+ * 0 and log probabilities of -inf. A row with an x of NaN or +inf gives NaN, and its alternatives rank a
+ * NaN with -inf. f32 arithmetic on any type; no allocation; one kernel. */
 int moearc_x_token_logprobs(moearc_ctx *c, const void *logits, unsigned int type, unsigned long row_stride,
                             unsigned int n_rows, unsigned int n_vocab, float scale, const unsigned int *tokens,
                             float *logprob, float *entropy, unsigned int k, unsigned int *top_ids, float *top_logprobs);

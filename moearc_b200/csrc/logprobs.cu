@@ -374,6 +374,9 @@ __global__ void __launch_bounds__(TH, (sizeof(T) == 4 ? 4 : 5) * 256 / TH) k_log
     }
     r.m *= scale;  // rounding keeps the order: this is the largest of the rounded products
     r.s *= scale;
+    // every product -inf: nothing here has a weight (the unscaled logits may be finite, a mask's lowest
+    // value, and equal); a sum that is NaN stays
+    if (r.m == -INFINITY) r.l = r.s = r.l * 0.f;
     const float mine = r.m;
 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
