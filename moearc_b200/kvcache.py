@@ -130,7 +130,9 @@ class KvCache:
                 n_live: DeviceBuffer | None = None) -> None:
         """Moves the pages in use below every free one; tables and counts in place, or into
         tables_out and refs_out (both)."""
-        t, r = tables_out or self.tables, refs_out or self.refs
+        if (tables_out is None) != (refs_out is None):
+            raise BadArgument("tables_out and refs_out go together")
+        t, r = (self.tables, self.refs) if tables_out is None else (tables_out, refs_out)
         t.require("compacted page table", 4 * self.max_seq * self.max_pages)
         r.require("compacted reference count", 4 * self.n_pages)
         if n_live is not None:
