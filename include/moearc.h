@@ -696,7 +696,9 @@ int moearc_x_kv_reset(moearc_ctx *c, const moearc_x_kv_cache *kv);
 int moearc_x_kv_grow(moearc_ctx *c, const moearc_x_kv_cache *kv, const unsigned int *seqs, const unsigned int *add,
                      unsigned int n);
 /* Row dst[i] (empty) becomes row src[i]: full pages are shared, a partly filled last page is copied
- * in every pool; with deep != 0 every page is copied (a hole's place in list order takes no page).
+ * in every pool; with deep != 0 every page is copied. A hole stays one: a deep fork passes over the
+ * free page whose turn it is at its place in list order, so as many free pages as the row has table entries,
+ * holes included, have to be there (MOEARC_X_KV_FULL otherwise), and the passed ones are still free.
  * dst rows are distinct and none of the src rows; a src may repeat. */
 int moearc_x_kv_fork(moearc_ctx *c, const moearc_x_kv_cache *kv, const unsigned int *src, const unsigned int *dst,
                      unsigned int n, int deep);

@@ -112,7 +112,8 @@ class KvCache:
         self.ctx._finish(self.ctx.lib.moearc_x_kv_grow(self.ctx.raw, self._d, _at(s), _at(a), len(s)), "kv_grow")
 
     def fork(self, src, dst, deep: bool = False) -> None:
-        """Empty row dst[i] becomes row src[i], sharing full pages (or, deep, copying every page)."""
+        """Empty row dst[i] becomes row src[i], sharing full pages (or, deep, copying every page; as many
+        free pages as the row has table entries, holes included, have to be there)."""
         s, t = _list(src), _list(dst)
         if len(s) != len(t):
             raise BadArgument(f"{len(s)} rows to fork onto {len(t)}")
