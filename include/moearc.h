@@ -729,6 +729,9 @@ int moearc_x_kv_status(moearc_ctx *c, const moearc_x_kv_cache *kv);
  * are f32, keys and values count with every bit, q and the softmax weights with 22 or more. (With an
  * f16 cache: of a query's channels down to 2^-14 of its head's largest, of weights down to 2^-35 of their row's
  * largest; smaller ones with fewer, to none at 2^-37 and 2^-57.)
+ * Tiles are numbered in 32 bits for the longest rows that the tables have room for: with n_seq x n_heads x
+ * (max_pages x page_tokens / 8 + 2) < 2^31 every call is served, above it -2 is the answer where a shape's tiles
+ * would be too many (16-bit caches of 40 to 256 channels have 128 keys a tile, others at least 8).
  * out overlaps no input. Results do not depend on timing: the same call gives the same bits. Enqueues two kernels (three
  * with seqs), no allocation; lengths and tables are read on the device, so a captured call follows them. */
 int moearc_x_attn_decode_batch(moearc_ctx *c, const moearc_x_kv_cache *kv, unsigned int layer, float *out, const float *q,
