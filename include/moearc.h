@@ -741,8 +741,8 @@ int moearc_x_attn_decode_batch(moearc_ctx *c, const moearc_x_kv_cache *kv, unsig
 
 /* ---- log probabilities (logprobs.cu; no counterpart in the reference) ------------------------
  * For each of n_rows rows of logits (type F32, F16 or BF16; row i at i * row_stride elements,
- * n_vocab <= row_stride of them used), with x = scale * logit (scale, one over the temperature,
- * in 1e-30 .. 1e30):
+ * n_vocab <= row_stride of them used; n_rows <= 2^26, n_vocab <= 2^30), with x = scale * logit (scale,
+ * one over the temperature, in 1e-30 .. 1e30):
  * logprob[i] = log softmax(x)[tokens[i]] (a token id not below n_vocab, as padding, gives 0);
  * entropy[i] = -sum softmax(x) log softmax(x); top_ids[i][0 .. k-1], top_logprobs[i][..] the k <= 32
  * largest, largest first, equal values by lowest id. tokens and logprob go together and may be

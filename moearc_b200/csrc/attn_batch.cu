@@ -28,7 +28,8 @@
 //   on mma.sync with tf32 terms (tcgen05's tf32 would want keys and values taken apart in shared
 //   memory, three times the bytes there); every other size, and pools off a 16-byte boundary, on CUDA cores.
 // - f32 keys and values keep all 24 bits there, as three tf32 terms; q and the softmax weights are two
-//   rounded ones (23 bits, a last place more than f32's own rounding of a product). A tile's P V is summed from zero and added to the f32 accumulator by an ordinary add: the
+//   rounded ones (23 bits, a last place more than f32's own rounding of a product). A tile's P V is
+//   summed from zero and added to the f32 accumulator by an ordinary add: the
 //   tensor core's own accumulation truncates, which a long context would show.
 #include <algorithm>
 #include <cmath>
@@ -48,7 +49,8 @@ namespace {
 // ---- the tensor-core tile of f32 caches ---------------------------------------------------------
 //
 // head_dim up to D_, a multiple of 4. mma.sync m16n8k8 on tf32 terms: a key or value is cut into 11, 11 and
-// 2 bits (three MMAs), q and the weights are two rounded terms on rows 0-7 and 8-15 of the A operand. Which channel (or key) stands for which k of an MMA is free as long as both
+// 2 bits (three MMAs), q and the weights are two rounded terms on rows 0-7 and 8-15 of the A operand.
+// Which channel (or key) stands for which k of an MMA is free as long as both
 // operands agree: k = j and j + 4 are channels 2 j and 2 j + 1 of an eight, read as one 8-byte load,
 // and keys 2 j and 2 j + 1, as the scores come out. Rows are 8 (keys) and 4 (values) words off a
 // multiple of 32, so that these reads meet 32 banks.

@@ -9,7 +9,7 @@
 //   p = 2^(S - m), thread = key  eight heads a thread, from tensor memory
 //   O [channels x 32] = V' P     V as it was loaded (channel-major) as the A operand, P from the threads
 //
-// Measured: 3 rows of up to 100001 tokens, 8 heads of 128, f16, 1.08 GB: 171 us, 6.3 TB/s of a measured 6.56
+// Measured: 3 rows of up to 100001 tokens, 8 heads of 128, f16, 1.08 GB: 172 us, 6.3 TB/s of a measured 6.56
 // (164 us); 64 rows of up to 4096, 4 heads of 128, bf16, 362 MB: 71 us (55), of which about 12 are the start
 // (lengths, tables, the first tile's way through the roles) and the join; 120 rows of 128 tokens, 8 heads
 // of 64: 19 us (5). The tensor pipe is 9% busy: HBM bounds long rows, the chain from load to weights to
@@ -18,8 +18,9 @@
 // The 32 columns are the 16-bit terms of eight heads, three each of q and of p. f16's range is short: p's second
 // and third terms are 2^11 and 2^22 times as fine, so that a weight has 22 bits down to 2^-35 of its row's
 // largest (24 natural units of score) and the last of them at 2^-57; a row whose largest weights have
-// values of zero is made of the small ones. The tensor core sums a tile (8 MMAs) and the threads, now one a channel, add the columns
-// of a head to f32 registers, since its sums truncate and a long row's would show it.
+// values of zero is made of the small ones. (200 rows of up to 500, 64/8 x 64, f16: 57 us, 54 with two plain
+// terms.) The tensor core sums a tile (8 MMAs) and the threads, now one a channel, add the columns of a
+// head to f32 registers, since its sums truncate and a long row's would show it.
 //
 // Two tiles are in flight or in use (one of 256 channels, its keys loaded again while its weights are
 // worked out: 16 heads over 1 of 256 channels, 30 rows of up to 6000, 50 us, 94 on mma.sync). They are loaded by 16-byte asynchronous copies, two warps a
